@@ -1,0 +1,162 @@
+"""ctypes binding of the block operators in libgfield.so (include/gfblock.h)
+and the checks their Python entry points share."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from guass_b200 import _lib
+
+GF_F16 = 2
+GF_FLAG_TIMEOUT = 0x10
+ACTIVATIONS = {"gelu": 0, "silu": 1}
+DTYPES = {torch.float32: _lib.GF_F32, torch.bfloat16: _lib.GF_BF16, torch.float16: GF_F16}
+
+# Every symbol include/gfblock.h declares.
+EXPORTED = ("gf_gated_ff_workspace_bytes", "gf_gated_ff_forward", "gf_gated_ff_backward", "gf_dropout",
+            "gf_quantize_rows", "gf_int8_product_workspace_bytes", "gf_int8_matmul", "gf_block_status")
+
+
+class GfDropoutRule(ctypes.Structure):
+    _fields_ = [
+        ("p", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("seed_ptr", ctypes.c_void_p),
+        ("site", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class GfGatedFf(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("in_features", ctypes.c_int64),
+        ("hidden", ctypes.c_int64),
+        ("out_features", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("dropout", GfDropoutRule),
+        ("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64),
+        ("w_in", ctypes.c_void_p), ("ld_w_in", ctypes.c_int64),
+        ("b_in", ctypes.c_void_p),
+        ("w_out", ctypes.c_void_p), ("ld_w_out", ctypes.c_int64),
+        ("b_out", ctypes.c_void_p),
+        ("u", ctypes.c_void_p),
+        ("h", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ld_y", ctypes.c_int64),
+        ("dy", ctypes.c_void_p), ("ld_dy", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dw_in", ctypes.c_void_p),
+        ("db_in", ctypes.c_void_p),
+        ("dw_out", ctypes.c_void_p),
+        ("db_out", ctypes.c_void_p),
+    ]
+
+
+class GfInt8Product(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("a", ctypes.c_void_p), ("ld_a", ctypes.c_int64),
+        ("b", ctypes.c_void_p), ("ld_b", ctypes.c_int64),
+        ("a_scale", ctypes.c_void_p),
+        ("b_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64),
+    ]
+
+
+_ready = None
+
+
+def lib() -> ctypes.CDLL:
+    """libgfield.so with the block operators' signatures."""
+    global _ready
+    if _ready is not None:
+        return _ready
+    L = _lib.lib()
+    i64, i32, ptr, size = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_size_t
+    ff = ctypes.POINTER(GfGatedFf)
+    L.gf_gated_ff_workspace_bytes.argtypes = [ff, ctypes.c_int]
+    L.gf_gated_ff_workspace_bytes.restype = size
+    for fn in (L.gf_gated_ff_forward, L.gf_gated_ff_backward):
+        fn.argtypes = [ff, ptr, size, ptr]
+        fn.restype = ctypes.c_int
+    L.gf_dropout.argtypes = [i64, i64, i32, ctypes.POINTER(GfDropoutRule), ptr, i64, i64, ptr, i64, i64, ptr, ptr]
+    L.gf_dropout.restype = ctypes.c_int
+    L.gf_quantize_rows.argtypes = [i64, i64, i32, ptr, i64, ptr, i64, ptr, ptr]
+    L.gf_quantize_rows.restype = ctypes.c_int
+    prod = ctypes.POINTER(GfInt8Product)
+    L.gf_int8_product_workspace_bytes.argtypes = [prod]
+    L.gf_int8_product_workspace_bytes.restype = size
+    L.gf_int8_matmul.argtypes = [prod, ptr, size, ptr]
+    L.gf_int8_matmul.restype = ctypes.c_int
+    L.gf_block_status.argtypes = [ptr, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
+    L.gf_block_status.restype = ctypes.c_int
+    _ready = L
+    return L
+
+
+def device_flags(device="cuda", reset: bool = False) -> int:
+    """Condition bits the block operators set on ``device`` since the last
+    reset (GF_FLAG_TIMEOUT: an output is not valid).  Synchronises the
+    current stream."""
+    flags = ctypes.c_uint32(0)
+    with torch.cuda.device(device):
+        _lib.check(lib().gf_block_status(torch.cuda.current_stream().cuda_stream, int(reset), ctypes.byref(flags)))
+    return flags.value
+
+
+def require(cond: bool, message: str, kind=ValueError) -> None:
+    if not cond:
+        raise kind(message)
+
+
+def check_tensor(name: str, t, dtypes, device=None) -> None:
+    """A CUDA tensor of one of ``dtypes`` (and on ``device``)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t)!r}")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} must be a CUDA tensor (there is no CPU implementation), got {t.device}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the input on {device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def on_device(t: torch.Tensor):
+    """Context that makes the tensor's device current."""
+    return torch.cuda.device(t.device)
+
+
+def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as [rows, cols] with unit column stride and rows that do not
+    overlap: a view where its strides allow one, else a copy."""
+    v = t.reshape(-1, cols)
+    if cols > 1 and v.stride(1) != 1 or v.shape[0] > 1 and v.stride(0) < cols:
+        v = v.contiguous()
+    return v
+
+
+def ld(v: torch.Tensor) -> int:
+    """Leading dimension of a [rows, cols] view."""
+    return v.stride(0) if v.shape[0] > 1 else v.shape[1]
+
+
+def fill_rule(rule: GfDropoutRule, p: float, seed, site: int, device) -> None:
+    """``seed``: an int, or a one-element int64 CUDA tensor that the kernel reads."""
+    p = float(p)
+    require(0.0 <= p < 1.0, f"dropout probability must be in [0, 1), got {p}")
+    site = int(site)
+    require(0 <= site < 1 << 32, f"site must be in [0, 2**32), got {site}")
+    rule.p, rule.site = p, site
+    if isinstance(seed, torch.Tensor):
+        check_tensor("seed", seed, (torch.int64,), device)
+        require(seed.numel() == 1, f"a seed tensor has one element, got {tuple(seed.shape)}")
+        rule.seed_ptr = seed.data_ptr()
+    else:
+        rule.seed = int(seed) & 0xFFFFFFFFFFFFFFFF

@@ -15,8 +15,8 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
-SOURCES = [PKG / "csrc" / "gfield.cu"]
-HEADERS = [ROOT / "include" / "gfield.h"]
+SOURCES = [PKG / "csrc" / "gfield.cu", PKG / "csrc" / "gfblock.cu"]
+HEADERS = [ROOT / "include" / "gfield.h", ROOT / "include" / "gfblock.h", PKG / "csrc" / "tc100.cuh"]
 LIB = PKG / "libgfield.so"
 # debug build: every shape-derived global access bounds-checked (GF_FLAG_BOUNDS);
 # load it instead of the release library with GUASS_B200_LIB=<path>
@@ -25,9 +25,12 @@ LIB_CHECK = PKG / "libgfield_check.so"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xptxas", "-warn-spills",
 ]
+# sources whose debug build differs (GF_CHECK); the others share one object
+CHECKED = {"gfield.cu"}
+OBJECTS = PKG / "build"
 
 
 def nvcc() -> str:
@@ -36,21 +39,42 @@ def nvcc() -> str:
     return str(cand) if cand.exists() else "nvcc"
 
 
+def _newer(target: Path, inputs) -> bool:
+    """True when ``target`` is missing or older than one of ``inputs``."""
+    return not target.exists() or any(p.stat().st_mtime > target.stat().st_mtime for p in inputs)
+
+
 def needs_build(lib: Path = LIB) -> bool:
-    if not lib.exists():
-        return True
-    t = lib.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
+    return _newer(lib, SOURCES + HEADERS)
+
+
+def _object(src: Path, check: bool) -> Path:
+    return OBJECTS / (src.stem + ("_check.o" if check and src.name in CHECKED else ".o"))
 
 
 def build(force: bool = False, verbose: bool = False, check: bool = False) -> Path:
-    """Build the release library (or, with ``check``, the bounds-checked one)."""
+    """Build the release library (or, with ``check``, the bounds-checked one):
+    one object per source, compiled side by side and kept for the next build."""
     lib = LIB_CHECK if check else LIB
     if not force and not needs_build(lib):
         return lib
+    OBJECTS.mkdir(exist_ok=True)
+    jobs = []
+    for src in SOURCES:
+        obj = _object(src, check)
+        if force or _newer(obj, [src, *HEADERS]):
+            tmp = obj.with_suffix(".tmp.o")
+            cmd = [nvcc(), *NVCC_FLAGS, *(["-DGF_CHECK"] if check and src.name in CHECKED else []),
+                   f"-I{ROOT / 'include'}", "-c", str(src), "-o", str(tmp)]
+            if verbose:
+                print(" ".join(cmd), file=sys.stderr)
+            jobs.append((subprocess.Popen(cmd), cmd, tmp, obj))
+    for proc, cmd, tmp, obj in jobs:
+        if proc.wait() != 0:
+            raise subprocess.CalledProcessError(proc.returncode, cmd)
+        os.replace(tmp, obj)
     tmp = lib.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, *(["-DGF_CHECK"] if check else []), f"-I{ROOT / 'include'}", *map(str, SOURCES),
-           "-o", str(tmp), "-lcudart"]
+    cmd = [nvcc(), *NVCC_FLAGS, "-shared", *(str(_object(s, check)) for s in SOURCES), "-o", str(tmp), "-lcudart"]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)

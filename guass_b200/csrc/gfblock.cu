@@ -1,0 +1,1466 @@
+// Transformer-block operators for B200 (sm_100a): the gated feed-forward
+// block with its backward, counter-based dropout, and the product in 8-bit
+// integers.  C ABI: include/gfblock.h.
+//
+// All matrix products run on one persistent, warp-specialised tcgen05 kernel
+// (gemm_kernel) whose epilogues hold the rest of each operator.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <nvtx3/nvToolsExt.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "gfblock.h"
+#include "tc100.cuh"
+
+namespace gf {
+gf_status fail(gf_status s, const char* fmt, ...) __attribute__((format(printf, 2, 3)));  // gfield.cu
+}
+
+namespace gfb {
+
+using gf::fail;
+
+struct Range {
+  explicit Range(const char* name) { nvtxRangePushA(name); }
+  ~Range() { nvtxRangePop(); }
+};
+
+constexpr int64_t kMaxDim = (int64_t(1) << 31) - 512;  // sizes stay in int32 after rounding up to a tile
+
+template <typename I>
+constexpr I round_up(I v, I m) {
+  return (v + m - 1) / m * m;
+}
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+__device__ uint32_t g_status;  // GF_FLAG_TIMEOUT, sticky (gf_block_status)
+
+// ---------------------------------------------------------------------------
+// element types
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+  else return __half2float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(v);
+  else return __float2half_rn(v);
+}
+// two 16-bit elements in a register, the first in the low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+
+// ---------------------------------------------------------------------------
+// Philox-4x32-10 (Salmon et al., SC 2011): ten rounds of two 32x32 -> 64-bit
+// products, the words swapped and the two halves of the key xored in; the key
+// steps by the two Weyl constants.
+
+struct DropArgs {
+  uint64_t seed;
+  const uint64_t* seed_ptr;
+  uint32_t site;
+  uint32_t threshold;  // keep when the word is at least this
+  float scale;
+  int32_t on;
+};
+
+struct Philox {
+  uint32_t k0, k1, site;
+  __device__ __forceinline__ Philox(const DropArgs& d) {
+    const uint64_t s = d.seed_ptr ? *d.seed_ptr : d.seed;
+    k0 = (uint32_t)s;
+    k1 = (uint32_t)(s >> 32);
+    site = d.site;
+  }
+  // the four words of elements (row, 4 * block .. 4 * block + 3)
+  __device__ __forceinline__ uint4 operator()(uint32_t block, uint64_t row) const {
+    uint32_t c0 = block, c1 = (uint32_t)row, c2 = site, c3 = (uint32_t)(row >> 32);
+    uint32_t a = k0, b = k1;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+      c0 = (uint32_t)(p1 >> 32) ^ c1 ^ a;
+      c2 = (uint32_t)(p0 >> 32) ^ c3 ^ b;
+      c1 = (uint32_t)p1;
+      c3 = (uint32_t)p0;
+      a += 0x9E3779B9u;
+      b += 0xBB67AE85u;
+    }
+    return make_uint4(c0, c1, c2, c3);
+  }
+};
+
+DropArgs drop_args(const gf_dropout_rule& r) {
+  DropArgs d{};
+  d.seed = r.seed;
+  d.seed_ptr = r.seed_ptr;
+  d.site = r.site;
+  double t = r.p * 4294967296.0;
+  t = __builtin_rint(t);
+  d.threshold = t >= 4294967295.0 ? 0xFFFFFFFFu : (uint32_t)t;
+  d.scale = (float)(1.0 / (1.0 - r.p));
+  d.on = r.p > 0.0;
+  return d;
+}
+
+gf_status check_rule(const char* who, const gf_dropout_rule& r) {
+  if (!(r.p >= 0.0 && r.p < 1.0)) return fail(GF_ERR_INVALID_ARG, "%s: dropout p must be in [0, 1)", who);
+  if (r.reserved != 0) return fail(GF_ERR_INVALID_ARG, "%s: reserved fields must be 0", who);
+  if (reinterpret_cast<uintptr_t>(r.seed_ptr) & 7u)
+    return fail(GF_ERR_INVALID_ARG, "%s: seed_ptr must be 8-byte aligned", who);
+  return GF_OK;
+}
+
+// ---------------------------------------------------------------------------
+// activations: value and slope
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float g) {
+  if constexpr (ACT == GF_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
+  else return g / (1.0f + expf(-g));
+}
+template <int ACT>
+__device__ __forceinline__ void act_both(float g, float& value, float& slope) {
+  if constexpr (ACT == GF_ACT_GELU) {
+    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
+    value = g * cdf;
+    slope = cdf + g * 0.39894228f * expf(-0.5f * g * g);
+  } else {
+    const float sig = 1.0f / (1.0f + expf(-g));
+    value = g * sig;
+    slope = sig * (1.0f + g * (1.0f - sig));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The product kernel.  D[m, n] = sum_k A(m, k) B(n, k) on 128 x bn tiles:
+//  warp 0      TMA producer: 64 k (128 bytes) of both operands per stage
+//  warp 1      issues tcgen05.mma into one of two TMEM accumulators
+//  warps 2-9   epilogue of the other accumulator (warp w reads TMEM lanes
+//              32 * (w % 4) onwards; the two warps of a quarter take the
+//              32-column chunks in turn)
+// Each CTA walks over tiles (and K ranges) with a stride of the grid.
+
+constexpr int kTileM = 128;
+constexpr int kMaxN = 256;
+constexpr int kStages = 4;
+constexpr int kABytes = kTileM * 128;
+constexpr int kStageBytes = kABytes + kMaxN * 128;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kPitch = 80;                        // staging: 64 bytes of each of a warp's 32 rows, spread over the banks
+constexpr int kWarpStage = 32 * kPitch + 2 * 32 * 4;  // and two vectors of 32 floats (bias, scales)
+constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kWarpStage + 256;
+constexpr uint32_t kTmemCols = 512;
+
+enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
+
+struct alignas(64) GemmParams {
+  CUtensorMap ma, mb;
+  int32_t M, N;                // rows and columns of the result (gated: columns of h, without padding)
+  int32_t tiles_m, tiles_n, splits, kb_total, kb_split;
+  int32_t bn;                  // columns of the MMA
+  int32_t cols;                // columns of the result per tile: bn, or bn / 2 (gated: value and gate side by side)
+  int32_t a_mn, b_mn;          // operand is M/N-contiguous
+  int32_t gate_row;            // gated: row of B where the gate half starts
+  uint32_t idesc, tx_bytes;
+  int32_t seg_pad, seg;        // result rows come in two runs of `seg` rows, the second starting at seg_pad (0: one run)
+  int32_t vec_out;             // rows of out are 16-byte aligned and whole 16-byte pieces
+  int64_t ld_out;
+  void* out;                   // STORE, INT8: result; GATED: h; GATED_BWD: du
+  float* partial;              // splits > 1: [splits][M][ld_partial]
+  int64_t ld_partial;
+  const void* bias;            // [N] (gated: [2 N])
+  void* u;                     // GATED: written when not null; GATED_BWD: read
+  int32_t hp;                  // gated: padded hidden size
+  int32_t bias_dtype;
+  const float* a_scale;
+  const float* b_scale;
+  DropArgs drop;
+};
+
+struct Pipe {  // barriers and the abort flag, in shared memory
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint32_t tmem, abort;
+};
+
+// Writes 64 bytes of each of this warp's 32 rows: lane = row in `v`, to rows
+// of `ld` bytes at `dst`, through the staging rows so that four lanes write
+// one row's 64 bytes.  `rows` rows and `bytes` bytes of each are written.
+template <int ES>
+__device__ __forceinline__ void store_rows(char* stage, const uint32_t (&v)[16], char* dst, int64_t ld, int rows,
+                                           int bytes, bool vec) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint4*>(stage + lane * kPitch + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2), b = (lane & 3) * 16;
+      if (r < rows && b < bytes)
+        *reinterpret_cast<uint4*>(dst + r * ld + b) = *reinterpret_cast<const uint4*>(stage + r * kPitch + b);
+    }
+  } else {
+    constexpr int per_row = 64 / ES;
+    for (int i = lane; i < 32 * per_row; i += 32) {
+      const int r = i / per_row, b = (i % per_row) * ES;
+      if (r < rows && b < bytes) {
+        if constexpr (ES == 2)
+          *reinterpret_cast<uint16_t*>(dst + r * ld + b) = *reinterpret_cast<const uint16_t*>(stage + r * kPitch + b);
+        else
+          *reinterpret_cast<uint32_t*>(dst + r * ld + b) = *reinterpret_cast<const uint32_t*>(stage + r * kPitch + b);
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// The reverse for reading: four lanes load one row's 64 bytes (16-byte aligned
+// rows), each lane then holds its own row.  Split in two so that the loads of
+// a chunk are in flight while the previous one is computed.
+__device__ __forceinline__ void fetch_rows(uint4 (&v)[4], const char* src, int64_t ld, int rows) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 2), b = (lane & 3) * 16;
+    v[i] = r < rows ? *reinterpret_cast<const uint4*>(src + r * ld + b) : make_uint4(0, 0, 0, 0);
+  }
+}
+__device__ __forceinline__ void turn_rows(char* stage, uint4 (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint4*>(stage + (8 * i + (lane >> 2)) * kPitch + (lane & 3) * 16) = v[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(stage + lane * kPitch + 16 * i);
+  __syncwarp();
+}
+
+struct Tile {
+  int m0, n0, split, kb0, kb1;
+};
+__device__ __forceinline__ Tile tile_of(const GemmParams& p, int64_t item) {
+  Tile t;
+  const int n = (int)(item % p.tiles_n);
+  const int64_t rest = item / p.tiles_n;
+  t.m0 = (int)(rest % p.tiles_m) * kTileM;
+  t.split = (int)(rest / p.tiles_m);
+  t.n0 = n * p.cols;
+  t.kb0 = t.split * p.kb_split;
+  t.kb1 = min(t.kb0 + p.kb_split, p.kb_total);
+  return t;
+}
+
+template <int EPI, typename T, int ACT, bool DROP>
+struct EpilogueWarp {
+  const GemmParams& p;
+  char* stage;
+  float* vec0;  // two vectors of 32 floats behind the staging rows
+  float* vec1;
+  Philox rng;
+  const int lane;
+
+  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* s)
+      : p(p_), stage(s), vec0(reinterpret_cast<float*>(s + 32 * kPitch)), vec1(vec0 + 32), rng(p_.drop),
+        lane(threadIdx.x & 31) {}
+
+  // one 32-column chunk at result column n of rows m .. m + 31
+  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int c, uint4 (&uv)[4], uint4 (&ug)[4]) {
+    const int n = t.n0 + c;
+    const int rows = min(32, p.M - m);
+    if constexpr (EPI == EPI_STORE) {
+      uint32_t d[32];
+      tc::tmem_load32(d, acc + c);
+      tc::tmem_wait();
+      if (p.splits > 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = d[16 * h + i];
+          char* dst = reinterpret_cast<char*>(p.partial + ((int64_t)t.split * p.M + m) * p.ld_partial + n + 16 * h);
+          store_rows<4>(stage, v, dst, 4 * p.ld_partial, rows, 64, true);
+        }
+        return;
+      }
+      bias_vector(n, p.N - n, p.bias, vec0);
+      uint32_t v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = pack2<T>(__uint_as_float(d[2 * i]) + vec0[2 * i], __uint_as_float(d[2 * i + 1]) + vec0[2 * i + 1]);
+      store_result<2>(v, m, n, rows, min(64, 2 * (p.N - n)));
+    } else if constexpr (EPI == EPI_INT8) {
+      uint32_t d[32];
+      tc::tmem_load32(d, acc + c);
+      tc::tmem_wait();
+      bias_vector(n, p.N - n, p.bias, vec0);
+      __syncwarp();
+      vec1[lane] = n + lane < p.N ? p.b_scale[n + lane] : 0.0f;
+      __syncwarp();
+      const float s = lane < rows ? p.a_scale[m + lane] : 0.0f;
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = (float)(int)d[i] * s * vec1[i] + vec0[i];
+      if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(f[16 * h + i]);
+          store_result<4>(v, m, n + 16 * h, rows, min(64, 4 * (p.N - n - 16 * h)));
+        }
+      } else {
+        uint32_t v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        store_result<2>(v, m, n, rows, min(64, 2 * (p.N - n)));
+      }
+    } else if constexpr (EPI == EPI_GATED) {
+      uint32_t a[32], g[32];
+      tc::tmem_load32(a, acc + c);
+      tc::tmem_load32(g, acc + p.cols + c);
+      tc::tmem_wait();
+      const int left = p.N - n;  // columns before the padding
+      bias_vector(n, left, p.bias, vec0);
+      bias_vector(p.N + n, left, p.bias, vec1);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        a[i] = __float_as_uint(__uint_as_float(a[i]) + vec0[i]);
+        g[i] = __float_as_uint(__uint_as_float(g[i]) + vec1[i]);
+      }
+      if (left < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= left) a[i] = g[i] = 0u;
+      }
+      uint32_t v[16];
+      if (p.u) {
+        char* u = static_cast<char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
+        store_rows<2>(stage, v, u, 4 * (int64_t)p.hp, rows, 64, true);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+        store_rows<2>(stage, v, u + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows, 64, true);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          h[i] = __uint_as_float(a[4 * q + i]) * act_value<ACT>(__uint_as_float(g[4 * q + i]));
+        if constexpr (DROP) drop(h, m + lane, n + 4 * q);
+        v[2 * q] = pack2<T>(h[0], h[1]);
+        v[2 * q + 1] = pack2<T>(h[2], h[3]);
+      }
+      store_rows<2>(stage, v, static_cast<char*>(p.out) + 2 * ((int64_t)m * p.hp + n), 2 * (int64_t)p.hp, rows, 64, true);
+    } else {
+      turn_rows(stage, uv);
+      turn_rows(stage, ug);
+      uint32_t d[32];
+      tc::tmem_load32(d, acc + c);
+      tc::tmem_wait();
+      const int left = p.N - n;
+      uint32_t dv[16], dg[16];
+      const uint32_t* pv = reinterpret_cast<const uint32_t*>(uv);
+      const uint32_t* pg = reinterpret_cast<const uint32_t*>(ug);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        float h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = 4 * q + i < left ? __uint_as_float(d[4 * q + i]) : 0.0f;
+        if constexpr (DROP) drop(h, m + lane, n + 4 * q);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 a = unpack2<T>(pv[2 * q + i]), g = unpack2<T>(pg[2 * q + i]);
+          float v0, s0, v1, s1;
+          act_both<ACT>(g.x, v0, s0);
+          act_both<ACT>(g.y, v1, s1);
+          dv[2 * q + i] = pack2<T>(h[2 * i] * v0, h[2 * i + 1] * v1);
+          dg[2 * q + i] = pack2<T>(h[2 * i] * a.x * s0, h[2 * i + 1] * a.y * s1);
+        }
+      }
+      char* du = static_cast<char*>(p.out) + 2 * ((int64_t)m * 2 * p.hp + n);
+      store_rows<2>(stage, dv, du, 4 * (int64_t)p.hp, rows, 64, true);
+      store_rows<2>(stage, dg, du + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows, 64, true);
+    }
+  }
+
+  __device__ __forceinline__ void fetch_u(int m, int n, uint4 (&uv)[4], uint4 (&ug)[4]) {
+    const char* u = static_cast<const char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
+    const int rows = min(32, p.M - m);
+    fetch_rows(uv, u, 4 * (int64_t)p.hp, rows);
+    fetch_rows(ug, u + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows);
+  }
+
+ private:
+  __device__ __forceinline__ void bias_vector(int at, int left, const void* bias, float* vec) {
+    float b = 0.0f;
+    if (bias && lane < left) b = to_float(static_cast<const T*>(bias)[at + lane]);
+    __syncwarp();
+    vec[lane] = b;
+    __syncwarp();
+  }
+  __device__ __forceinline__ void drop(float (&h)[4], int row, int col) {
+    const uint4 w = rng((uint32_t)col >> 2, (uint32_t)row);
+    h[0] = w.x >= p.drop.threshold ? h[0] * p.drop.scale : 0.0f;
+    h[1] = w.y >= p.drop.threshold ? h[1] * p.drop.scale : 0.0f;
+    h[2] = w.z >= p.drop.threshold ? h[2] * p.drop.scale : 0.0f;
+    h[3] = w.w >= p.drop.threshold ? h[3] * p.drop.scale : 0.0f;
+  }
+  // result rows m .. m + rows - 1, honouring the two runs of rows of seg_pad
+  template <int ES>
+  __device__ __forceinline__ void store_result(const uint32_t (&v)[16], int m, int n, int rows, int bytes) {
+    int64_t out_row = m;
+    if (p.seg_pad) {  // seg_pad is a multiple of 64, so 32 rows never straddle the runs
+      const int in = m >= p.seg_pad ? m - p.seg_pad : m;
+      rows = min(rows, p.seg - in);
+      out_row = m >= p.seg_pad ? (int64_t)p.seg + in : in;
+    }
+    store_rows<ES>(stage, v, static_cast<char*>(p.out) + ES * (out_row * p.ld_out + n), ES * p.ld_out, rows, bytes,
+                   p.vec_out);
+  }
+};
+
+template <int EPI, typename T, int ACT, bool DROP>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  extern __shared__ char smem_raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  char* staging = smem + kStages * kStageBytes;
+  Pipe* pipe = reinterpret_cast<Pipe*>(staging + kEpiWarps * kWarpStage);
+  const uint32_t base = tc::smem_addr(smem);
+  const uint32_t full = tc::smem_addr(pipe->full), empty = tc::smem_addr(pipe->empty);
+  const uint32_t acc_full = tc::smem_addr(pipe->acc_full), acc_empty = tc::smem_addr(pipe->acc_empty);
+  volatile uint32_t* abort = &pipe->abort;
+  const int warp = threadIdx.x >> 5;
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+
+  if (threadIdx.x == 0) {
+    tc::tma_prefetch(&p.ma);
+    tc::tma_prefetch(&p.mb);
+    for (int i = 0; i < kStages; ++i) {
+      tc::mbar_init(full + 8 * i, 1);
+      tc::mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(acc_full + 8 * i, 1);
+      tc::mbar_init(acc_empty + 8 * i, kEpiWarps);
+    }
+    pipe->abort = 0;
+    tc::fence_barrier_init();
+    tc::fence_proxy_async();
+  }
+  if (warp == 1) tc::tmem_alloc(tc::smem_addr(&pipe->tmem), kTmemCols);
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&pipe->tmem);
+
+  if (warp == 0) {
+    if (tc::elect_one()) {
+      uint32_t n = 0;  // stages filled
+      bool ok = true;
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const Tile t = tile_of(p, item);
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
+          const int s = n % kStages;
+          ok = tc::mbar_wait(empty + 8 * s, ((n / kStages) & 1) ^ 1, abort);
+          if (!ok) break;
+          const uint32_t bar = full + 8 * s, a = base + s * kStageBytes, b = a + kABytes;
+          tc::mbar_expect_tx(bar, p.tx_bytes);
+          const int k0 = kb * (EPI == EPI_INT8 ? 128 : 64);
+          if (p.a_mn) {
+            tc::tma_load(a, &p.ma, bar, t.m0, k0);
+            tc::tma_load(a + tc::kMnGroupBytes, &p.ma, bar, t.m0 + 64, k0);
+          } else {
+            tc::tma_load(a, &p.ma, bar, k0, t.m0);
+          }
+          if (EPI == EPI_GATED) {
+            tc::tma_load(b, &p.mb, bar, k0, t.n0);
+            tc::tma_load(b + p.cols * 128, &p.mb, bar, k0, p.gate_row + t.n0);
+          } else if (p.b_mn) {
+            for (int i = 0; i < p.bn; i += 64) tc::tma_load(b + 128 * i, &p.mb, bar, t.n0 + i, k0);
+          } else {
+            tc::tma_load(b, &p.mb, bar, k0, t.n0);
+          }
+        }
+      }
+      if (!ok) {  // the copies in flight must land before the CTA ends
+        volatile uint32_t ignore = 0;
+        const uint32_t first = n > kStages ? n - kStages : 0;
+        for (uint32_t i = first; i < n; ++i) tc::mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, &ignore);
+      }
+    }
+  } else if (warp == 1) {
+    if (tc::elect_one()) {
+      uint32_t n = 0, it = 0;
+      bool ok = true;
+      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x, ++it) {
+        const Tile t = tile_of(p, item);
+        const uint32_t buf = it & 1;
+        ok = tc::mbar_wait(acc_empty + 8 * buf, ((it >> 1) & 1) ^ 1, abort);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t d = tmem + buf * kMaxN;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
+          const int s = n % kStages;
+          ok = tc::mbar_wait(full + 8 * s, (n / kStages) & 1, abort);
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t a = base + s * kStageBytes;
+          const uint64_t da = tc::operand_desc(a, p.a_mn), db = tc::operand_desc(a + kABytes, p.b_mn);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            tc::mma<EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, p.idesc, kb > t.kb0 || i > 0);
+          tc::mma_commit(empty + 8 * s);
+        }
+        if (!ok) break;
+        tc::mma_commit(acc_full + 8 * buf);
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * kWarpStage);
+    uint32_t it = 0;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++it) {
+      const Tile t = tile_of(p, item);
+      const uint32_t buf = it & 1;
+      const int m = t.m0 + 32 * quarter;
+      const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + buf * kMaxN;
+      uint4 uv[4], ug[4];
+      if constexpr (EPI == EPI_GATED_BWD) {
+        if (32 * half < p.cols && t.n0 + 32 * half < p.hp) epi.fetch_u(m, t.n0 + 32 * half, uv, ug);
+      }
+      if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
+      tc::fence_after();
+      // gated: the padding columns of h, u and du are written too (zeros)
+      const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
+      for (int c = 32 * half; c < p.cols && t.n0 + c < n_end; c += 64) {
+        epi.chunk(acc, t, m, c, uv, ug);
+        if constexpr (EPI == EPI_GATED_BWD) {
+          if (c + 64 < p.cols && t.n0 + c + 64 < p.hp) epi.fetch_u(m, t.n0 + c + 64, uv, ug);
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) tc::mbar_arrive(acc_empty + 8 * buf);
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort) atomicOr(&g_status, GF_FLAG_TIMEOUT);
+  if (warp == 1) {
+    tc::fence_after();
+    if (*abort) {  // products may still be running: their end is a commit away
+      if (tc::elect_one()) {
+        volatile uint32_t ignore = 0;
+        tc::mbar_init(tc::smem_addr(&pipe->acc_full[0]), 1);
+        tc::mma_commit(tc::smem_addr(&pipe->acc_full[0]));
+        tc::mbar_wait(tc::smem_addr(&pipe->acc_full[0]), 0, &ignore);
+      }
+      __syncwarp();
+    }
+    tc::tmem_free(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// K ranges joined: out = sum of the partial products (in order) + bias
+
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmParams p) {
+  const int64_t groups = p.ld_partial / 4, total = (int64_t)p.M * groups;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t m = i / groups;
+    const int n = (int)(i - m * groups) * 4;
+    if (n >= p.N) continue;
+    int64_t row = m;
+    if (p.seg_pad) {
+      const int64_t in = m >= p.seg_pad ? m - p.seg_pad : m;
+      if (in >= p.seg) continue;
+      row = m >= p.seg_pad ? p.seg + in : in;
+    }
+    float4 s = make_float4(0, 0, 0, 0);
+    for (int k = 0; k < p.splits; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.M + m) * p.ld_partial + n);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float f[4] = {s.x, s.y, s.z, s.w};
+    T* out = static_cast<T*>(p.out) + row * p.ld_out + n;
+    const T* bias = static_cast<const T*>(p.bias);
+    T r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = from_float<T>(f[j] + (bias && n + j < p.N ? to_float(bias[n + j]) : 0.0f));
+    if (p.vec_out) {  // N is then a multiple of 4
+      *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(r);
+    } else {
+      for (int j = 0; j < 4 && n + j < p.N; ++j) out[j] = r[j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// column sums (bias gradients): rows cut into `parts` runs, each summed in
+// order, the runs then added in order
+
+template <typename T>
+__global__ void __launch_bounds__(256) column_sums_kernel(const T* src, int64_t ld, int rows, int cols, int run,
+                                                          float* partial) {
+  const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
+  const int64_t r0 = (int64_t)blockIdx.y * run, r1 = min((int64_t)rows, r0 + run);
+  float s = 0.0f;
+  if (c < cols)
+    for (int64_t r = r0 + w; r < r1; r += 8) s += to_float(src[r * ld + c]);
+  __shared__ float sums[8][32];
+  sums[w][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
+    partial[(int64_t)blockIdx.y * cols + c] = s;
+  }
+}
+// out[c] = sum over the runs; `seg` columns from 0 and from seg_pad (0: all)
+template <typename T>
+__global__ void __launch_bounds__(256) column_join_kernel(const float* partial, int parts, int cols, int seg_pad, int seg,
+                                                          T* out) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  const int n = seg_pad ? 2 * seg : cols;
+  if (i >= n) return;
+  const int c = seg_pad && i >= seg ? seg_pad + i - seg : i;
+  float s = 0.0f;
+  for (int k = 0; k < parts; ++k) s += partial[(int64_t)k * cols + c];
+  out[i] = from_float<T>(s);
+}
+
+// ---------------------------------------------------------------------------
+// copies into 16-byte aligned rows: dst row r holds src row r (or, with two
+// runs of rows, src rows 0 .. seg - 1 and seg .. 2 seg - 1 at 0 and seg_pad);
+// everything else is zero
+
+template <typename E>
+__global__ void __launch_bounds__(256) align_kernel(const E* src, int64_t ld, int64_t src_rows, int cols, E* dst,
+                                                    int ld_dst, int64_t dst_rows, int seg_pad, int seg) {
+  const int64_t total = dst_rows * ld_dst;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / ld_dst;
+    const int c = (int)(i - r * ld_dst);
+    int64_t from = r;
+    if (seg_pad) {
+      const int64_t in = r >= seg_pad ? r - seg_pad : r;
+      from = in < seg ? (r >= seg_pad ? seg + in : in) : src_rows;
+    }
+    dst[i] = from < src_rows && c < cols ? src[from * ld + c] : E(0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dropout
+
+struct DropoutParams {
+  int64_t rows, groups;  // groups of V columns in a row
+  int64_t cols;
+  const void* x;
+  int64_t x_rs, x_cs;
+  const void* res;
+  int64_t r_rs, r_cs;
+  void* y;
+  DropArgs drop;
+};
+
+// One thread takes V columns of a row at a time: 16 bytes of aligned rows, or
+// (VEC false) four elements through any strides.  ROWS: neighbouring threads
+// take neighbouring rows, for inputs whose rows are the contiguous dimension.
+template <typename T, bool VEC, bool ROWS>
+__global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
+  constexpr int V = VEC ? 16 / sizeof(T) : 4;
+  const Philox rng(p.drop);
+  const int64_t inner = ROWS ? p.rows : p.groups, outer = ROWS ? p.groups : p.rows;
+  const int64_t step = (int64_t)gridDim.x * blockDim.x;
+  const int64_t step_o = step / inner, step_i = step - step_o * inner;
+  int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+  int64_t o = i / inner;
+  i -= o * inner;
+  while (o < outer) {
+    const int64_t row = ROWS ? i : o, group = ROWS ? o : i;
+    const int64_t col = group * V;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_rs + col * p.x_cs;
+    const T* res = p.res ? static_cast<const T*>(p.res) + row * p.r_rs + col * p.r_cs : nullptr;
+    T* y = static_cast<T*>(p.y) + row * p.cols + col;
+    T in[V], add[V], out[V];
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(in) = *reinterpret_cast<const uint4*>(x);
+      if (res) *reinterpret_cast<uint4*>(add) = *reinterpret_cast<const uint4*>(res);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (col + j < p.cols) {
+          in[j] = x[j * p.x_cs];
+          if (res) add[j] = res[j * p.r_cs];
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < V / 4; ++b) {
+      const uint4 w = rng((uint32_t)(col / 4 + b), (uint64_t)row);
+      const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v = word[j] >= p.drop.threshold ? to_float(in[4 * b + j]) * p.drop.scale : 0.0f;
+        if (res) v += to_float(add[4 * b + j]);
+        out[4 * b + j] = from_float<T>(v);
+      }
+    }
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(out);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (col + j < p.cols) y[j] = out[j];
+    }
+    o += step_o;
+    i += step_i;
+    if (i >= inner) i -= inner, ++o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// row quantisation: TPR threads per row, two passes over the row (the second
+// finds it in L1 or L2)
+
+constexpr float kTinyRow = 7.8886090522101181e-31f;  // 2^-100: below it 127 / max could overflow
+
+template <typename T, int TPR>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int cols, const T* x, int64_t ld, int8_t* q,
+                                                            int64_t ld_q, float* scale, int vec) {
+  const int t = threadIdx.x % TPR;
+  const int64_t per_block = 256 / TPR;
+  __shared__ uint32_t warp_max[8];
+  for (int64_t base = blockIdx.x * per_block; base < rows; base += gridDim.x * per_block) {
+    const int64_t r = base + threadIdx.x / TPR;
+    const bool live = r < rows;
+    const T* row = x + r * ld;
+    // magnitudes compare like their bits, with infinity and NaN above every finite value
+    uint32_t top = 0;
+    auto see = [&](float v) { top = max(top, __float_as_uint(v) & 0x7FFFFFFFu); };
+    if (live) {
+      if (vec) {
+        for (int c = 8 * t; c < cols; c += 8 * TPR) {
+          T v[8];
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + c);
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(row + c + 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) see(to_float(v[j]));
+        }
+      } else {
+        for (int c = t; c < cols; c += TPR) see(to_float(row[c]));
+      }
+    }
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if constexpr (TPR > 32) {
+      if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = top;
+      __syncthreads();
+      top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, warp_max[i]);
+      __syncthreads();
+    }
+    if (!live) continue;
+    const float most = __uint_as_float(top);
+    float s = __fdiv_rn(most, 127.0f), inv = __fdiv_rn(127.0f, most);
+    bool zero = false;
+    if (most < kTinyRow) s = 0.0f, zero = true;
+    if (top >= 0x7F800000u) s = __uint_as_float(0x7FFFFFFFu), zero = true;
+    if (t == 0) scale[r] = s;
+    auto quant = [&](float v) -> int {
+      return zero ? 0 : (int)(int8_t)__float2int_rn(__fmul_rn(v, inv));
+    };
+    int8_t* out = q + r * ld_q;
+    if (vec) {
+      for (int c = 8 * t; c < ld_q; c += 8 * TPR) {
+        uint32_t w[2] = {0, 0};
+        if (c < cols) {
+          T v[8];
+          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + c);
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(row + c + 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(quant(to_float(v[j])) & 0xFF) << (8 * (j % 4));
+        }
+        *reinterpret_cast<uint2*>(out + c) = make_uint2(w[0], w[1]);
+      }
+    } else {
+      for (int c = t; c < ld_q; c += TPR) out[c] = c < cols ? (int8_t)quant(to_float(row[c])) : (int8_t)0;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+#define GFB_CUDA(call)                                                                            \
+  do {                                                                                            \
+    const cudaError_t e_ = (call);                                                                \
+    if (e_ != cudaSuccess) return gf::fail(GF_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));     \
+  } while (0)
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+gf_status encode_fn(EncodeFn* out) {
+  static std::atomic<void*> fn{nullptr};
+  void* f = fn.load();
+  if (!f) {
+    cudaDriverEntryPointQueryResult found;
+    GFB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !f) return fail(GF_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    fn.store(f);
+  }
+  *out = reinterpret_cast<EncodeFn>(f);
+  return GF_OK;
+}
+
+// A row-major operand: `rows` rows of `cols` elements, 16-byte aligned rows.
+struct Operand {
+  const void* ptr;
+  int64_t rows, cols, ld;
+};
+
+inline bool aligned_rows(const void* ptr, int64_t rows, int64_t ld, int es) {
+  return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (rows == 1 || (ld * es) % 16 == 0);
+}
+
+gf_status make_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type, int es, int box_cols, int box_rows) {
+  EncodeFn encode;
+  if (const gf_status s = encode_fn(&encode); s != GF_OK) return s;
+  const int64_t ld = o.rows == 1 ? round_up<int64_t>(o.cols * es, 16) : o.ld * es;
+  const cuuint64_t dims[2] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, unit[2] = {1, 1};
+  auto run = [&] {
+    return encode(map, type, 2, const_cast<void*>(o.ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = run();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no runtime call yet (autograd's): give it the context
+    int dev = 0;
+    GFB_CUDA(cudaGetDevice(&dev));
+    GFB_CUDA(cudaSetDevice(dev));
+    r = run();
+  }
+  if (r != CUDA_SUCCESS)
+    return fail(GF_ERR_CUDA, "cuTensorMapEncodeTiled(%lld x %lld, ld %lld): error %d", (long long)o.rows, (long long)o.cols,
+                (long long)o.ld, (int)r);
+  return GF_OK;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      n <= 0) {
+    cudaGetLastError();
+    return 148;  // workspace queries work without a device
+  }
+  return n;
+}
+
+// Tile width and K ranges.  A CTA's time for one tile is taken as its loads,
+// (128 + bn) * 128 bytes a 64-k step at 64 bytes a clock, plus a fixed cost;
+// the grid's as that of the CTA with most tiles; K ranges add the partial
+// sums' way to memory and back.  Narrower tiles or K ranges win only where
+// wide ones leave SMs idle.
+struct Shape {
+  int bn, splits, kb_split, tiles_m, tiles_n;
+};
+Shape choose_shape(int64_t M, int64_t N, int64_t kb, bool gated, bool may_split, int sms) {
+  Shape best{};
+  double best_cost = 0;
+  const int step = gated ? 64 : 32;
+  const int64_t tm = ceil_div(M, kTileM);
+  for (int bn = step; bn <= kMaxN; bn += step) {
+    const int cols = gated ? bn / 2 : bn;
+    const int64_t tn = ceil_div(N, cols);
+    if (cols > 32 && cols - 32 >= N) break;  // wider than the result
+    for (int64_t s = 1; s <= (may_split ? kb : 1) && s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
+      const int64_t per = ceil_div(kb, s), parts = ceil_div(kb, per);
+      if (parts != s) continue;
+      const int64_t waves = ceil_div(tm * tn * s, sms);
+      double cost = (double)waves * (per * 2.0 * (128 + bn) + 600.0) + 2.0 * bn;
+      if (s > 1) cost += 4000.0 + (double)(s + 1) * M * N * 4 / 3000.0;
+      if (best.bn == 0 || cost < best_cost) {
+        best_cost = cost;
+        best = Shape{bn, (int)s, (int)per, (int)tm, (int)tn};
+      }
+    }
+  }
+  return best;
+}
+
+inline size_t partial_bytes(const Shape& s, int64_t M, int64_t N) {
+  return s.splits > 1 ? round_up<size_t>((size_t)s.splits * M * round_up<int64_t>(N, 32) * 4, 256) : 0;
+}
+
+template <auto Kernel>
+gf_status launch_gemm(const GemmParams& p, int sms, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
+  int dev = 0;
+  GFB_CUDA(cudaGetDevice(&dev));
+  if (dev > 63 || !(ready.load() >> dev & 1)) {
+    GFB_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    if (dev <= 63) ready.fetch_or(uint64_t(1) << dev);
+  }
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  Kernel<<<(int)(items < sms ? items : sms), kThreads, kSmemBytes, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GF_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
+  return GF_OK;
+}
+
+inline int grid_for(int64_t work, int threads, int sms) {
+  const int64_t b = ceil_div(work, threads);
+  return (int)(b < 8 * (int64_t)sms ? (b > 0 ? b : 1) : 8 * (int64_t)sms);
+}
+
+// Fills the operand part of a product: A (m, k), B (n, k) as stored.
+gf_status set_operands(GemmParams& p, const Shape& s, const Operand& a, bool a_mn, const Operand& b, bool b_mn, int es,
+                       CUtensorMapDataType type, uint32_t acc, uint32_t fmt, bool gated) {
+  const int line = 128 / es;
+  p.tiles_m = s.tiles_m;
+  p.tiles_n = s.tiles_n;
+  p.splits = s.splits;
+  p.kb_split = s.kb_split;
+  p.bn = s.bn;
+  p.cols = gated ? s.bn / 2 : s.bn;
+  p.a_mn = a_mn;
+  p.b_mn = b_mn;
+  p.idesc = tc::instruction_desc(acc, fmt, a_mn, b_mn, s.bn);
+  p.tx_bytes = kABytes + 128 * (b_mn ? round_up(s.bn, 64) : s.bn);
+  gf_status r = a_mn ? make_map(&p.ma, a, type, es, 64, 64) : make_map(&p.ma, a, type, es, line, kTileM);
+  if (r != GF_OK) return r;
+  return b_mn ? make_map(&p.mb, b, type, es, 64, 64) : make_map(&p.mb, b, type, es, line, p.cols);
+}
+
+// ---- the feed-forward block
+
+struct Bump {  // workspace layout: offsets first (null base), pointers when it exists
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    char* p = base ? base + used : nullptr;
+    used += round_up<size_t>(bytes, 256);
+    return p;
+  }
+};
+
+struct FfPlan {
+  int64_t M, D, F, O, Hp;
+  bool copy_x, copy_w_in, copy_w_out, copy_dy;
+  Shape in, out, dh, dx, dw_in, dw_out;
+  int in_parts, in_run, out_parts, out_run;  // column sums
+  void *x, *w_in, *w_out, *dy, *du, *partial, *sums;
+  size_t bytes;
+};
+
+void column_runs(int64_t rows, int64_t cols, int sms, int* parts, int* run) {
+  // about four CTAs of 32 columns for each SM, runs of at least 64 rows
+  int64_t want = 4 * (int64_t)sms / ceil_div(cols, 32);
+  if (want < 1) want = 1;
+  int64_t r = ceil_div(rows, want);
+  if (r < 64) r = 64;
+  *run = (int)r;
+  *parts = (int)ceil_div(rows, r);
+}
+
+FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
+  FfPlan p{};
+  const int sms = sm_count();
+  p.M = f.tokens, p.D = f.in_features, p.F = f.hidden, p.O = f.out_features;
+  p.Hp = round_up<int64_t>(p.F, 64);
+  const bool back = pass == GF_PASS_BACKWARD;
+  const bool use_x = !back || f.dw_in, use_w_in = !back || f.dx;
+  const bool use_du = back && (f.dx || f.dw_in || f.db_in);
+  const bool use_w_out = !back || use_du, use_dy = back && (use_du || f.dw_out);
+  p.copy_x = use_x && !aligned_rows(f.x, p.M, f.ld_x, 2);
+  p.copy_w_in = use_w_in && (p.Hp != p.F || !aligned_rows(f.w_in, 2 * p.F, f.ld_w_in, 2));
+  p.copy_w_out = use_w_out && !aligned_rows(f.w_out, p.O, f.ld_w_out, 2);
+  p.copy_dy = use_dy && !aligned_rows(f.dy, p.M, f.ld_dy, 2);
+  Bump b{ws};
+  if (p.copy_x) p.x = b.take(2 * p.M * round_up<int64_t>(p.D, 8));
+  if (p.copy_w_in) p.w_in = b.take(2 * 2 * p.Hp * round_up<int64_t>(p.D, 8));
+  if (p.copy_w_out) p.w_out = b.take(2 * p.O * round_up<int64_t>(p.F, 8));
+  if (p.copy_dy) p.dy = b.take(2 * p.M * round_up<int64_t>(p.O, 8));
+  size_t partial = 0, sums = 0;
+  auto need = [&](const Shape& s, int64_t M, int64_t N) {
+    const size_t n = partial_bytes(s, M, N);
+    if (n > partial) partial = n;
+  };
+  if (!back) {
+    p.in = choose_shape(p.M, p.Hp, ceil_div(p.D, 64), true, false, sms);
+    p.out = choose_shape(p.M, p.O, ceil_div(p.F, 64), false, true, sms);
+    need(p.out, p.M, p.O);
+  } else {
+    if (use_du) {
+      p.du = b.take(2 * p.M * 2 * p.Hp);
+      p.dh = choose_shape(p.M, p.Hp, ceil_div(p.O, 64), false, false, sms);
+    }
+    if (f.dx) {
+      p.dx = choose_shape(p.M, p.D, 2 * p.Hp / 64, false, true, sms);
+      need(p.dx, p.M, p.D);
+    }
+    if (f.dw_in) {
+      p.dw_in = choose_shape(2 * p.Hp, p.D, ceil_div(p.M, 64), false, true, sms);
+      need(p.dw_in, 2 * p.Hp, p.D);
+    }
+    if (f.dw_out) {
+      p.dw_out = choose_shape(p.O, p.F, ceil_div(p.M, 64), false, true, sms);
+      need(p.dw_out, p.O, p.F);
+    }
+    if (f.db_in) {
+      column_runs(p.M, 2 * p.Hp, sms, &p.in_parts, &p.in_run);
+      sums = (size_t)4 * p.in_parts * 2 * p.Hp;
+    }
+    if (f.db_out) {
+      column_runs(p.M, p.O, sms, &p.out_parts, &p.out_run);
+      const size_t n = (size_t)4 * p.out_parts * p.O;
+      if (n > sums) sums = n;
+    }
+  }
+  if (partial) p.partial = b.take(partial);
+  if (sums) p.sums = b.take(sums);
+  p.bytes = b.used > 256 ? b.used : 256;
+  return p;
+}
+
+gf_status check_ff(const char* who, const gf_gated_ff* f) {
+  if (!f) return fail(GF_ERR_INVALID_ARG, "%s: the description must be non-null", who);
+  if (f->tokens < 0 || f->in_features <= 0 || f->hidden <= 0 || f->out_features <= 0)
+    return fail(GF_ERR_INVALID_ARG, "%s: sizes must be positive (tokens may be 0)", who);
+  if (f->tokens > kMaxDim || f->in_features > kMaxDim || f->hidden > kMaxDim / 2 || f->out_features > kMaxDim)
+    return fail(GF_ERR_UNSUPPORTED, "%s: a size is above 2^31 - 512 (2 * hidden counts)", who);
+  if (f->dtype != GF_BF16 && f->dtype != GF_F16)
+    return fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_BF16 or GF_F16", who);
+  if (f->activation != GF_ACT_GELU && f->activation != GF_ACT_SILU)
+    return fail(GF_ERR_INVALID_ARG, "%s: unknown activation", who);
+  if (f->ld_x < f->in_features || f->ld_w_in < f->in_features || f->ld_w_out < f->hidden)
+    return fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
+  return check_rule(who, f->dropout);
+}
+
+gf_status check_workspace(const char* who, const void* ws, size_t have, size_t want) {
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(GF_ERR_INVALID_ARG, "%s: workspace must be non-null and 256-byte aligned", who);
+  if (have < want) return fail(GF_ERR_INVALID_ARG, "%s: workspace too small: %zu bytes given, %zu needed", who, have, want);
+  return GF_OK;
+}
+
+template <typename E>
+gf_status align_copy(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ld_dst, int64_t dst_rows,
+                     int64_t seg_pad, int64_t seg, int sms, cudaStream_t st) {
+  align_kernel<E><<<grid_for(dst_rows * ld_dst, 256, sms), 256, 0, st>>>(
+      static_cast<const E*>(src), ld, rows, (int)cols, static_cast<E*>(dst), (int)ld_dst, dst_rows, (int)seg_pad, (int)seg);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(GF_ERR_CUDA, "align_kernel: %s", cudaGetErrorString(e));
+  return GF_OK;
+}
+
+#define GFB_TRY(call)                                 \
+  do {                                                \
+    const gf_status s_ = (call);                      \
+    if (s_ != GF_OK) return s_;                       \
+  } while (0)
+
+// The operands of the block as the products see them: rows aligned, the two
+// halves of w_in Hp rows apart.
+struct FfOperands {
+  Operand x, w_in, w_out, dy;
+};
+gf_status align_ff(const gf_gated_ff& f, const FfPlan& p, FfOperands* o, int sms, cudaStream_t st) {
+  o->x = Operand{f.x, p.M, p.D, f.ld_x};
+  o->w_in = Operand{f.w_in, 2 * p.Hp, p.D, f.ld_w_in};
+  o->w_out = Operand{f.w_out, p.O, p.F, f.ld_w_out};
+  o->dy = Operand{f.dy, p.M, p.O, f.ld_dy};
+  const int64_t ld_d = round_up<int64_t>(p.D, 8), ld_f = round_up<int64_t>(p.F, 8), ld_o = round_up<int64_t>(p.O, 8);
+  if (p.copy_x) {
+    GFB_TRY(align_copy<uint16_t>(f.x, f.ld_x, p.M, p.D, p.x, ld_d, p.M, 0, 0, sms, st));
+    o->x = Operand{p.x, p.M, p.D, ld_d};
+  }
+  if (p.copy_w_in) {
+    GFB_TRY(align_copy<uint16_t>(f.w_in, f.ld_w_in, 2 * p.F, p.D, p.w_in, ld_d, 2 * p.Hp, p.Hp, p.F, sms, st));
+    o->w_in = Operand{p.w_in, 2 * p.Hp, p.D, ld_d};
+  }
+  if (p.copy_w_out) {
+    GFB_TRY(align_copy<uint16_t>(f.w_out, f.ld_w_out, p.O, p.F, p.w_out, ld_f, p.O, 0, 0, sms, st));
+    o->w_out = Operand{p.w_out, p.O, p.F, ld_f};
+  }
+  if (p.copy_dy) {
+    GFB_TRY(align_copy<uint16_t>(f.dy, f.ld_dy, p.M, p.O, p.dy, ld_o, p.M, 0, 0, sms, st));
+    o->dy = Operand{p.dy, p.M, p.O, ld_o};
+  }
+  return GF_OK;
+}
+
+template <typename T>
+constexpr CUtensorMapDataType map_type() {
+  return std::is_same_v<T, __nv_bfloat16> ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+template <typename T>
+constexpr uint32_t mma_format() {
+  return std::is_same_v<T, __nv_bfloat16> ? tc::kFmtBf16 : tc::kFmtF16;
+}
+
+// out [M, N] = A B^T (+ bias), rows in one run or two
+template <typename T>
+gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b, bool b_mn, int64_t M, int64_t N, int64_t K,
+                  void* out, int64_t ld_out, const void* bias, int64_t seg_pad, int64_t seg, void* partial, int sms,
+                  cudaStream_t st) {
+  GemmParams p{};
+  GFB_TRY(set_operands(p, s, a, a_mn, b, b_mn, 2, map_type<T>(), tc::kAccF32, mma_format<T>(), false));
+  p.M = (int)M;
+  p.N = (int)N;
+  p.kb_total = (int)ceil_div(K, 64);
+  p.out = out;
+  p.ld_out = ld_out;
+  p.vec_out = aligned_rows(out, 2, ld_out, 2) && N % 8 == 0;
+  p.bias = bias;
+  p.seg_pad = (int)seg_pad;
+  p.seg = (int)seg;
+  p.partial = static_cast<float*>(partial);
+  p.ld_partial = round_up<int64_t>(N, 32);
+  GFB_TRY((launch_gemm<gemm_kernel<EPI_STORE, T, 0, false>>(p, sms, st)));
+  if (s.splits > 1) {
+    join_kernel<T><<<grid_for(M * (p.ld_partial / 4), 256, sms), 256, 0, st>>>(p);
+    GFB_CUDA(cudaGetLastError());
+  }
+  return GF_OK;
+}
+
+template <typename T, int ACT, bool DROP>
+gf_status gated(GemmParams& p, bool back, int sms, cudaStream_t st) {
+  return back ? launch_gemm<gemm_kernel<EPI_GATED_BWD, T, ACT, DROP>>(p, sms, st)
+              : launch_gemm<gemm_kernel<EPI_GATED, T, ACT, DROP>>(p, sms, st);
+}
+template <typename T>
+gf_status gated(GemmParams& p, bool back, int act, int sms, cudaStream_t st) {
+  if (act == GF_ACT_GELU)
+    return p.drop.on ? gated<T, GF_ACT_GELU, true>(p, back, sms, st) : gated<T, GF_ACT_GELU, false>(p, back, sms, st);
+  return p.drop.on ? gated<T, GF_ACT_SILU, true>(p, back, sms, st) : gated<T, GF_ACT_SILU, false>(p, back, sms, st);
+}
+
+template <typename T>
+gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
+  const int sms = sm_count();
+  FfOperands o;
+  GFB_TRY(align_ff(f, pl, &o, sms, st));
+  GemmParams p{};
+  GFB_TRY(set_operands(p, pl.in, o.x, false, o.w_in, false, 2, map_type<T>(), tc::kAccF32, mma_format<T>(), true));
+  p.M = (int)pl.M;
+  p.N = (int)pl.F;
+  p.hp = (int)pl.Hp;
+  p.gate_row = (int)pl.Hp;
+  p.kb_total = (int)ceil_div(pl.D, 64);
+  p.bias = f.b_in;
+  p.u = f.u;
+  p.out = f.h;
+  p.drop = drop_args(f.dropout);
+  GFB_TRY(gated<T>(p, false, f.activation, sms, st));
+  return product<T>(pl.out, Operand{f.h, pl.M, pl.Hp, pl.Hp}, false, o.w_out, false, pl.M, pl.O, pl.F, f.y, f.ld_y, f.b_out,
+                    0, 0, pl.partial, sms, st);
+}
+
+template <typename T>
+gf_status column_sums(const void* src, int64_t ld, int64_t rows, int64_t cols, int parts, int run, void* partial,
+                      int64_t seg_pad, int64_t seg, void* out, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)parts);
+  column_sums_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(src), ld, (int)rows, (int)cols, run,
+                                              static_cast<float*>(partial));
+  GFB_CUDA(cudaGetLastError());
+  const int64_t n = seg_pad ? 2 * seg : cols;
+  column_join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(static_cast<const float*>(partial), parts, (int)cols,
+                                                                    (int)seg_pad, (int)seg, static_cast<T*>(out));
+  GFB_CUDA(cudaGetLastError());
+  return GF_OK;
+}
+
+template <typename T>
+gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
+  const int sms = sm_count();
+  FfOperands o;
+  GFB_TRY(align_ff(f, pl, &o, sms, st));
+  const Operand du{pl.du, pl.M, 2 * pl.Hp, 2 * pl.Hp};
+  if (pl.du) {
+    GemmParams p{};
+    GFB_TRY(set_operands(p, pl.dh, o.dy, false, o.w_out, true, 2, map_type<T>(), tc::kAccF32, mma_format<T>(), false));
+    p.M = (int)pl.M;
+    p.N = (int)pl.F;
+    p.hp = (int)pl.Hp;
+    p.kb_total = (int)ceil_div(pl.O, 64);
+    p.u = f.u;
+    p.out = pl.du;
+    p.drop = drop_args(f.dropout);
+    GFB_TRY(gated<T>(p, true, f.activation, sms, st));
+  }
+  if (f.dx)
+    GFB_TRY(product<T>(pl.dx, du, false, o.w_in, true, pl.M, pl.D, 2 * pl.Hp, f.dx, pl.D, nullptr, 0, 0, pl.partial, sms, st));
+  if (f.dw_in)
+    GFB_TRY(product<T>(pl.dw_in, du, true, o.x, true, 2 * pl.Hp, pl.D, pl.M, f.dw_in, pl.D, nullptr,
+                       pl.Hp == pl.F ? 0 : pl.Hp, pl.F, pl.partial, sms, st));
+  if (f.dw_out)
+    GFB_TRY(product<T>(pl.dw_out, o.dy, true, Operand{f.h, pl.M, pl.Hp, pl.Hp}, true, pl.O, pl.F, pl.M, f.dw_out, pl.F,
+                       nullptr, 0, 0, pl.partial, sms, st));
+  if (f.db_in)
+    GFB_TRY(column_sums<T>(pl.du, 2 * pl.Hp, pl.M, 2 * pl.Hp, pl.in_parts, pl.in_run, pl.sums, pl.Hp == pl.F ? 0 : pl.Hp,
+                           pl.F, f.db_in, st));
+  if (f.db_out)
+    GFB_TRY(column_sums<T>(f.dy, f.ld_dy, pl.M, pl.O, pl.out_parts, pl.out_run, pl.sums, 0, 0, f.db_out, st));
+  return GF_OK;
+}
+
+// ---- dropout and the 8-bit product
+
+template <typename T>
+void launch_dropout(DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
+  p.groups = ceil_div(p.cols, vec ? 16 / (int64_t)sizeof(T) : 4);
+  const int grid = grid_for(p.rows * p.groups, 256, sms);
+  if (vec) dropout_kernel<T, true, false><<<grid, 256, 0, st>>>(p);
+  else if (by_rows) dropout_kernel<T, false, true><<<grid, 256, 0, st>>>(p);
+  else dropout_kernel<T, false, false><<<grid, 256, 0, st>>>(p);
+}
+
+template <typename T>
+void launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
+                     cudaStream_t st) {
+  const int vec = aligned_rows(x, rows, ld_x, sizeof(T)) && cols % 8 == 0 && ld_q % 8 == 0 &&
+                  (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  // a warp for a row of up to 2048 values, a CTA for a longer one
+  if (cols <= 2048)
+    quantize_rows_kernel<T, 32><<<grid_for(rows, 8, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x), ld_x, q,
+                                                                        ld_q, scale, vec);
+  else
+    quantize_rows_kernel<T, 256><<<grid_for(rows, 1, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x), ld_x, q,
+                                                                         ld_q, scale, vec);
+}
+
+bool known_dtype(int d) { return d == GF_F32 || d == GF_BF16 || d == GF_F16; }
+int dtype_size(int d) { return d == GF_F32 ? 4 : 2; }
+
+struct Int8Plan {
+  bool copy_a, copy_b;
+  Shape shape;
+  void *a, *b;
+  size_t bytes;
+};
+gf_status check_int8(const gf_int8_product* p) {
+  const char* who = "gf_int8_matmul";
+  if (!p) return fail(GF_ERR_INVALID_ARG, "%s: the description must be non-null", who);
+  if (p->m < 0 || p->n <= 0 || p->k <= 0) return fail(GF_ERR_INVALID_ARG, "%s: sizes must be positive (m may be 0)", who);
+  if (p->m > kMaxDim || p->n > kMaxDim) return fail(GF_ERR_UNSUPPORTED, "%s: a size is above 2^31 - 512", who);
+  if (p->k > 131071) return fail(GF_ERR_UNSUPPORTED, "%s: k must be at most 131071 (the sums are 32-bit integers)", who);
+  if (!known_dtype(p->dtype)) return fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_F32, GF_BF16 or GF_F16", who);
+  if (p->reserved != 0) return fail(GF_ERR_INVALID_ARG, "%s: reserved fields must be 0", who);
+  if (p->ld_a < p->k || p->ld_b < p->k || p->ld_out < p->n)
+    return fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
+  return GF_OK;
+}
+Int8Plan plan_int8(const gf_int8_product& p, char* ws) {
+  Int8Plan pl{};
+  Bump b{ws};
+  pl.copy_a = !aligned_rows(p.a, p.m, p.ld_a, 1);
+  pl.copy_b = !aligned_rows(p.b, p.n, p.ld_b, 1);
+  const int64_t ld = round_up<int64_t>(p.k, 16);
+  if (pl.copy_a) pl.a = b.take(p.m * ld);
+  if (pl.copy_b) pl.b = b.take(p.n * ld);
+  pl.shape = choose_shape(p.m, p.n, ceil_div(p.k, 128), false, false, sm_count());
+  pl.bytes = b.used > 256 ? b.used : 256;
+  return pl;
+}
+
+}  // namespace gfb
+
+// ---------------------------------------------------------------------------
+// C ABI
+
+extern "C" {
+
+size_t gf_gated_ff_workspace_bytes(const gf_gated_ff* ff, gf_pass pass) {
+  if (gfb::check_ff("gf_gated_ff_workspace_bytes", ff) != GF_OK) return 0;
+  return ff->tokens == 0 ? 256 : gfb::plan_ff(*ff, pass, nullptr).bytes;
+}
+
+gf_status gf_gated_ff_forward(const gf_gated_ff* ff, void* workspace, size_t workspace_bytes, gf_stream stream) {
+  const char* who = "gf_gated_ff_forward";
+  GFB_TRY(gfb::check_ff(who, ff));
+  if (ff->ld_y < ff->out_features) return gf::fail(GF_ERR_INVALID_ARG, "%s: ld_y is smaller than its row", who);
+  if (ff->tokens == 0) return GF_OK;
+  if (!ff->x || !ff->w_in || !ff->w_out || !ff->h || !ff->y)
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: x, w_in, w_out, h and y must be non-null", who);
+  if ((reinterpret_cast<uintptr_t>(ff->u) | reinterpret_cast<uintptr_t>(ff->h)) & 15u)
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: u and h must be 16-byte aligned", who);
+  const gfb::FfPlan pl = gfb::plan_ff(*ff, GF_PASS_FORWARD, static_cast<char*>(workspace));
+  GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
+  gfb::Range r("gfblock.gated_ff_forward");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return ff->dtype == GF_BF16 ? gfb::ff_forward<__nv_bfloat16>(*ff, pl, st) : gfb::ff_forward<__half>(*ff, pl, st);
+}
+
+gf_status gf_gated_ff_backward(const gf_gated_ff* ff, void* workspace, size_t workspace_bytes, gf_stream stream) {
+  const char* who = "gf_gated_ff_backward";
+  GFB_TRY(gfb::check_ff(who, ff));
+  if (ff->ld_dy < ff->out_features) return gf::fail(GF_ERR_INVALID_ARG, "%s: ld_dy is smaller than its row", who);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (ff->tokens == 0) {  // empty sums
+    const size_t d = ff->in_features, f = ff->hidden, o = ff->out_features;
+    if (ff->dw_in) GFB_CUDA(cudaMemsetAsync(ff->dw_in, 0, 2 * 2 * f * d, st));
+    if (ff->db_in) GFB_CUDA(cudaMemsetAsync(ff->db_in, 0, 2 * 2 * f, st));
+    if (ff->dw_out) GFB_CUDA(cudaMemsetAsync(ff->dw_out, 0, 2 * o * f, st));
+    if (ff->db_out) GFB_CUDA(cudaMemsetAsync(ff->db_out, 0, 2 * o, st));
+    return GF_OK;
+  }
+  if (!ff->dy || !ff->w_out || !ff->u) return gf::fail(GF_ERR_INVALID_ARG, "%s: dy, w_out and u must be non-null", who);
+  if (ff->dx && !ff->w_in) return gf::fail(GF_ERR_INVALID_ARG, "%s: dx needs w_in", who);
+  if (ff->dw_in && !ff->x) return gf::fail(GF_ERR_INVALID_ARG, "%s: dw_in needs x", who);
+  if (ff->dw_out && !ff->h) return gf::fail(GF_ERR_INVALID_ARG, "%s: dw_out needs h", who);
+  if ((reinterpret_cast<uintptr_t>(ff->u) | reinterpret_cast<uintptr_t>(ff->h)) & 15u)
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: u and h must be 16-byte aligned", who);
+  const gfb::FfPlan pl = gfb::plan_ff(*ff, GF_PASS_BACKWARD, static_cast<char*>(workspace));
+  GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
+  gfb::Range r("gfblock.gated_ff_backward");
+  return ff->dtype == GF_BF16 ? gfb::ff_backward<__nv_bfloat16>(*ff, pl, st) : gfb::ff_backward<__half>(*ff, pl, st);
+}
+
+gf_status gf_dropout(int64_t rows, int64_t cols, int32_t dtype, const gf_dropout_rule* rule, const void* x,
+                     int64_t x_row_stride, int64_t x_col_stride, const void* residual, int64_t r_row_stride,
+                     int64_t r_col_stride, void* y, gf_stream stream) {
+  const char* who = "gf_dropout";
+  if (!rule) return gf::fail(GF_ERR_INVALID_ARG, "%s: the rule must be non-null", who);
+  GFB_TRY(gfb::check_rule(who, *rule));
+  if (rows < 0 || cols < 0) return gf::fail(GF_ERR_INVALID_ARG, "%s: sizes must not be negative", who);
+  if (!gfb::known_dtype(dtype)) return gf::fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_F32, GF_BF16 or GF_F16", who);
+  if (rows == 0 || cols == 0) return GF_OK;
+  if (cols > (int64_t(1) << 33) || rows > (int64_t(1) << 62) / cols)
+    return gf::fail(GF_ERR_UNSUPPORTED, "%s: more than 2^33 columns or 2^62 elements", who);
+  if (!x || !y) return gf::fail(GF_ERR_INVALID_ARG, "%s: x and y must be non-null", who);
+  gfb::Range range("gfblock.dropout");
+  const int es = gfb::dtype_size(dtype);
+  gfb::DropoutParams p{};
+  p.rows = rows, p.cols = cols;
+  p.x = x, p.x_rs = x_row_stride, p.x_cs = x_col_stride;
+  p.res = residual, p.r_rs = r_row_stride, p.r_cs = r_col_stride;
+  p.y = y;
+  p.drop = gfb::drop_args(*rule);
+  // 16-byte accesses where every row of every operand starts on such a boundary
+  const bool vec = cols % (16 / es) == 0 && x_col_stride == 1 && gfb::aligned_rows(x, rows, x_row_stride, es) &&
+                   gfb::aligned_rows(y, rows, cols, es) &&
+                   (!residual || (r_col_stride == 1 && gfb::aligned_rows(residual, rows, r_row_stride, es)));
+  const bool by_rows = x_col_stride > x_row_stride && x_row_stride > 0;
+  const int sms = gfb::sm_count();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == GF_F32) gfb::launch_dropout<float>(p, vec, by_rows, sms, st);
+  else if (dtype == GF_BF16) gfb::launch_dropout<__nv_bfloat16>(p, vec, by_rows, sms, st);
+  else gfb::launch_dropout<__half>(p, vec, by_rows, sms, st);
+  GFB_CUDA(cudaGetLastError());
+  return GF_OK;
+}
+
+gf_status gf_quantize_rows(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q,
+                           float* scale, gf_stream stream) {
+  const char* who = "gf_quantize_rows";
+  if (rows < 0 || cols <= 0) return gf::fail(GF_ERR_INVALID_ARG, "%s: sizes must be positive (rows may be 0)", who);
+  if (cols > gfb::kMaxDim) return gf::fail(GF_ERR_UNSUPPORTED, "%s: cols is above 2^31 - 512", who);
+  if (!gfb::known_dtype(dtype)) return gf::fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_F32, GF_BF16 or GF_F16", who);
+  if (ld_x < cols || ld_q < cols) return gf::fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
+  if (rows == 0) return GF_OK;
+  if (!x || !q || !scale) return gf::fail(GF_ERR_INVALID_ARG, "%s: x, q and scale must be non-null", who);
+  gfb::Range range("gfblock.quantize_rows");
+  const int sms = gfb::sm_count();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == GF_F32) gfb::launch_quantize<float>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (dtype == GF_BF16) gfb::launch_quantize<__nv_bfloat16>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else gfb::launch_quantize<__half>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  GFB_CUDA(cudaGetLastError());
+  return GF_OK;
+}
+
+size_t gf_int8_product_workspace_bytes(const gf_int8_product* p) {
+  if (gfb::check_int8(p) != GF_OK) return 0;
+  return p->m == 0 ? 256 : gfb::plan_int8(*p, nullptr).bytes;
+}
+
+gf_status gf_int8_matmul(const gf_int8_product* d, void* workspace, size_t workspace_bytes, gf_stream stream) {
+  const char* who = "gf_int8_matmul";
+  GFB_TRY(gfb::check_int8(d));
+  if (d->m == 0) return GF_OK;
+  if (!d->a || !d->b || !d->a_scale || !d->b_scale || !d->out)
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: a, b, a_scale, b_scale and out must be non-null", who);
+  const gfb::Int8Plan pl = gfb::plan_int8(*d, static_cast<char*>(workspace));
+  GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
+  gfb::Range range("gfblock.int8_matmul");
+  const int sms = gfb::sm_count(), es = gfb::dtype_size(d->dtype);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  gfb::Operand a{d->a, d->m, d->k, d->ld_a}, b{d->b, d->n, d->k, d->ld_b};
+  const int64_t ld = gfb::round_up<int64_t>(d->k, 16);
+  if (pl.copy_a) {
+    GFB_TRY(gfb::align_copy<uint8_t>(d->a, d->ld_a, d->m, d->k, pl.a, ld, d->m, 0, 0, sms, st));
+    a = gfb::Operand{pl.a, d->m, d->k, ld};
+  }
+  if (pl.copy_b) {
+    GFB_TRY(gfb::align_copy<uint8_t>(d->b, d->ld_b, d->n, d->k, pl.b, ld, d->n, 0, 0, sms, st));
+    b = gfb::Operand{pl.b, d->n, d->k, ld};
+  }
+  gfb::GemmParams p{};
+  GFB_TRY(gfb::set_operands(p, pl.shape, a, false, b, false, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, tc::kAccS32, tc::kFmtS8,
+                            false));
+  p.M = (int)d->m;
+  p.N = (int)d->n;
+  p.kb_total = (int)gfb::ceil_div(d->k, 128);
+  p.out = d->out;
+  p.ld_out = d->ld_out;
+  p.vec_out = gfb::aligned_rows(d->out, 2, d->ld_out, es) && d->n % (16 / es) == 0;
+  p.bias = d->bias;
+  p.a_scale = d->a_scale;
+  p.b_scale = d->b_scale;
+  if (d->dtype == GF_F32) return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, float, 0, false>>(p, sms, st);
+  if (d->dtype == GF_BF16) return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, __nv_bfloat16, 0, false>>(p, sms, st);
+  return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, __half, 0, false>>(p, sms, st);
+}
+
+gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out) {
+  if (!flags_out) return gf::fail(GF_ERR_INVALID_ARG, "gf_block_status: flags_out must be non-null");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const uint32_t zero = 0;
+  uint32_t flags = 0;
+  GFB_CUDA(cudaMemcpyFromSymbolAsync(&flags, gfb::g_status, sizeof(flags), 0, cudaMemcpyDeviceToHost, st));
+  GFB_CUDA(cudaStreamSynchronize(st));
+  if (reset) {
+    GFB_CUDA(cudaMemcpyToSymbolAsync(gfb::g_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st));
+    GFB_CUDA(cudaStreamSynchronize(st));
+  }
+  *flags_out = flags;
+  return GF_OK;
+}
+
+}  // extern "C"
