@@ -71,6 +71,11 @@ def parse_args():
                          "reference layer's base GEMM + row-chunked delta GEMMs (reference); every layer rendering "
                          "itself through the drop-in runtime, the reference's call pattern (dropin)")
     ap.add_argument("--batch", type=int, default=4, help="cfg4: samples per GPU")
+    ap.add_argument("--feed-forward", choices=["composed", "kernel"], default="composed",
+                    help="cfg4: the transformer blocks' feed-forward as torch operations or as the fused kernels of "
+                         "guass_b200.feedforward")
+    ap.add_argument("--dropout", type=float, default=0.0,
+                    help="cfg4: training dropout of the transformer blocks (guass_b200.dropout)")
     ap.add_argument("--bwd-exp", choices=["expf", "ex2"], default="ex2",
                     help="backward basis: the base-2 hardware approximation (GF_CFG_BWD_EXP2, default; held to the "
                          "same gradient tolerance) or CUDA expf as the reference; the line reports both")
@@ -762,7 +767,7 @@ def train_arm(a, rank: int, world: int, local: int) -> None:
     from guass_b200.partition import field_costs
 
     L = _lib.lib()
-    cfg = sd15.UNetConfig()
+    cfg = sd15.UNetConfig(feed_forward=a.feed_forward, dropout=a.dropout)
     torch.manual_seed(0)  # identical base weights on every rank
     with torch.device("cuda"):
         model = sd15.SD15UNet(cfg, dtype=torch.bfloat16)
@@ -893,6 +898,7 @@ def train_arm(a, rank: int, world: int, local: int) -> None:
                        "latent": [cfg.latent_channels, cfg.latent_size, cfg.latent_size],
                        "text": [cfg.text_tokens, cfg.cross_dim], "adapters": nf, "K": cfg.num_gaussians,
                        "delta_elements": elements, "evals": evals, "adapter_apply": a.adapter_apply,
+                       "feed_forward": a.feed_forward, "dropout": a.dropout,
                        "render_bases": "ex2.approx (forward and backward)" if fast else "expf",
                        "parallelism": f"dp{world}: flat NCCL all-reduce of Gaussian-parameter gradients"
                        if world > 1 else "single GPU", "optimizer": "AdamW on mu_raw/chol_raw/amp",

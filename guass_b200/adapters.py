@@ -168,7 +168,8 @@ class BatchedAdapters:
     ``modules`` maps names to adapter modules (``GaussianLinear``); their
     shapes and K fix the batch: after densify changes a K,
     :meth:`shapes_changed` is true and :meth:`rebuilt` returns the binding for
-    the new K.  :meth:`freeze` / :meth:`merge_into_weights` serve inference.
+    the new K.  :meth:`freeze` / :meth:`merge_into_weights` /
+    :meth:`quantize_merged` serve inference.
     ``batch_factory(shapes, **cfg)`` builds the batch (default:
     :class:`~guass_b200.batched.FieldBatch` on the modules' device).
 
@@ -305,6 +306,32 @@ class BatchedAdapters:
             m.weight.sub_(dw)
         self._merged = []
         self._current = None
+
+    @torch.no_grad()
+    def quantize_merged(self):
+        """Inference: serve every layer from ``W0 + adapter_scale * delta``
+        held in 8 bits (one scale per output channel; the activations are
+        quantised per token at each call,
+        :class:`guass_b200.int8.Int8Linear`).  The modules keep their base
+        weights; undo with :meth:`unquantize`."""
+        from guass_b200.int8 import Int8Linear
+
+        if getattr(self, "_int8", None):
+            raise RuntimeError("quantize_merged: the layers are already served in 8 bits")
+        self._int8 = []
+        for m, d in zip(self.modules, self.render()):
+            w = d.float() if self.fused else m.weight.float() + d.float()
+            self._int8.append((m, m.__dict__.get("forward"), Int8Linear.from_weight(w, m.bias)))
+        for m, _, layer in self._int8:
+            m.forward = layer.forward
+
+    def unquantize(self):
+        for m, forward, _ in getattr(self, "_int8", None) or []:
+            if forward is None:
+                m.__dict__.pop("forward", None)
+            else:
+                m.forward = forward
+        self._int8 = None
 
     def render(self):
         """Render every adapter's delta (autograd-connected) and return the

@@ -117,4 +117,5 @@ class Int8Linear(nn.Module):
         return cls(q, scale, None if bias is None else bias.detach().clone())
 
     def forward(self, x):
-        return int8_linear(x, self.q_weight, self.weight_scale, self.bias)
+        bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
+        return int8_linear(x, self.q_weight, self.weight_scale, bias)

@@ -34,6 +34,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from guass_b200 import synthetic
+from guass_b200.dropout import dropout
+from guass_b200.feedforward import gated_feed_forward
 
 
 @dataclass
@@ -48,6 +50,18 @@ class UNetConfig:
     latent_size: int = 64
     groups: int = 32
     num_gaussians: int = 256
+    # feed-forward blocks: torch operations ("composed") or the fused kernels of
+    # guass_b200.feedforward ("kernel"; CUDA, bf16 or fp16)
+    feed_forward: str = "composed"
+    # training dropout of both attention branches and of the feed-forward's
+    # hidden activations (guass_b200.dropout; CUDA)
+    dropout: float = 0.0
+
+    def __post_init__(self):
+        if self.feed_forward not in ("composed", "kernel"):
+            raise ValueError(f"feed_forward must be 'composed' or 'kernel', got {self.feed_forward!r}")
+        if not 0.0 <= self.dropout < 1.0:
+            raise ValueError(f"dropout must be in [0, 1), got {self.dropout}")
 
 
 def tiny_config() -> UNetConfig:
@@ -125,8 +139,13 @@ class Attention(nn.Module):
 
 
 class TransformerBlock(nn.Module):
-    def __init__(self, ch, cfg: UNetConfig, proj):
+    """Self-attention, cross-attention and the gated feed-forward.  ``index``
+    numbers the block in its model: its three dropouts use the sites 4 * index
+    (self-attention), + 1 (cross-attention) and + 2 (feed-forward)."""
+
+    def __init__(self, ch, cfg: UNetConfig, proj, index: int = 0):
         super().__init__()
+        self.fused_ff, self.p, self.site = cfg.feed_forward == "kernel", cfg.dropout, 4 * index
         self.norm = nn.GroupNorm(cfg.groups, ch, eps=1e-6)
         self.proj_in = nn.Conv2d(ch, ch, 1)
         self.norm1, self.norm2, self.norm3 = nn.LayerNorm(ch), nn.LayerNorm(ch), nn.LayerNorm(ch)
@@ -136,14 +155,27 @@ class TransformerBlock(nn.Module):
         self.ff_out = nn.Linear(4 * ch, ch)
         self.proj_out = nn.Conv2d(ch, ch, 1)
 
-    def forward(self, x, ctx):
+    def _branch(self, t, out, seed, site):
+        """t + dropout(out), without dropout when ``seed`` is None."""
+        return t + out if seed is None else dropout(out, self.p, seed, site=site, residual=t)
+
+    def feed_forward(self, x, seed=None):
+        """Gated feed-forward of ``x``, its hidden activations dropped by ``seed``."""
+        p, site = (0.0, 0) if seed is None else (self.p, self.site + 2)
+        if self.fused_ff:
+            return gated_feed_forward(x, self.ff_in.weight, self.ff_out.weight, self.ff_in.bias, self.ff_out.bias,
+                                      dropout_p=p, seed=0 if seed is None else seed, site=site)
+        a, gate = self.ff_in(x).chunk(2, dim=-1)
+        h = a * F.gelu(gate)
+        return self.ff_out(h if seed is None else dropout(h, p, seed, site=site))
+
+    def forward(self, x, ctx, seed=None):
         b, c, hh, ww = x.shape
         res = x
         t = self.proj_in(self.norm(x)).flatten(2).transpose(1, 2)
-        t = t + self.attn1(self.norm1(t))
-        t = t + self.attn2(self.norm2(t), ctx)
-        a, gate = self.ff_in(self.norm3(t)).chunk(2, dim=-1)
-        t = t + self.ff_out(a * F.gelu(gate))
+        t = self._branch(t, self.attn1(self.norm1(t)), seed, self.site)
+        t = self._branch(t, self.attn2(self.norm2(t), ctx), seed, self.site + 1)
+        t = t + self.feed_forward(self.norm3(t), seed)
         return self.proj_out(t.transpose(1, 2).reshape(b, c, hh, ww)) + res
 
 
@@ -184,6 +216,12 @@ class SD15UNet(nn.Module):
             counter[0] += 1
             return GaussianProjection(i, o, bias, cfg.num_gaussians, counter[0], dtype, settings)
 
+        blocks = [0]
+
+        def transformer(c):
+            blocks[0] += 1
+            return TransformerBlock(c, cfg, proj, blocks[0] - 1)
+
         chs = cfg.block_channels
         c0, tdim = chs[0], 4 * chs[0]
         self.conv_in = nn.Conv2d(cfg.latent_channels, c0, 3, padding=1)
@@ -196,13 +234,13 @@ class SD15UNet(nn.Module):
                 level.append(ResBlock(ch, c, tdim, cfg.groups))
                 ch = c
                 if cfg.attn_levels[i]:
-                    level.append(TransformerBlock(ch, cfg, proj))
+                    level.append(transformer(ch))
                 skips.append(ch)
             if i != len(chs) - 1:
                 level.append(nn.Conv2d(ch, ch, 3, stride=2, padding=1))
                 skips.append(ch)
             self.down.append(level)
-        self.mid = nn.ModuleList([ResBlock(ch, ch, tdim, cfg.groups), TransformerBlock(ch, cfg, proj),
+        self.mid = nn.ModuleList([ResBlock(ch, ch, tdim, cfg.groups), transformer(ch),
                                   ResBlock(ch, ch, tdim, cfg.groups)])
         self.up = nn.ModuleList()
         for i in reversed(range(len(chs))):
@@ -212,7 +250,7 @@ class SD15UNet(nn.Module):
                 level.append(ResBlock(ch + skips.pop(), c, tdim, cfg.groups))
                 ch = c
                 if cfg.attn_levels[i]:
-                    level.append(TransformerBlock(ch, cfg, proj))
+                    level.append(transformer(ch))
             if i != 0:
                 level.append(nn.Conv2d(ch, ch, 3, padding=1))  # after a nearest x2 upsample
             self.up.append(level)
@@ -222,11 +260,15 @@ class SD15UNet(nn.Module):
             if not name.endswith(("mu_raw", "chol_raw", "amp")):
                 p.requires_grad_(False)
                 p.data = p.data.to(dtype)
+        # the dropouts' seed lives on the device, so that a captured step can advance it
+        self.register_buffer("dropout_seed", torch.zeros(1, dtype=torch.int64) if cfg.dropout else None,
+                             persistent=False)
 
     def adapters(self) -> dict:
         return {n: m for n, m in self.named_modules() if isinstance(m, GaussianProjection)}
 
     def forward(self, x, t, ctx):
+        seed = self.dropout_seed if self.training else None
         temb = self.time2(F.silu(self.time1(timestep_embedding(t, self.cfg.block_channels[0]).to(x.dtype))))
         h = self.conv_in(x)
         skips = [h]
@@ -237,18 +279,18 @@ class SD15UNet(nn.Module):
                     if not self.cfg.attn_levels[i]:
                         skips.append(h)
                 elif isinstance(blk, TransformerBlock):
-                    h = blk(h, ctx)
+                    h = blk(h, ctx, seed)
                     skips.append(h)
                 else:  # downsample
                     h = blk(h)
                     skips.append(h)
-        h = self.mid[2](self.mid[1](self.mid[0](h, temb), ctx), temb)
+        h = self.mid[2](self.mid[1](self.mid[0](h, temb), ctx, seed), temb)
         for level in self.up:
             for blk in level:
                 if isinstance(blk, ResBlock):
                     h = blk(torch.cat([h, skips.pop()], dim=1), temb)
                 elif isinstance(blk, TransformerBlock):
-                    h = blk(h, ctx)
+                    h = blk(h, ctx, seed)
                 else:  # upsample
                     h = blk(F.interpolate(h, scale_factor=2.0, mode="nearest"))
         return self.conv_out(F.silu(self.norm_out(h)))
@@ -337,9 +379,13 @@ class DataParallelTrainer:
     forward + epsilon MSE, backward (the renderer's batched backward gives the
     Gaussian-parameter gradients), one flat all-reduce of those gradients
     averaged over the ranks (:func:`guass_b200.adapters.allreduce_adapter_grads`),
-    AdamW step.  Returns the detached loss."""
+    AdamW step.  Returns the detached loss.
 
-    def __init__(self, model: SD15UNet, bank, lr: float = 1e-4, world: int = 1, group=None):
+    A model with dropout draws new masks each step: its seed starts at
+    ``seed`` (offset by the rank, so that ranks drop independently) and is
+    advanced on the device after every :meth:`step`."""
+
+    def __init__(self, model: SD15UNet, bank, lr: float = 1e-4, world: int = 1, group=None, seed: int = 0):
         from guass_b200.adapters import adapter_parameters
 
         self.model, self.bank, self.world, self.group = model, bank, world, group
@@ -349,6 +395,9 @@ class DataParallelTrainer:
         self.alphas_cumprod = noise_schedule(self.params[0].device)
         # optional list of (start, end) CUDA events around each step's all-reduce
         self.allreduce_events = None
+        if model.dropout_seed is not None:
+            rank = torch.distributed.get_rank(group) if world > 1 else 0
+            model.dropout_seed.fill_(seed + (rank << 40))
 
     def backward(self, inputs: StepInputs) -> torch.Tensor:
         """Render, forward, backward and gradient all-reduce (no optimizer step)."""
@@ -372,4 +421,6 @@ class DataParallelTrainer:
         loss = self.backward(inputs)
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
+        if self.model.dropout_seed is not None:
+            self.model.dropout_seed.add_(1)
         return loss

@@ -189,3 +189,19 @@ def test_reference_mask_is_the_generator():
         for c in range(10):
             w = ref.philox([c // 4, r, 6, 0], [0x23456789, 0x1])[c % 4]
             assert bool(keep[r, c]) == (w >= round(0.4 * 2 ** 32))
+
+
+def test_model_options():
+    from guass_b200 import sd15
+
+    with pytest.raises(ValueError, match="feed_forward"):
+        sd15.UNetConfig(feed_forward="fast")
+    with pytest.raises(ValueError, match="dropout"):
+        sd15.UNetConfig(dropout=1.0)
+    model = sd15.SD15UNet(sd15.tiny_config(), dtype=torch.float32)
+    assert model.dropout_seed is None and "dropout_seed" not in model.state_dict()
+    cfg = sd15.tiny_config()
+    cfg.feed_forward = "kernel"
+    blk = sd15.TransformerBlock(32, cfg, lambda i, o, b: torch.nn.Linear(i, o, b))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        blk.feed_forward(torch.zeros(1, 2, 32, dtype=torch.bfloat16))
