@@ -133,23 +133,41 @@ gf_status check_rule(const char* who, const gf_dropout_rule& r) {
 }
 
 // ---------------------------------------------------------------------------
-// activations: value and slope
+// activations, two arguments at a time: value and slope.
+//
+// gelu: with z = |g| / sqrt(2), erfc(z) = P(t) exp(-z^2), t = 1 / (1 + p z)
+// (Abramowitz and Stegun 7.1.26, off by at most 1.5e-7).  Its exponential is
+// also the density in the slope Phi(g) + g phi(g).  silu: g / (1 + exp(-g)).
+// Both take one base-2 exponential and one reciprocal of the special-function
+// unit per argument, a few 2^-22 relative, far inside the 16-bit rounding.
 
-template <int ACT>
-__device__ __forceinline__ float act_value(float g) {
-  if constexpr (ACT == GF_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678f));
-  else return g / (1.0f + expf(-g));
-}
-template <int ACT>
-__device__ __forceinline__ void act_both(float g, float& value, float& slope) {
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void activate(float g0, float g1, uint64_t& value, uint64_t& slope) {
+  using namespace tc;
+  const uint64_t g = pack_f2(g0, g1);
   if constexpr (ACT == GF_ACT_GELU) {
-    const float cdf = 0.5f * (1.0f + erff(g * 0.70710678f));
-    value = g * cdf;
-    slope = cdf + g * 0.39894228f * expf(-0.5f * g * g);
+    constexpr float kP = 0.3275911f * 0.70710678118654752f;
+    const uint64_t t = pack_f2(rcp(fmaf(fabsf(g0), kP, 1.0f)), rcp(fmaf(fabsf(g1), kP, 1.0f)));
+    constexpr float kE = -0.72134752044448170f;  // -log2(e) / 2
+    const float2 x = unpack_f2(mul_f2(mul_f2(g, pack_f2(kE, kE)), g));
+    const uint64_t e = pack_f2(ex2(x.x), ex2(x.y));
+    // half of P(t), by Horner's rule
+    uint64_t q = pack_f2(0.5f * 1.061405429f, 0.5f * 1.061405429f);
+    q = fma_f2(q, t, pack_f2(0.5f * -1.453152027f, 0.5f * -1.453152027f));
+    q = fma_f2(q, t, pack_f2(0.5f * 1.421413741f, 0.5f * 1.421413741f));
+    q = fma_f2(q, t, pack_f2(0.5f * -0.284496736f, 0.5f * -0.284496736f));
+    q = fma_f2(q, t, pack_f2(0.5f * 0.254829592f, 0.5f * 0.254829592f));
+    const float2 tail = unpack_f2(mul_f2(mul_f2(q, t), e));  // Phi(-|g|)
+    const uint64_t cdf = pack_f2(g0 > 0.0f ? 1.0f - tail.x : tail.x, g1 > 0.0f ? 1.0f - tail.y : tail.y);
+    value = mul_f2(g, cdf);
+    if constexpr (SLOPE) slope = fma_f2(mul_f2(g, pack_f2(0.3989422804f, 0.3989422804f)), e, cdf);
   } else {
-    const float sig = 1.0f / (1.0f + expf(-g));
-    value = g * sig;
-    slope = sig * (1.0f + g * (1.0f - sig));
+    constexpr float kE = -1.4426950408889634f;
+    const float2 x = unpack_f2(mul_f2(g, pack_f2(kE, kE)));
+    const uint64_t sig = pack_f2(rcp(1.0f + ex2(x.x)), rcp(1.0f + ex2(x.y)));
+    value = mul_f2(g, sig);
+    // sig (1 + g (1 - sig)) = sig + value - value sig
+    if constexpr (SLOPE) slope = add_f2(sig, fma_f2(value, mul_f2(sig, pack_f2(-1.0f, -1.0f)), value));
   }
 }
 
@@ -169,15 +187,18 @@ constexpr int kABytes = kTileM * 128;
 constexpr int kStageBytes = kABytes + kMaxN * 128;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kPitch = 80;                        // staging: 64 bytes of each of a warp's 32 rows, spread over the banks
-constexpr int kWarpStage = 32 * kPitch + 2 * 32 * 4;  // and two vectors of 32 floats (bias, scales)
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kWarpStage + 256;
+constexpr int kRowsBytes = 32 * 64;              // staging: 64 bytes of each of a warp's 32 rows
+constexpr int kWarpStage = 2 * kRowsBytes;       // two of them: one is filled while the other is written out
+constexpr int kWarpVectors = 2 * 32 * 4;         // two vectors of 32 floats (biases, scales)
+constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * (kWarpStage + kWarpVectors) + 256;
+static_assert(kSmemBytes <= 232448, "shared memory of one SM");
 constexpr uint32_t kTmemCols = 512;
 
 enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
 
 struct alignas(64) GemmParams {
   CUtensorMap ma, mb;
+  CUtensorMap mo, mu;            // tiles of 64 bytes x 32 rows: result (or partial products), and u
   int32_t M, N;                // rows and columns of the result (gated: columns of h, without padding)
   int32_t tiles_m, tiles_n, splits, kb_total, kb_split;
   int32_t bn;                  // columns of the MMA
@@ -186,15 +207,14 @@ struct alignas(64) GemmParams {
   int32_t gate_row;            // gated: row of B where the gate half starts
   uint32_t idesc, tx_bytes;
   int32_t seg_pad, seg;        // result rows come in two runs of `seg` rows, the second starting at seg_pad (0: one run)
-  int32_t vec_out;             // rows of out are 16-byte aligned and whole 16-byte pieces
+  int32_t tma_out;             // the result is written through mo (its rows are 16-byte aligned, in one run)
   int64_t ld_out;
-  void* out;                   // STORE, INT8: result; GATED: h; GATED_BWD: du
-  float* partial;              // splits > 1: [splits][M][ld_partial]
+  void* out;                   // STORE, INT8: result
+  float* partial;              // splits > 1: [splits][tiles_m * 128][ld_partial]
   int64_t ld_partial;
   const void* bias;            // [N] (gated: [2 N])
-  void* u;                     // GATED: written when not null; GATED_BWD: read
+  void* u;                     // GATED: written (through mu) when not null; GATED_BWD: read
   int32_t hp;                  // gated: padded hidden size
-  int32_t bias_dtype;
   const float* a_scale;
   const float* b_scale;
   DropArgs drop;
@@ -204,61 +224,6 @@ struct Pipe {  // barriers and the abort flag, in shared memory
   uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
   uint32_t tmem, abort;
 };
-
-// Writes 64 bytes of each of this warp's 32 rows: lane = row in `v`, to rows
-// of `ld` bytes at `dst`, through the staging rows so that four lanes write
-// one row's 64 bytes.  `rows` rows and `bytes` bytes of each are written.
-template <int ES>
-__device__ __forceinline__ void store_rows(char* stage, const uint32_t (&v)[16], char* dst, int64_t ld, int rows,
-                                           int bytes, bool vec) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(stage + lane * kPitch + 16 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  __syncwarp();
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2), b = (lane & 3) * 16;
-      if (r < rows && b < bytes)
-        *reinterpret_cast<uint4*>(dst + r * ld + b) = *reinterpret_cast<const uint4*>(stage + r * kPitch + b);
-    }
-  } else {
-    constexpr int per_row = 64 / ES;
-    for (int i = lane; i < 32 * per_row; i += 32) {
-      const int r = i / per_row, b = (i % per_row) * ES;
-      if (r < rows && b < bytes) {
-        if constexpr (ES == 2)
-          *reinterpret_cast<uint16_t*>(dst + r * ld + b) = *reinterpret_cast<const uint16_t*>(stage + r * kPitch + b);
-        else
-          *reinterpret_cast<uint32_t*>(dst + r * ld + b) = *reinterpret_cast<const uint32_t*>(stage + r * kPitch + b);
-      }
-    }
-  }
-  __syncwarp();
-}
-
-// The reverse for reading: four lanes load one row's 64 bytes (16-byte aligned
-// rows), each lane then holds its own row.  Split in two so that the loads of
-// a chunk are in flight while the previous one is computed.
-__device__ __forceinline__ void fetch_rows(uint4 (&v)[4], const char* src, int64_t ld, int rows) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + (lane >> 2), b = (lane & 3) * 16;
-    v[i] = r < rows ? *reinterpret_cast<const uint4*>(src + r * ld + b) : make_uint4(0, 0, 0, 0);
-  }
-}
-__device__ __forceinline__ void turn_rows(char* stage, uint4 (&v)[4]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    *reinterpret_cast<uint4*>(stage + (8 * i + (lane >> 2)) * kPitch + (lane & 3) * 16) = v[i];
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(stage + lane * kPitch + 16 * i);
-  __syncwarp();
-}
 
 struct Tile {
   int m0, n0, split, kb0, kb1;
@@ -279,180 +244,275 @@ template <int EPI, typename T, int ACT, bool DROP>
 struct EpilogueWarp {
   const GemmParams& p;
   char* stage;
-  float* vec0;  // two vectors of 32 floats behind the staging rows
+  float* vec0;  // two vectors of 32 floats
   float* vec1;
-  Philox rng;
   const int lane;
+  Philox rng;
+  uint32_t out = 0;  // blocks of rows written
 
-  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* s)
-      : p(p_), stage(s), vec0(reinterpret_cast<float*>(s + 32 * kPitch)), vec1(vec0 + 32), rng(p_.drop),
-        lane(threadIdx.x & 31) {}
+  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors)
+      : p(p_), stage(stage_), vec0(reinterpret_cast<float*>(vectors)), vec1(vec0 + 32), lane(threadIdx.x & 31),
+        rng(p_.drop) {}
 
-  // one 32-column chunk at result column n of rows m .. m + 31
-  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int c, uint4 (&uv)[4], uint4 (&ug)[4]) {
-    const int n = t.n0 + c;
-    const int rows = min(32, p.M - m);
+  // Bias and scale of this lane's column of a chunk, fetched ahead.
+  struct Ahead {
+    float a, b;
+    uint4 u[2][4];  // GATED_BWD: the chunk's saved rows, four lanes to a row
+  };
+  __device__ __forceinline__ void fetch(Ahead& x, int m, int n) const {
+    const int left = p.N - n;
+    x.a = x.b = 0.0f;
+    if constexpr (EPI == EPI_GATED_BWD) {
+      const char* u = static_cast<const char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        const char* at = u + r * 4 * (int64_t)p.hp + (lane & 3) * 16;
+        const bool in = m + r < p.M;
+        x.u[0][i] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+        x.u[1][i] = in ? *reinterpret_cast<const uint4*>(at + 2 * (int64_t)p.hp) : make_uint4(0, 0, 0, 0);
+      }
+    } else if (lane < left) {
+      const T* bias = static_cast<const T*>(p.bias);
+      if (bias) x.a = to_float(bias[n + lane]);
+      if (EPI == EPI_GATED && bias) x.b = to_float(bias[p.N + n + lane]);
+      if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
+    }
+  }
+
+  // One 32-column chunk at result column n of rows m .. m + 31, from the
+  // accumulator columns at `acc`.  `release` runs once they are read.
+  template <typename Release>
+  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int n, const Ahead& ahead, Release release) {
+    uint32_t d[32];
+    tc::tmem_load32(d, acc);
     if constexpr (EPI == EPI_STORE) {
-      uint32_t d[32];
-      tc::tmem_load32(d, acc + c);
       tc::tmem_wait();
+      release();
       if (p.splits > 1) {
+        const int row = t.split * p.tiles_m * kTileM + m;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = d[16 * h + i];
-          char* dst = reinterpret_cast<char*>(p.partial + ((int64_t)t.split * p.M + m) * p.ld_partial + n + 16 * h);
-          store_rows<4>(stage, v, dst, 4 * p.ld_partial, rows, 64, true);
+          write(v, &p.mo, n + 16 * h, row);
         }
         return;
       }
-      bias_vector(n, p.N - n, p.bias, vec0);
+      vectors(ahead);
       uint32_t v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        v[i] = pack2<T>(__uint_as_float(d[2 * i]) + vec0[2 * i], __uint_as_float(d[2 * i + 1]) + vec0[2 * i + 1]);
-      store_result<2>(v, m, n, rows, min(64, 2 * (p.N - n)));
+      for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f(d[2 * i]) + vec0[2 * i], f(d[2 * i + 1]) + vec0[2 * i + 1]);
+      result<2>(v, m, n);
     } else if constexpr (EPI == EPI_INT8) {
-      uint32_t d[32];
-      tc::tmem_load32(d, acc + c);
+      const float s = m + lane < p.M ? p.a_scale[m + lane] : 0.0f;
+      vectors(ahead);
       tc::tmem_wait();
-      bias_vector(n, p.N - n, p.bias, vec0);
-      __syncwarp();
-      vec1[lane] = n + lane < p.N ? p.b_scale[n + lane] : 0.0f;
-      __syncwarp();
-      const float s = lane < rows ? p.a_scale[m + lane] : 0.0f;
-      float f[32];
+      release();
+      // |sum| < 2^31: one rounding to fp32, then the two scales and the bias
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = (float)(int)d[i] * s * vec1[i] + vec0[i];
+      for (int i = 0; i < 32; ++i) d[i] = __float_as_uint((float)(int)d[i] * s * vec1[i] + vec0[i]);
+      uint32_t v[16];
       if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(f[16 * h + i]);
-          store_result<4>(v, m, n + 16 * h, rows, min(64, 4 * (p.N - n - 16 * h)));
+          for (int i = 0; i < 16; ++i) v[i] = d[16 * h + i];
+          result<4>(v, m, n + 16 * h);
         }
       } else {
-        uint32_t v[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
-        store_result<2>(v, m, n, rows, min(64, 2 * (p.N - n)));
+        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f(d[2 * i]), f(d[2 * i + 1]));
+        result<2>(v, m, n);
       }
     } else if constexpr (EPI == EPI_GATED) {
-      uint32_t a[32], g[32];
-      tc::tmem_load32(a, acc + c);
-      tc::tmem_load32(g, acc + p.cols + c);
+      uint32_t g[32];
+      tc::tmem_load32(g, acc + p.cols);
+      vectors(ahead);
       tc::tmem_wait();
-      const int left = p.N - n;  // columns before the padding
-      bias_vector(n, left, p.bias, vec0);
-      bias_vector(p.N + n, left, p.bias, vec1);
+      release();
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        a[i] = __float_as_uint(__uint_as_float(a[i]) + vec0[i]);
-        g[i] = __float_as_uint(__uint_as_float(g[i]) + vec1[i]);
+        d[i] = __float_as_uint(f(d[i]) + vec0[i]);
+        g[i] = __float_as_uint(f(g[i]) + vec1[i]);
       }
-      if (left < 32) {
+      if (p.N - n < 32) {  // the padding columns of h and u are zeros
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (i >= left) a[i] = g[i] = 0u;
+          if (i >= p.N - n) d[i] = g[i] = 0u;
       }
-      uint32_t v[16];
-      if (p.u) {
-        char* u = static_cast<char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
-        store_rows<2>(stage, v, u, 4 * (int64_t)p.hp, rows, 64, true);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = pack2<T>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-        store_rows<2>(stage, v, u + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows, 64, true);
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          h[i] = __uint_as_float(a[4 * q + i]) * act_value<ACT>(__uint_as_float(g[4 * q + i]));
-        if constexpr (DROP) drop(h, m + lane, n + 4 * q);
-        v[2 * q] = pack2<T>(h[0], h[1]);
-        v[2 * q + 1] = pack2<T>(h[2], h[3]);
-      }
-      store_rows<2>(stage, v, static_cast<char*>(p.out) + 2 * ((int64_t)m * p.hp + n), 2 * (int64_t)p.hp, rows, 64, true);
+      if (p.u) gated<true>(d, g, m, n);
+      else gated<false>(d, g, m, n);
     } else {
-      turn_rows(stage, uv);
-      turn_rows(stage, ug);
-      uint32_t d[32];
-      tc::tmem_load32(d, acc + c);
+      uint32_t v[16], w[16];
+      turn(v, ahead.u[0]);
       tc::tmem_wait();
-      const int left = p.N - n;
-      uint32_t dv[16], dg[16];
-      const uint32_t* pv = reinterpret_cast<const uint32_t*>(uv);
-      const uint32_t* pg = reinterpret_cast<const uint32_t*>(ug);
+      release();
+      // du_value = dh * u_value, du_gate = dh * u_gate (see gated)
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        float h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = 4 * q + i < left ? __uint_as_float(d[4 * q + i]) : 0.0f;
-        if constexpr (DROP) drop(h, m + lane, n + 4 * q);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 a = unpack2<T>(pv[2 * q + i]), g = unpack2<T>(pg[2 * q + i]);
-          float v0, s0, v1, s1;
-          act_both<ACT>(g.x, v0, s0);
-          act_both<ACT>(g.y, v1, s1);
-          dv[2 * q + i] = pack2<T>(h[2 * i] * v0, h[2 * i + 1] * v1);
-          dg[2 * q + i] = pack2<T>(h[2 * i] * a.x * s0, h[2 * i + 1] * a.y * s1);
-        }
+      for (int i = 0; i < 16; ++i) {
+        const float2 a = unpack2<T>(v[i]);
+        w[i] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
       }
-      char* du = static_cast<char*>(p.out) + 2 * ((int64_t)m * 2 * p.hp + n);
-      store_rows<2>(stage, dv, du, 4 * (int64_t)p.hp, rows, 64, true);
-      store_rows<2>(stage, dg, du + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows, 64, true);
+      turn(v, ahead.u[1]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 a = unpack2<T>(v[i]);
+        v[i] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
+      }
+      write(w, &p.mo, n, m);
+      write(v, &p.mo, p.hp + n, m);
     }
   }
 
-  __device__ __forceinline__ void fetch_u(int m, int n, uint4 (&uv)[4], uint4 (&ug)[4]) {
-    const char* u = static_cast<const char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
-    const int rows = min(32, p.M - m);
-    fetch_rows(uv, u, 4 * (int64_t)p.hp, rows);
-    fetch_rows(ug, u + 2 * (int64_t)p.hp, 4 * (int64_t)p.hp, rows);
+  // Every block must be out of shared memory before the CTA ends.
+  __device__ __forceinline__ void finish() {
+    if (lane == 0) tc::tma_store_drain();
+    __syncwarp();
   }
 
  private:
-  __device__ __forceinline__ void bias_vector(int at, int left, const void* bias, float* vec) {
-    float b = 0.0f;
-    if (bias && lane < left) b = to_float(static_cast<const T*>(bias)[at + lane]);
+  static __device__ __forceinline__ float f(uint32_t v) { return __uint_as_float(v); }
+
+  __device__ __forceinline__ void vectors(const Ahead& x) {
     __syncwarp();
-    vec[lane] = b;
+    vec0[lane] = x.a;
+    vec1[lane] = x.b;
     __syncwarp();
   }
-  __device__ __forceinline__ void drop(float (&h)[4], int row, int col) {
-    const uint4 w = rng((uint32_t)col >> 2, (uint32_t)row);
-    h[0] = w.x >= p.drop.threshold ? h[0] * p.drop.scale : 0.0f;
-    h[1] = w.y >= p.drop.threshold ? h[1] * p.drop.scale : 0.0f;
-    h[2] = w.z >= p.drop.threshold ? h[2] * p.drop.scale : 0.0f;
-    h[3] = w.w >= p.drop.threshold ? h[3] * p.drop.scale : 0.0f;
+
+  // h = keep * value * act(gate); saved for the backward (SAVE): what the
+  // gradient of h is multiplied with, keep * act(gate) and keep * value *
+  // act'(gate).  keep is 1 / (1 - p) or 0, so that the backward needs neither
+  // the activation nor the mask again, for the bytes that value and gate
+  // themselves would take.
+  template <bool SAVE>
+  __device__ __forceinline__ void gated(const uint32_t (&a)[32], const uint32_t (&g)[32], int m, int n) {
+    uint32_t h[16], sv[16], sg[16];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      uint64_t keep[2];
+      if constexpr (DROP) {
+        const uint4 w = rng((uint32_t)(n + 4 * q) >> 2, (uint32_t)(m + lane));
+        const uint32_t th = p.drop.threshold;
+        const float s = p.drop.scale;
+        keep[0] = tc::pack_f2(w.x >= th ? s : 0.0f, w.y >= th ? s : 0.0f);
+        keep[1] = tc::pack_f2(w.z >= th ? s : 0.0f, w.w >= th ? s : 0.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = 4 * q + 2 * i;
+        uint64_t value, slope = 0;
+        activate<ACT, SAVE>(f(g[c]), f(g[c + 1]), value, slope);
+        if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
+        const uint64_t x = tc::pack_f2(f(a[c]), f(a[c + 1]));
+        float2 r = tc::unpack_f2(tc::mul_f2(x, value));
+        h[c / 2] = pack2<T>(r.x, r.y);
+        if constexpr (SAVE) {
+          slope = tc::mul_f2(x, slope);
+          if constexpr (DROP) slope = tc::mul_f2(slope, keep[i]);
+          r = tc::unpack_f2(value);
+          sv[c / 2] = pack2<T>(r.x, r.y);
+          r = tc::unpack_f2(slope);
+          sg[c / 2] = pack2<T>(r.x, r.y);
+        }
+      }
+    }
+    write(h, &p.mo, n, m);
+    if constexpr (SAVE) {
+      write(sv, &p.mu, n, m);
+      write(sg, &p.mu, p.hp + n, m);
+    }
   }
-  // result rows m .. m + rows - 1, honouring the two runs of rows of seg_pad
+
+  // Writes 64 bytes of each of the 32 rows, lane = row in `v`, through a
+  // staging block whose 16-byte pieces are swizzled as the tensor map says
+  // (piece ^ (row / 2 % 4): eight lanes then cover all banks).
+  __device__ __forceinline__ void write(const uint32_t (&v)[16], const CUtensorMap* map, int x, int y) {
+    char* s = stage + (out & 1) * kRowsBytes;
+    ++out;
+    if (lane == 0) tc::tma_store_wait<1>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(s + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    tc::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store(map, tc::smem_addr(s), x, y);
+      tc::tma_store_commit();
+    }
+  }
+
+  // The reverse turn, of rows fetched by four lanes each (GATED_BWD).
+  __device__ __forceinline__ void turn(uint32_t (&v)[16], const uint4 (&u)[4]) {
+    if (lane == 0) tc::tma_store_wait<0>();
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2), c = lane & 3;
+      *reinterpret_cast<uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = u[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 w = *reinterpret_cast<const uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
+      v[4 * i] = w.x, v[4 * i + 1] = w.y, v[4 * i + 2] = w.z, v[4 * i + 3] = w.w;
+    }
+    __syncwarp();
+  }
+
+  // A piece of the result: 64 bytes of rows m .. m + 31 from column n.
   template <int ES>
-  __device__ __forceinline__ void store_result(const uint32_t (&v)[16], int m, int n, int rows, int bytes) {
-    int64_t out_row = m;
-    if (p.seg_pad) {  // seg_pad is a multiple of 64, so 32 rows never straddle the runs
+  __device__ __forceinline__ void result(const uint32_t (&v)[16], int m, int n) {
+    if (n >= p.N) return;
+    if (p.tma_out) {
+      write(v, &p.mo, n, m);
+      return;
+    }
+    // rows off the 16-byte grid, or in two runs (seg_pad is a multiple of 64:
+    // 32 rows never straddle them): element by element, a row's together
+    int rows = min(32, p.M - m);
+    int64_t row = m;
+    if (p.seg_pad) {
       const int in = m >= p.seg_pad ? m - p.seg_pad : m;
       rows = min(rows, p.seg - in);
-      out_row = m >= p.seg_pad ? (int64_t)p.seg + in : in;
+      row = m >= p.seg_pad ? (int64_t)p.seg + in : in;
     }
-    store_rows<ES>(stage, v, static_cast<char*>(p.out) + ES * (out_row * p.ld_out + n), ES * p.ld_out, rows, bytes,
-                   p.vec_out);
+    constexpr int per_row = 64 / ES;
+    const int cols = min(per_row, p.N - n);
+    char* dst = static_cast<char*>(p.out) + ES * (row * p.ld_out + n);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+    for (int i = lane; i < 32 * per_row; i += 32) {
+      const int r = i / per_row, c = i % per_row, b = c * ES;
+      if (r < rows && c < cols) {
+        const char* src = stage + r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
+        if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint16_t*>(src);
+        else *reinterpret_cast<uint32_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint32_t*>(src);
+      }
+    }
+    __syncwarp();
   }
 };
 
 template <int EPI, typename T, int ACT, bool DROP>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  extern __shared__ char smem_raw[];
-  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) char smem[];
   char* staging = smem + kStages * kStageBytes;
-  Pipe* pipe = reinterpret_cast<Pipe*>(staging + kEpiWarps * kWarpStage);
+  char* vectors = staging + kEpiWarps * kWarpStage;
+  Pipe* pipe = reinterpret_cast<Pipe*>(vectors + kEpiWarps * kWarpVectors);
   const uint32_t base = tc::smem_addr(smem);
+  if (base & 1023u) {  // the operand tiles' swizzle needs it; the kernel has no other shared memory
+    if (threadIdx.x == 0) atomicOr(&g_status, GF_FLAG_TIMEOUT);
+    return;
+  }
   const uint32_t full = tc::smem_addr(pipe->full), empty = tc::smem_addr(pipe->empty);
   const uint32_t acc_full = tc::smem_addr(pipe->acc_full), acc_empty = tc::smem_addr(pipe->acc_empty);
   volatile uint32_t* abort = &pipe->abort;
@@ -546,31 +606,39 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     }
   } else {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * kWarpStage);
+    EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * kWarpStage, vectors + (warp - 2) * kWarpVectors);
+    // gated: the padding columns of h, u and du are written too (zeros)
+    const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
     uint32_t it = 0;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++it) {
       const Tile t = tile_of(p, item);
       const uint32_t buf = it & 1;
       const int m = t.m0 + 32 * quarter;
+      const int c_end = m < p.M ? min(p.cols, n_end - t.n0) : 0;
       const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + buf * kMaxN;
-      uint4 uv[4], ug[4];
-      if constexpr (EPI == EPI_GATED_BWD) {
-        if (32 * half < p.cols && t.n0 + 32 * half < p.hp) epi.fetch_u(m, t.n0 + 32 * half, uv, ug);
-      }
+      const uint32_t freed = acc_empty + 8 * buf;
+      int c = 32 * half;
+      typename decltype(epi)::Ahead ahead;
+      if (c < c_end) epi.fetch(ahead, m, t.n0 + c);
       if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
       tc::fence_after();
-      // gated: the padding columns of h, u and du are written too (zeros)
-      const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
-      for (int c = 32 * half; c < p.cols && t.n0 + c < n_end; c += 64) {
-        epi.chunk(acc, t, m, c, uv, ug);
-        if constexpr (EPI == EPI_GATED_BWD) {
-          if (c + 64 < p.cols && t.n0 + c + 64 < p.hp) epi.fetch_u(m, t.n0 + c + 64, uv, ug);
-        }
+      bool held = true;
+      auto release = [&](bool last) {
+        if (!last) return;
+        tc::fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(freed);
+        held = false;
+      };
+      for (; c < c_end; c += 64) {
+        const bool last = c + 64 >= c_end;
+        const auto now = ahead;
+        if (!last) epi.fetch(ahead, m, t.n0 + c + 64);
+        epi.chunk(acc + c, t, m, t.n0 + c, now, [&] { release(last); });
       }
-      tc::fence_before();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) tc::mbar_arrive(acc_empty + 8 * buf);
+      if (held) release(true);  // no chunk of this tile was this warp's
     }
+    epi.finish();
   }
   __syncwarp();
   tc::fence_before();
@@ -609,7 +677,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
     }
     float4 s = make_float4(0, 0, 0, 0);
     for (int k = 0; k < p.splits; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.M + m) * p.ld_partial + n);
+      const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.tiles_m * kTileM + m) * p.ld_partial + n);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
     const float f[4] = {s.x, s.y, s.z, s.w};
@@ -618,7 +686,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
     T r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = from_float<T>(f[j] + (bias && n + j < p.N ? to_float(bias[n + j]) : 0.0f));
-    if (p.vec_out) {  // N is then a multiple of 4
+    if (p.N % 8 == 0 && p.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0) {
       *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(r);
     } else {
       for (int j = 0; j < 4 && n + j < p.N; ++j) out[j] = r[j];
@@ -856,7 +924,8 @@ inline bool aligned_rows(const void* ptr, int64_t rows, int64_t ld, int es) {
   return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0 && (rows == 1 || (ld * es) % 16 == 0);
 }
 
-gf_status make_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type, int es, int box_cols, int box_rows) {
+gf_status make_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type, int es, int box_cols, int box_rows,
+                   CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeFn encode;
   if (const gf_status s = encode_fn(&encode); s != GF_OK) return s;
   const int64_t ld = o.rows == 1 ? round_up<int64_t>(o.cols * es, 16) : o.ld * es;
@@ -864,7 +933,7 @@ gf_status make_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type,
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, unit[2] = {1, 1};
   auto run = [&] {
     return encode(map, type, 2, const_cast<void*>(o.ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = run();
   if (r == CUDA_ERROR_INVALID_CONTEXT) {  // a thread that has made no runtime call yet (autograd's): give it the context
@@ -877,6 +946,11 @@ gf_status make_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type,
     return fail(GF_ERR_CUDA, "cuTensorMapEncodeTiled(%lld x %lld, ld %lld): error %d", (long long)o.rows, (long long)o.cols,
                 (long long)o.ld, (int)r);
   return GF_OK;
+}
+
+// Where the epilogue writes 64 bytes of 32 rows at a time.
+gf_status make_out_map(CUtensorMap* map, const Operand& o, CUtensorMapDataType type, int es) {
+  return make_map(map, o, type, es, 64 / es, 32, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int sm_count() {
@@ -921,8 +995,8 @@ Shape choose_shape(int64_t M, int64_t N, int64_t kb, bool gated, bool may_split,
   return best;
 }
 
-inline size_t partial_bytes(const Shape& s, int64_t M, int64_t N) {
-  return s.splits > 1 ? round_up<size_t>((size_t)s.splits * M * round_up<int64_t>(N, 32) * 4, 256) : 0;
+inline size_t partial_bytes(const Shape& s, int64_t N) {
+  return s.splits > 1 ? (size_t)s.splits * s.tiles_m * kTileM * round_up<int64_t>(N, 32) * 4 : 0;
 }
 
 template <auto Kernel>
@@ -1015,14 +1089,14 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
   if (p.copy_w_out) p.w_out = b.take(2 * p.O * round_up<int64_t>(p.F, 8));
   if (p.copy_dy) p.dy = b.take(2 * p.M * round_up<int64_t>(p.O, 8));
   size_t partial = 0, sums = 0;
-  auto need = [&](const Shape& s, int64_t M, int64_t N) {
-    const size_t n = partial_bytes(s, M, N);
+  auto need = [&](const Shape& s, int64_t N) {
+    const size_t n = partial_bytes(s, N);
     if (n > partial) partial = n;
   };
   if (!back) {
     p.in = choose_shape(p.M, p.Hp, ceil_div(p.D, 64), true, false, sms);
     p.out = choose_shape(p.M, p.O, ceil_div(p.F, 64), false, true, sms);
-    need(p.out, p.M, p.O);
+    need(p.out, p.O);
   } else {
     if (use_du) {
       p.du = b.take(2 * p.M * 2 * p.Hp);
@@ -1030,15 +1104,15 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
     }
     if (f.dx) {
       p.dx = choose_shape(p.M, p.D, 2 * p.Hp / 64, false, true, sms);
-      need(p.dx, p.M, p.D);
+      need(p.dx, p.D);
     }
     if (f.dw_in) {
       p.dw_in = choose_shape(2 * p.Hp, p.D, ceil_div(p.M, 64), false, true, sms);
-      need(p.dw_in, 2 * p.Hp, p.D);
+      need(p.dw_in, p.D);
     }
     if (f.dw_out) {
       p.dw_out = choose_shape(p.O, p.F, ceil_div(p.M, 64), false, true, sms);
-      need(p.dw_out, p.O, p.F);
+      need(p.dw_out, p.F);
     }
     if (f.db_in) {
       column_runs(p.M, 2 * p.Hp, sms, &p.in_parts, &p.in_run);
@@ -1145,12 +1219,17 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
   p.kb_total = (int)ceil_div(K, 64);
   p.out = out;
   p.ld_out = ld_out;
-  p.vec_out = aligned_rows(out, 2, ld_out, 2) && N % 8 == 0;
+  p.tma_out = aligned_rows(out, M, ld_out, 2) && !seg_pad;
   p.bias = bias;
   p.seg_pad = (int)seg_pad;
   p.seg = (int)seg;
   p.partial = static_cast<float*>(partial);
   p.ld_partial = round_up<int64_t>(N, 32);
+  if (s.splits > 1)
+    GFB_TRY(make_out_map(&p.mo, Operand{partial, (int64_t)s.splits * s.tiles_m * kTileM, p.ld_partial, p.ld_partial},
+                         CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4));
+  else if (p.tma_out)
+    GFB_TRY(make_out_map(&p.mo, Operand{out, M, N, ld_out}, map_type<T>(), 2));
   GFB_TRY((launch_gemm<gemm_kernel<EPI_STORE, T, 0, false>>(p, sms, st)));
   if (s.splits > 1) {
     join_kernel<T><<<grid_for(M * (p.ld_partial / 4), 256, sms), 256, 0, st>>>(p);
@@ -1159,16 +1238,13 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
   return GF_OK;
 }
 
-template <typename T, int ACT, bool DROP>
-gf_status gated(GemmParams& p, bool back, int sms, cudaStream_t st) {
-  return back ? launch_gemm<gemm_kernel<EPI_GATED_BWD, T, ACT, DROP>>(p, sms, st)
-              : launch_gemm<gemm_kernel<EPI_GATED, T, ACT, DROP>>(p, sms, st);
-}
 template <typename T>
-gf_status gated(GemmParams& p, bool back, int act, int sms, cudaStream_t st) {
+gf_status gated(const GemmParams& p, int act, int sms, cudaStream_t st) {
   if (act == GF_ACT_GELU)
-    return p.drop.on ? gated<T, GF_ACT_GELU, true>(p, back, sms, st) : gated<T, GF_ACT_GELU, false>(p, back, sms, st);
-  return p.drop.on ? gated<T, GF_ACT_SILU, true>(p, back, sms, st) : gated<T, GF_ACT_SILU, false>(p, back, sms, st);
+    return p.drop.on ? launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_GELU, true>>(p, sms, st)
+                     : launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_GELU, false>>(p, sms, st);
+  return p.drop.on ? launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_SILU, true>>(p, sms, st)
+                   : launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_SILU, false>>(p, sms, st);
 }
 
 template <typename T>
@@ -1185,9 +1261,10 @@ gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   p.kb_total = (int)ceil_div(pl.D, 64);
   p.bias = f.b_in;
   p.u = f.u;
-  p.out = f.h;
   p.drop = drop_args(f.dropout);
-  GFB_TRY(gated<T>(p, false, f.activation, sms, st));
+  GFB_TRY(make_out_map(&p.mo, Operand{f.h, pl.M, pl.Hp, pl.Hp}, map_type<T>(), 2));
+  if (f.u) GFB_TRY(make_out_map(&p.mu, Operand{f.u, pl.M, 2 * pl.Hp, 2 * pl.Hp}, map_type<T>(), 2));
+  GFB_TRY(gated<T>(p, f.activation, sms, st));
   return product<T>(pl.out, Operand{f.h, pl.M, pl.Hp, pl.Hp}, false, o.w_out, false, pl.M, pl.O, pl.F, f.y, f.ld_y, f.b_out,
                     0, 0, pl.partial, sms, st);
 }
@@ -1220,9 +1297,8 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
     p.hp = (int)pl.Hp;
     p.kb_total = (int)ceil_div(pl.O, 64);
     p.u = f.u;
-    p.out = pl.du;
-    p.drop = drop_args(f.dropout);
-    GFB_TRY(gated<T>(p, true, f.activation, sms, st));
+    GFB_TRY(make_out_map(&p.mo, du, map_type<T>(), 2));
+    GFB_TRY((launch_gemm<gemm_kernel<EPI_GATED_BWD, T, 0, false>>(p, sms, st)));
   }
   if (f.dx)
     GFB_TRY(product<T>(pl.dx, du, false, o.w_in, true, pl.M, pl.D, 2 * pl.Hp, f.dx, pl.D, nullptr, 0, 0, pl.partial, sms, st));
@@ -1439,7 +1515,13 @@ gf_status gf_int8_matmul(const gf_int8_product* d, void* workspace, size_t works
   p.kb_total = (int)gfb::ceil_div(d->k, 128);
   p.out = d->out;
   p.ld_out = d->ld_out;
-  p.vec_out = gfb::aligned_rows(d->out, 2, d->ld_out, es) && d->n % (16 / es) == 0;
+  p.tma_out = gfb::aligned_rows(d->out, d->m, d->ld_out, es);
+  if (p.tma_out)
+    GFB_TRY(gfb::make_out_map(&p.mo, gfb::Operand{d->out, d->m, d->n, d->ld_out},
+                              d->dtype == GF_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : d->dtype == GF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              es));
   p.bias = d->bias;
   p.a_scale = d->a_scale;
   p.b_scale = d->b_scale;

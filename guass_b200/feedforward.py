@@ -7,8 +7,9 @@ input projections, the activation, the product and the dropout are one kernel;
 the output projection is a second.  Matrices are bf16 or fp16, products
 accumulate in fp32.
 
-The backward keeps the rounded projections and regenerates the dropout mask.
-It computes only the gradients that are asked for: with frozen weights (how
+The training forward saves, in the room the two projections would take, what
+the backward multiplies with: the activation and its slope times the value,
+each with the dropout folded in.  The backward computes only the gradients that are asked for: with frozen weights (how
 the Gaussian adapters are trained) that is two kernels.
 """
 from __future__ import annotations
