@@ -172,35 +172,54 @@ __device__ __forceinline__ void activate(float g0, float g1, uint64_t& value, ui
 }
 
 // ---------------------------------------------------------------------------
-// The product kernel.  D[m, n] = sum_k A(m, k) B(n, k) on 128 x bn tiles:
+// The product kernel.  D[m, n] = sum_k A(m, k) B(n, k), persistent and
+// warp-specialised, on tiles of 128 x bn for one CTA or 256 x bn for a pair:
 //  warp 0      TMA producer: 64 k (128 bytes) of both operands per stage
 //  warp 1      issues tcgen05.mma into one of two TMEM accumulators
-//  warps 2-9   epilogue of the other accumulator (warp w reads TMEM lanes
-//              32 * (w % 4) onwards; the two warps of a quarter take the
-//              32-column chunks in turn)
-// Each CTA walks over tiles (and K ranges) with a stride of the grid.
+//  the others  epilogue of the other accumulator: warp w reads TMEM lanes
+//              32 * (w % 4) onwards, and the warps of a quarter take its
+//              32-column chunks in turn
+// Each CTA (or pair) walks over tiles and K ranges with a stride of the grid.
+//
+// Why pairs: a CTA's tile of 128 x 256 takes (128 + 256) * 128 bytes of
+// operands every 512 clocks of products, 96 bytes a clock, and the way from L2
+// into an SM gave about 70; in a pair each CTA loads its own rows of A and
+// half of B, 64 bytes a clock.
 
-constexpr int kTileM = 128;
+constexpr int kTileM = 128;   // rows of a CTA
 constexpr int kMaxN = 256;
-constexpr int kStages = 4;
 constexpr int kABytes = kTileM * 128;
-constexpr int kStageBytes = kABytes + kMaxN * 128;
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kRowsBytes = 32 * 64;              // staging: 64 bytes of each of a warp's 32 rows
-constexpr int kWarpStage = 2 * kRowsBytes;       // two of them: one is filled while the other is written out
-constexpr int kWarpVectors = 2 * 32 * 4;         // two vectors of 32 floats (biases, scales)
-constexpr int kSmemBytes = kStages * kStageBytes + kEpiWarps * (kWarpStage + kWarpVectors) + 256;
-static_assert(kSmemBytes <= 232448, "shared memory of one SM");
+constexpr int kRowsBytes = 32 * 64;     // staging block: 64 bytes of each of a warp's 32 rows
+constexpr int kWarpVectors = 2 * 32 * 4;  // two vectors of 32 floats (biases, scales)
 constexpr uint32_t kTmemCols = 512;
+constexpr int kSmemLimit = 232448;
 
 enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
+
+// Warps and shared memory of a variant.  The gated epilogue does about 25
+// instructions for each element of h and hides their latencies behind 16
+// warps; the others do little, and keep 8 warps with room for more registers.
+// Staging blocks: two for results (one fills while the other is written out),
+// and two for the saved rows that the backward's epilogue turns.
+template <int EPI, bool PAIR>
+struct Config {
+  static constexpr int epi_warps = EPI == EPI_GATED ? 16 : 8;
+  static constexpr int threads = 64 + 32 * epi_warps;
+  static constexpr int blocks = EPI == EPI_GATED_BWD ? 4 : 2;
+  static constexpr int warp_bytes = blocks * kRowsBytes + kWarpVectors;
+  static constexpr int stage_bytes = kABytes + (PAIR ? kMaxN / 2 : kMaxN) * 128;
+  static constexpr int stages = (kSmemLimit - 512 - epi_warps * warp_bytes) / stage_bytes;
+  static constexpr int smem_bytes = stages * stage_bytes + epi_warps * warp_bytes + 512;
+  static_assert(stages >= 3 && smem_bytes <= kSmemLimit, "shared memory of one SM");
+};
+constexpr int kMaxStages = 8;
 
 struct alignas(64) GemmParams {
   CUtensorMap ma, mb;
   CUtensorMap mo, mu;            // tiles of 64 bytes x 32 rows: result (or partial products), and u
   int32_t M, N;                // rows and columns of the result (gated: columns of h, without padding)
   int32_t tiles_m, tiles_n, splits, kb_total, kb_split;
+  int32_t rows_m;              // rows of all tiles of M
   int32_t bn;                  // columns of the MMA
   int32_t cols;                // columns of the result per tile: bn, or bn / 2 (gated: value and gate side by side)
   int32_t a_mn, b_mn;          // operand is M/N-contiguous
@@ -221,18 +240,20 @@ struct alignas(64) GemmParams {
 };
 
 struct Pipe {  // barriers and the abort flag, in shared memory
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   uint32_t tmem, abort;
 };
+static_assert(sizeof(Pipe) <= 512, "the room behind the staging blocks");
 
-struct Tile {
+struct Tile {  // m0: first row of this CTA
   int m0, n0, split, kb0, kb1;
 };
-__device__ __forceinline__ Tile tile_of(const GemmParams& p, int64_t item) {
+template <bool PAIR>
+__device__ __forceinline__ Tile tile_of(const GemmParams& p, int64_t item, uint32_t rank) {
   Tile t;
   const int n = (int)(item % p.tiles_n);
   const int64_t rest = item / p.tiles_n;
-  t.m0 = (int)(rest % p.tiles_m) * kTileM;
+  t.m0 = ((int)(rest % p.tiles_m) * (PAIR ? 2 : 1) + rank) * kTileM;
   t.split = (int)(rest / p.tiles_m);
   t.n0 = n * p.cols;
   t.kb0 = t.split * p.kb_split;
@@ -285,12 +306,12 @@ struct EpilogueWarp {
   template <typename Release>
   __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int n, const Ahead& ahead, Release release) {
     uint32_t d[32];
-    tc::tmem_load32(d, acc);
+    if constexpr (EPI != EPI_GATED) tc::tmem_load32(d, acc);
     if constexpr (EPI == EPI_STORE) {
       tc::tmem_wait();
       release();
       if (p.splits > 1) {
-        const int row = t.split * p.tiles_m * kTileM + m;
+        const int row = t.split * p.rows_m + m;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t v[16];
@@ -327,39 +348,20 @@ struct EpilogueWarp {
         result<2>(v, m, n);
       }
     } else if constexpr (EPI == EPI_GATED) {
-      uint32_t g[32];
-      tc::tmem_load32(g, acc + p.cols);
       vectors(ahead);
-      tc::tmem_wait();
-      release();
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        d[i] = __float_as_uint(f(d[i]) + vec0[i]);
-        g[i] = __float_as_uint(f(g[i]) + vec1[i]);
-      }
-      if (p.N - n < 32) {  // the padding columns of h and u are zeros
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i >= p.N - n) d[i] = g[i] = 0u;
-      }
-      if (p.u) gated<true>(d, g, m, n);
-      else gated<false>(d, g, m, n);
+      if (p.u) gated<true>(acc, m, n, release);
+      else gated<false>(acc, m, n, release);
     } else {
       uint32_t v[16], w[16];
-      turn(v, ahead.u[0]);
+      turn(w, v, ahead.u);
       tc::tmem_wait();
       release();
       // du_value = dh * u_value, du_gate = dh * u_gate (see gated)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float2 a = unpack2<T>(v[i]);
+        const float2 a = unpack2<T>(w[i]), g = unpack2<T>(v[i]);
         w[i] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
-      }
-      turn(v, ahead.u[1]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 a = unpack2<T>(v[i]);
-        v[i] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
+        v[i] = pack2<T>(f(d[2 * i]) * g.x, f(d[2 * i + 1]) * g.y);
       }
       write(w, &p.mo, n, m);
       write(v, &p.mo, p.hp + n, m);
@@ -387,36 +389,57 @@ struct EpilogueWarp {
   // act'(gate).  keep is 1 / (1 - p) or 0, so that the backward needs neither
   // the activation nor the mask again, for the bytes that value and gate
   // themselves would take.
-  template <bool SAVE>
-  __device__ __forceinline__ void gated(const uint32_t (&a)[32], const uint32_t (&g)[32], int m, int n) {
+  template <bool SAVE, typename Release>
+  __device__ __forceinline__ void gated(uint32_t acc, int m, int n, Release release) {
     uint32_t h[16], sv[16], sg[16];
+    const int left = p.N - n;  // the padding columns of h and u are zeros
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      uint64_t keep[2];
-      if constexpr (DROP) {
-        const uint4 w = rng((uint32_t)(n + 4 * q) >> 2, (uint32_t)(m + lane));
-        const uint32_t th = p.drop.threshold;
-        const float s = p.drop.scale;
-        keep[0] = tc::pack_f2(w.x >= th ? s : 0.0f, w.y >= th ? s : 0.0f);
-        keep[1] = tc::pack_f2(w.z >= th ? s : 0.0f, w.w >= th ? s : 0.0f);
-      }
+    for (int half = 0; half < 2; ++half) {
+      uint32_t a[16], g[16];
+      tc::tmem_load16(a, acc + 16 * half);
+      tc::tmem_load16(g, acc + p.cols + 16 * half);
+      tc::tmem_wait();
+      if (half == 1) release();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = 4 * q + 2 * i;
-        uint64_t value, slope = 0;
-        activate<ACT, SAVE>(f(g[c]), f(g[c + 1]), value, slope);
-        if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
-        const uint64_t x = tc::pack_f2(f(a[c]), f(a[c + 1]));
-        float2 r = tc::unpack_f2(tc::mul_f2(x, value));
-        h[c / 2] = pack2<T>(r.x, r.y);
-        if constexpr (SAVE) {
-          slope = tc::mul_f2(x, slope);
-          if constexpr (DROP) slope = tc::mul_f2(slope, keep[i]);
-          r = tc::unpack_f2(value);
-          sv[c / 2] = pack2<T>(r.x, r.y);
-          r = tc::unpack_f2(slope);
-          sg[c / 2] = pack2<T>(r.x, r.y);
+      for (int q = 0; q < 4; ++q) {
+        uint64_t keep[2];
+        if constexpr (DROP) {
+          const uint4 w = rng((uint32_t)(n + 16 * half + 4 * q) >> 2, (uint32_t)(m + lane));
+          const uint32_t th = p.drop.threshold;
+          const float s = p.drop.scale;
+          keep[0] = tc::pack_f2(w.x >= th ? s : 0.0f, w.y >= th ? s : 0.0f);
+          keep[1] = tc::pack_f2(w.z >= th ? s : 0.0f, w.w >= th ? s : 0.0f);
         }
+        const float4 b0 = *reinterpret_cast<const float4*>(vec0 + 16 * half + 4 * q);
+        const float4 b1 = *reinterpret_cast<const float4*>(vec1 + 16 * half + 4 * q);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = 4 * q + 2 * i, o = 8 * half + 2 * q + i;
+          uint64_t x = tc::add_f2(tc::pack_f2(f(a[c]), f(a[c + 1])), i ? tc::pack_f2(b0.z, b0.w) : tc::pack_f2(b0.x, b0.y));
+          float2 y = tc::unpack_f2(
+              tc::add_f2(tc::pack_f2(f(g[c]), f(g[c + 1])), i ? tc::pack_f2(b1.z, b1.w) : tc::pack_f2(b1.x, b1.y)));
+          uint64_t value, slope = 0;
+          activate<ACT, SAVE>(y.x, y.y, value, slope);
+          if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
+          float2 r = tc::unpack_f2(tc::mul_f2(x, value));
+          h[o] = pack2<T>(r.x, r.y);
+          if constexpr (SAVE) {
+            slope = tc::mul_f2(x, slope);
+            if constexpr (DROP) slope = tc::mul_f2(slope, keep[i]);
+            r = tc::unpack_f2(value);
+            sv[o] = pack2<T>(r.x, r.y);
+            r = tc::unpack_f2(slope);
+            sg[o] = pack2<T>(r.x, r.y);
+          }
+        }
+      }
+    }
+    if (left < 32) {
+#pragma unroll
+      for (int o = 0; o < 16; ++o) {
+        const uint32_t mask = 2 * o + 1 < left ? 0xFFFFFFFFu : 2 * o < left ? 0xFFFFu : 0u;
+        h[o] &= mask;
+        if constexpr (SAVE) sv[o] &= mask, sg[o] &= mask;
       }
     }
     write(h, &p.mo, n, m);
@@ -446,22 +469,24 @@ struct EpilogueWarp {
     }
   }
 
-  // The reverse turn, of rows fetched by four lanes each (GATED_BWD).
-  __device__ __forceinline__ void turn(uint32_t (&v)[16], const uint4 (&u)[4]) {
-    if (lane == 0) tc::tma_store_wait<0>();
+  // The reverse turn of the two blocks of rows that four lanes each fetched
+  // (GATED_BWD), through staging blocks of their own.
+  __device__ __forceinline__ void turn(uint32_t (&v)[16], uint32_t (&w)[16], const uint4 (&u)[2][4]) {
+    char* s = stage + 2 * kRowsBytes;
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2), c = lane & 3;
-      *reinterpret_cast<uint4*>(stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = u[i];
+    for (int i = 0; i < 8; ++i) {
+      const int r = 8 * (i & 3) + (lane >> 2), c = lane & 3;
+      *reinterpret_cast<uint4*>(s + (i >> 2) * kRowsBytes + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = u[i >> 2][i & 3];
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint4 w = *reinterpret_cast<const uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4));
-      v[4 * i] = w.x, v[4 * i + 1] = w.y, v[4 * i + 2] = w.z, v[4 * i + 3] = w.w;
+      const char* at = s + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
+      const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + kRowsBytes);
+      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+      w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
     }
-    __syncwarp();
   }
 
   // A piece of the result: 64 bytes of rows m .. m + 31 from column n.
@@ -502,12 +527,15 @@ struct EpilogueWarp {
   }
 };
 
-template <int EPI, typename T, int ACT, bool DROP>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+template <int EPI, typename T, int ACT, bool DROP, bool PAIR>
+__global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  using C = Config<EPI, PAIR>;
+  constexpr int kStages = C::stages;
+  static_assert(kStages <= kMaxStages, "barriers");
   extern __shared__ __align__(1024) char smem[];
-  char* staging = smem + kStages * kStageBytes;
-  char* vectors = staging + kEpiWarps * kWarpStage;
-  Pipe* pipe = reinterpret_cast<Pipe*>(vectors + kEpiWarps * kWarpVectors);
+  char* staging = smem + kStages * C::stage_bytes;
+  char* vectors = staging + C::epi_warps * C::blocks * kRowsBytes;
+  Pipe* pipe = reinterpret_cast<Pipe*>(vectors + C::epi_warps * kWarpVectors);
   const uint32_t base = tc::smem_addr(smem);
   if (base & 1023u) {  // the operand tiles' swizzle needs it; the kernel has no other shared memory
     if (threadIdx.x == 0) atomicOr(&g_status, GF_FLAG_TIMEOUT);
@@ -517,7 +545,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   const uint32_t acc_full = tc::smem_addr(pipe->acc_full), acc_empty = tc::smem_addr(pipe->acc_empty);
   volatile uint32_t* abort = &pipe->abort;
   const int warp = threadIdx.x >> 5;
+  const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     tc::tma_prefetch(&p.ma);
@@ -528,61 +558,72 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(acc_full + 8 * i, 1);
-      tc::mbar_init(acc_empty + 8 * i, kEpiWarps);
+      tc::mbar_init(acc_empty + 8 * i, C::epi_warps * (PAIR ? 2 : 1));
     }
     pipe->abort = 0;
     tc::fence_barrier_init();
     tc::fence_proxy_async();
   }
-  if (warp == 1) tc::tmem_alloc(tc::smem_addr(&pipe->tmem), kTmemCols);
+  if (warp == 1) tc::tmem_alloc<PAIR>(tc::smem_addr(&pipe->tmem), kTmemCols);
   __syncwarp();
   tc::fence_before();
-  __syncthreads();
+  if constexpr (PAIR) tc::cluster_sync();
+  else __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&pipe->tmem);
 
   if (warp == 0) {
+    // Both CTAs of a pair load; the copies of both count on the first one's barrier.
     if (tc::elect_one()) {
       uint32_t n = 0;  // stages filled
       bool ok = true;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-        const Tile t = tile_of(p, item);
+      const uint32_t full0 = PAIR ? tc::peer_addr(full, 0) : full;
+      const int b_cols = PAIR ? p.bn / 2 : p.bn;
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+        if constexpr (PAIR) tc::tma_load_pair(dst, map, bar, x, y);
+        else tc::tma_load(dst, map, bar, x, y);
+      };
+      for (int64_t item = first; ok && item < items; item += stride) {
+        const Tile t = tile_of<PAIR>(p, item, rank);
+        const int n0 = t.n0 + (PAIR ? (int)rank * b_cols : 0);
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % kStages;
           ok = tc::mbar_wait(empty + 8 * s, ((n / kStages) & 1) ^ 1, abort);
           if (!ok) break;
-          const uint32_t bar = full + 8 * s, a = base + s * kStageBytes, b = a + kABytes;
-          tc::mbar_expect_tx(bar, p.tx_bytes);
+          const uint32_t bar = full0 + 8 * s, a = base + s * C::stage_bytes, b = a + kABytes;
+          if (rank == 0) tc::mbar_expect_tx(full + 8 * s, p.tx_bytes);
           const int k0 = kb * (EPI == EPI_INT8 ? 128 : 64);
           if (p.a_mn) {
-            tc::tma_load(a, &p.ma, bar, t.m0, k0);
-            tc::tma_load(a + tc::kMnGroupBytes, &p.ma, bar, t.m0 + 64, k0);
+            load(a, &p.ma, bar, t.m0, k0);
+            load(a + tc::kMnGroupBytes, &p.ma, bar, t.m0 + 64, k0);
           } else {
-            tc::tma_load(a, &p.ma, bar, k0, t.m0);
+            load(a, &p.ma, bar, k0, t.m0);
           }
-          if (EPI == EPI_GATED) {
-            tc::tma_load(b, &p.mb, bar, k0, t.n0);
-            tc::tma_load(b + p.cols * 128, &p.mb, bar, k0, p.gate_row + t.n0);
+          if (EPI == EPI_GATED) {  // value rows, then gate rows: one half of B each
+            if (!PAIR || rank == 0) load(b, &p.mb, bar, k0, t.n0);
+            if (!PAIR || rank == 1) load(b + (PAIR ? 0 : p.cols * 128), &p.mb, bar, k0, p.gate_row + t.n0);
           } else if (p.b_mn) {
-            for (int i = 0; i < p.bn; i += 64) tc::tma_load(b + 128 * i, &p.mb, bar, t.n0 + i, k0);
+            for (int i = 0; i < b_cols; i += 64) load(b + 128 * i, &p.mb, bar, n0 + i, k0);
           } else {
-            tc::tma_load(b, &p.mb, bar, k0, t.n0);
+            load(b, &p.mb, bar, k0, n0);
           }
         }
       }
-      if (!ok) {  // the copies in flight must land before the CTA ends
+      // The copies in flight must land before the CTA ends.  Every product
+      // waits for its copies, so this matters after a wait that gave up only.
+      if (!ok && rank == 0) {
         volatile uint32_t ignore = 0;
-        const uint32_t first = n > kStages ? n - kStages : 0;
-        for (uint32_t i = first; i < n; ++i) tc::mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, &ignore);
+        const uint32_t from = n > kStages ? n - kStages : 0;
+        for (uint32_t i = from; i < n; ++i) tc::mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, &ignore);
       }
     }
   } else if (warp == 1) {
-    if (tc::elect_one()) {
+    if (rank == 0 && tc::elect_one()) {
       uint32_t n = 0, it = 0;
       bool ok = true;
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x, ++it) {
-        const Tile t = tile_of(p, item);
+      for (int64_t item = first; ok && item < items; item += stride, ++it) {
+        const Tile t = tile_of<PAIR>(p, item, rank);
         const uint32_t buf = it & 1;
         ok = tc::mbar_wait(acc_empty + 8 * buf, ((it >> 1) & 1) ^ 1, abort);
         if (!ok) break;
@@ -593,50 +634,53 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           ok = tc::mbar_wait(full + 8 * s, (n / kStages) & 1, abort);
           if (!ok) break;
           tc::fence_after();
-          const uint32_t a = base + s * kStageBytes;
+          const uint32_t a = base + s * C::stage_bytes;
           const uint64_t da = tc::operand_desc(a, p.a_mn), db = tc::operand_desc(a + kABytes, p.b_mn);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            tc::mma<EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, p.idesc, kb > t.kb0 || i > 0);
-          tc::mma_commit(empty + 8 * s);
+            tc::mma<PAIR, EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, p.idesc, kb > t.kb0 || i > 0);
+          tc::mma_commit<PAIR>(empty + 8 * s);
         }
         if (!ok) break;
-        tc::mma_commit(acc_full + 8 * buf);
+        tc::mma_commit<PAIR>(acc_full + 8 * buf);
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * kWarpStage, vectors + (warp - 2) * kWarpVectors);
+    constexpr int kSets = C::epi_warps / 4;  // warps of a quarter
+    const int quarter = warp & 3, set = (warp - 2) >> 2;
+    EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * C::blocks * kRowsBytes,
+                                        vectors + (warp - 2) * kWarpVectors);
+    const uint32_t empty0 = PAIR ? tc::peer_addr(acc_empty, 0) : acc_empty;
     // gated: the padding columns of h, u and du are written too (zeros)
     const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
     uint32_t it = 0;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x, ++it) {
-      const Tile t = tile_of(p, item);
+    for (int64_t item = first; item < items; item += stride, ++it) {
+      const Tile t = tile_of<PAIR>(p, item, rank);
       const uint32_t buf = it & 1;
       const int m = t.m0 + 32 * quarter;
       const int c_end = m < p.M ? min(p.cols, n_end - t.n0) : 0;
       const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + buf * kMaxN;
-      const uint32_t freed = acc_empty + 8 * buf;
-      int c = 32 * half;
+      int c = 32 * set;
       typename decltype(epi)::Ahead ahead;
       if (c < c_end) epi.fetch(ahead, m, t.n0 + c);
       if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
       tc::fence_after();
-      bool held = true;
       auto release = [&](bool last) {
         if (!last) return;
         tc::fence_before();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(freed);
-        held = false;
+        if ((threadIdx.x & 31) == 0) {
+          if constexpr (PAIR) tc::mbar_arrive_cluster(empty0 + 8 * buf);
+          else tc::mbar_arrive(empty0 + 8 * buf);
+        }
       };
-      for (; c < c_end; c += 64) {
-        const bool last = c + 64 >= c_end;
+      if (c >= c_end) release(true);  // no chunk of this tile is this warp's
+      for (; c < c_end; c += 32 * kSets) {
+        const bool last = c + 32 * kSets >= c_end;
         const auto now = ahead;
-        if (!last) epi.fetch(ahead, m, t.n0 + c + 64);
+        if (!last) epi.fetch(ahead, m, t.n0 + c + 32 * kSets);
         epi.chunk(acc + c, t, m, t.n0 + c, now, [&] { release(last); });
       }
-      if (held) release(true);  // no chunk of this tile was this warp's
     }
     epi.finish();
   }
@@ -646,17 +690,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (threadIdx.x == 0 && *abort) atomicOr(&g_status, GF_FLAG_TIMEOUT);
   if (warp == 1) {
     tc::fence_after();
-    if (*abort) {  // products may still be running: their end is a commit away
+    if (*abort && rank == 0) {  // products may still be running: their end is a commit away
       if (tc::elect_one()) {
         volatile uint32_t ignore = 0;
-        tc::mbar_init(tc::smem_addr(&pipe->acc_full[0]), 1);
-        tc::mma_commit(tc::smem_addr(&pipe->acc_full[0]));
-        tc::mbar_wait(tc::smem_addr(&pipe->acc_full[0]), 0, &ignore);
+        const uint32_t spare = tc::smem_addr(&pipe->empty[kMaxStages - 1]);  // no variant has that many stages
+        static_assert(kStages < kMaxStages, "a spare barrier");
+        tc::mbar_init(spare, 1);
+        tc::mma_commit<false>(spare);
+        tc::mbar_wait(spare, 0, &ignore);
       }
       __syncwarp();
     }
-    tc::tmem_free(tmem, kTmemCols);
   }
+  if constexpr (PAIR) tc::cluster_sync();  // the peer still signals here, and reads this CTA's operands
+  if (warp == 1) tc::tmem_free<PAIR>(tmem, kTmemCols);
 }
 
 // ---------------------------------------------------------------------------
@@ -677,7 +724,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
     }
     float4 s = make_float4(0, 0, 0, 0);
     for (int k = 0; k < p.splits; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.tiles_m * kTileM + m) * p.ld_partial + n);
+      const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.rows_m + m) * p.ld_partial + n);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
     const float f[4] = {s.x, s.y, s.z, s.w};
@@ -963,32 +1010,41 @@ int sm_count() {
   return n;
 }
 
-// Tile width and K ranges.  A CTA's time for one tile is taken as its loads,
-// (128 + bn) * 128 bytes a 64-k step at 64 bytes a clock, plus a fixed cost;
-// the grid's as that of the CTA with most tiles; K ranges add the partial
-// sums' way to memory and back.  Narrower tiles or K ranges win only where
-// wide ones leave SMs idle.
+// Pairs or single CTAs, tile width, K ranges: whichever gives the least
+// estimated time.  A tile takes the longest of its products (2 clocks a
+// column and 64 k), its operands' way into the SM (70 bytes a clock) and its
+// epilogue; the grid's time is that of the CTA with most tiles, the fill of
+// its pipeline and one epilogue; K ranges add the partial products' way to
+// memory and back.
 struct Shape {
+  bool pair;
   int bn, splits, kb_split, tiles_m, tiles_n;
+  int rows_m() const { return tiles_m * kTileM * (pair ? 2 : 1); }
 };
-Shape choose_shape(int64_t M, int64_t N, int64_t kb, bool gated, bool may_split, int sms) {
+Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
   Shape best{};
   double best_cost = 0;
+  const bool gated = epi == EPI_GATED;
   const int step = gated ? 64 : 32;
-  const int64_t tm = ceil_div(M, kTileM);
-  for (int bn = step; bn <= kMaxN; bn += step) {
-    const int cols = gated ? bn / 2 : bn;
-    const int64_t tn = ceil_div(N, cols);
-    if (cols > 32 && cols - 32 >= N) break;  // wider than the result
-    for (int64_t s = 1; s <= (may_split ? kb : 1) && s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
-      const int64_t per = ceil_div(kb, s), parts = ceil_div(kb, per);
-      if (parts != s) continue;
-      const int64_t waves = ceil_div(tm * tn * s, sms);
-      double cost = (double)waves * (per * 2.0 * (128 + bn) + 600.0) + 2.0 * bn;
-      if (s > 1) cost += 4000.0 + (double)(s + 1) * M * N * 4 / 3000.0;
-      if (best.bn == 0 || cost < best_cost) {
-        best_cost = cost;
-        best = Shape{bn, (int)s, (int)per, (int)tm, (int)tn};
+  const double per_col = epi == EPI_GATED ? 34.0 : epi == EPI_GATED_BWD ? 20.0 : epi == EPI_INT8 ? 12.0 : 8.0;
+  for (int pair = 0; pair < 2; ++pair) {
+    const int64_t tm = ceil_div(M, pair ? 2 * kTileM : kTileM), units = pair ? sms / 2 : sms;
+    for (int bn = step; bn <= kMaxN; bn += step) {
+      const int cols = gated ? bn / 2 : bn;
+      if (cols > 32 && cols - 32 >= N) break;  // wider than the result
+      const int64_t tn = ceil_div(N, cols);
+      const double loads = (kTileM + (pair ? bn / 2 : bn)) * 128 / 70.0, products = 2.0 * bn;
+      const double step_cost = loads > products ? loads : products;
+      for (int64_t s = 1; s <= (may_split ? kb : 1) && s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
+        const int64_t per = ceil_div(kb, s);
+        if (ceil_div(kb, per) != s) continue;
+        const double waves = (double)ceil_div(tm * tn * s, units), epilogue = per_col * cols, main = per * step_cost;
+        double cost = waves * ((main > epilogue ? main : epilogue) + 100.0) + 1500.0 + epilogue;
+        if (s > 1) cost += 4000.0 + (double)(s + 1) * M * N * 4 / 3000.0;
+        if (best.bn == 0 || cost < best_cost) {
+          best_cost = cost;
+          best = Shape{pair != 0, bn, (int)s, (int)per, (int)tm, (int)tn};
+        }
       }
     }
   }
@@ -996,23 +1052,44 @@ Shape choose_shape(int64_t M, int64_t N, int64_t kb, bool gated, bool may_split,
 }
 
 inline size_t partial_bytes(const Shape& s, int64_t N) {
-  return s.splits > 1 ? (size_t)s.splits * s.tiles_m * kTileM * round_up<int64_t>(N, 32) * 4 : 0;
+  return s.splits > 1 ? (size_t)s.splits * s.rows_m() * round_up<int64_t>(N, 32) * 4 : 0;
 }
 
-template <auto Kernel>
+template <int EPI, typename T, int ACT, bool DROP, bool PAIR>
 gf_status launch_gemm(const GemmParams& p, int sms, cudaStream_t st) {
+  using C = Config<EPI, PAIR>;
+  const auto kernel = gemm_kernel<EPI, T, ACT, DROP, PAIR>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
   int dev = 0;
   GFB_CUDA(cudaGetDevice(&dev));
   if (dev > 63 || !(ready.load() >> dev & 1)) {
-    GFB_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    GFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_bytes));
     if (dev <= 63) ready.fetch_or(uint64_t(1) << dev);
   }
-  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  Kernel<<<(int)(items < sms ? items : sms), kThreads, kSmemBytes, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(GF_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits, units = PAIR ? sms / 2 : sms;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(items < units ? items : units) * (PAIR ? 2 : 1));
+  cfg.blockDim = dim3(C::threads);
+  cfg.dynamicSmemBytes = C::smem_bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  if (PAIR) {
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(GF_ERR_CUDA, "gemm_kernel: %s", cudaGetErrorString(e));
+  }
   return GF_OK;
+}
+template <int EPI, typename T, int ACT, bool DROP>
+gf_status launch_gemm(const GemmParams& p, const Shape& s, int sms, cudaStream_t st) {
+  return s.pair ? launch_gemm<EPI, T, ACT, DROP, true>(p, sms, st) : launch_gemm<EPI, T, ACT, DROP, false>(p, sms, st);
 }
 
 inline int grid_for(int64_t work, int threads, int sms) {
@@ -1028,15 +1105,17 @@ gf_status set_operands(GemmParams& p, const Shape& s, const Operand& a, bool a_m
   p.tiles_n = s.tiles_n;
   p.splits = s.splits;
   p.kb_split = s.kb_split;
+  p.rows_m = s.rows_m();
   p.bn = s.bn;
   p.cols = gated ? s.bn / 2 : s.bn;
   p.a_mn = a_mn;
   p.b_mn = b_mn;
-  p.idesc = tc::instruction_desc(acc, fmt, a_mn, b_mn, s.bn);
-  p.tx_bytes = kABytes + 128 * (b_mn ? round_up(s.bn, 64) : s.bn);
+  p.idesc = tc::instruction_desc(acc, fmt, a_mn, b_mn, s.bn, s.pair);
+  const int b_cols = s.pair ? s.bn / 2 : s.bn;  // of one CTA
+  p.tx_bytes = (kABytes + 128 * (b_mn ? round_up(b_cols, 64) : b_cols)) * (s.pair ? 2 : 1);
   gf_status r = a_mn ? make_map(&p.ma, a, type, es, 64, 64) : make_map(&p.ma, a, type, es, line, kTileM);
   if (r != GF_OK) return r;
-  return b_mn ? make_map(&p.mb, b, type, es, 64, 64) : make_map(&p.mb, b, type, es, line, p.cols);
+  return b_mn ? make_map(&p.mb, b, type, es, 64, 64) : make_map(&p.mb, b, type, es, line, gated ? p.cols : b_cols);
 }
 
 // ---- the feed-forward block
@@ -1094,24 +1173,24 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
     if (n > partial) partial = n;
   };
   if (!back) {
-    p.in = choose_shape(p.M, p.Hp, ceil_div(p.D, 64), true, false, sms);
-    p.out = choose_shape(p.M, p.O, ceil_div(p.F, 64), false, true, sms);
+    p.in = choose_shape(p.M, p.Hp, ceil_div(p.D, 64), EPI_GATED, false, sms);
+    p.out = choose_shape(p.M, p.O, ceil_div(p.F, 64), EPI_STORE, true, sms);
     need(p.out, p.O);
   } else {
     if (use_du) {
       p.du = b.take(2 * p.M * 2 * p.Hp);
-      p.dh = choose_shape(p.M, p.Hp, ceil_div(p.O, 64), false, false, sms);
+      p.dh = choose_shape(p.M, p.Hp, ceil_div(p.O, 64), EPI_GATED_BWD, false, sms);
     }
     if (f.dx) {
-      p.dx = choose_shape(p.M, p.D, 2 * p.Hp / 64, false, true, sms);
+      p.dx = choose_shape(p.M, p.D, 2 * p.Hp / 64, EPI_STORE, true, sms);
       need(p.dx, p.D);
     }
     if (f.dw_in) {
-      p.dw_in = choose_shape(2 * p.Hp, p.D, ceil_div(p.M, 64), false, true, sms);
+      p.dw_in = choose_shape(2 * p.Hp, p.D, ceil_div(p.M, 64), EPI_STORE, true, sms);
       need(p.dw_in, p.D);
     }
     if (f.dw_out) {
-      p.dw_out = choose_shape(p.O, p.F, ceil_div(p.M, 64), false, true, sms);
+      p.dw_out = choose_shape(p.O, p.F, ceil_div(p.M, 64), EPI_STORE, true, sms);
       need(p.dw_out, p.F);
     }
     if (f.db_in) {
@@ -1226,11 +1305,11 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
   p.partial = static_cast<float*>(partial);
   p.ld_partial = round_up<int64_t>(N, 32);
   if (s.splits > 1)
-    GFB_TRY(make_out_map(&p.mo, Operand{partial, (int64_t)s.splits * s.tiles_m * kTileM, p.ld_partial, p.ld_partial},
+    GFB_TRY(make_out_map(&p.mo, Operand{partial, (int64_t)s.splits * s.rows_m(), p.ld_partial, p.ld_partial},
                          CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4));
   else if (p.tma_out)
     GFB_TRY(make_out_map(&p.mo, Operand{out, M, N, ld_out}, map_type<T>(), 2));
-  GFB_TRY((launch_gemm<gemm_kernel<EPI_STORE, T, 0, false>>(p, sms, st)));
+  GFB_TRY((launch_gemm<EPI_STORE, T, 0, false>(p, s, sms, st)));
   if (s.splits > 1) {
     join_kernel<T><<<grid_for(M * (p.ld_partial / 4), 256, sms), 256, 0, st>>>(p);
     GFB_CUDA(cudaGetLastError());
@@ -1239,12 +1318,12 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
 }
 
 template <typename T>
-gf_status gated(const GemmParams& p, int act, int sms, cudaStream_t st) {
+gf_status gated(const GemmParams& p, const Shape& s, int act, int sms, cudaStream_t st) {
   if (act == GF_ACT_GELU)
-    return p.drop.on ? launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_GELU, true>>(p, sms, st)
-                     : launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_GELU, false>>(p, sms, st);
-  return p.drop.on ? launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_SILU, true>>(p, sms, st)
-                   : launch_gemm<gemm_kernel<EPI_GATED, T, GF_ACT_SILU, false>>(p, sms, st);
+    return p.drop.on ? launch_gemm<EPI_GATED, T, GF_ACT_GELU, true>(p, s, sms, st)
+                     : launch_gemm<EPI_GATED, T, GF_ACT_GELU, false>(p, s, sms, st);
+  return p.drop.on ? launch_gemm<EPI_GATED, T, GF_ACT_SILU, true>(p, s, sms, st)
+                   : launch_gemm<EPI_GATED, T, GF_ACT_SILU, false>(p, s, sms, st);
 }
 
 template <typename T>
@@ -1264,7 +1343,7 @@ gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   p.drop = drop_args(f.dropout);
   GFB_TRY(make_out_map(&p.mo, Operand{f.h, pl.M, pl.Hp, pl.Hp}, map_type<T>(), 2));
   if (f.u) GFB_TRY(make_out_map(&p.mu, Operand{f.u, pl.M, 2 * pl.Hp, 2 * pl.Hp}, map_type<T>(), 2));
-  GFB_TRY(gated<T>(p, f.activation, sms, st));
+  GFB_TRY(gated<T>(p, pl.in, f.activation, sms, st));
   return product<T>(pl.out, Operand{f.h, pl.M, pl.Hp, pl.Hp}, false, o.w_out, false, pl.M, pl.O, pl.F, f.y, f.ld_y, f.b_out,
                     0, 0, pl.partial, sms, st);
 }
@@ -1298,7 +1377,7 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
     p.kb_total = (int)ceil_div(pl.O, 64);
     p.u = f.u;
     GFB_TRY(make_out_map(&p.mo, du, map_type<T>(), 2));
-    GFB_TRY((launch_gemm<gemm_kernel<EPI_GATED_BWD, T, 0, false>>(p, sms, st)));
+    GFB_TRY((launch_gemm<EPI_GATED_BWD, T, 0, false>(p, pl.dh, sms, st)));
   }
   if (f.dx)
     GFB_TRY(product<T>(pl.dx, du, false, o.w_in, true, pl.M, pl.D, 2 * pl.Hp, f.dx, pl.D, nullptr, 0, 0, pl.partial, sms, st));
@@ -1370,7 +1449,7 @@ Int8Plan plan_int8(const gf_int8_product& p, char* ws) {
   const int64_t ld = round_up<int64_t>(p.k, 16);
   if (pl.copy_a) pl.a = b.take(p.m * ld);
   if (pl.copy_b) pl.b = b.take(p.n * ld);
-  pl.shape = choose_shape(p.m, p.n, ceil_div(p.k, 128), false, false, sm_count());
+  pl.shape = choose_shape(p.m, p.n, ceil_div(p.k, 128), EPI_INT8, false, sm_count());
   pl.bytes = b.used > 256 ? b.used : 256;
   return pl;
 }
@@ -1525,9 +1604,9 @@ gf_status gf_int8_matmul(const gf_int8_product* d, void* workspace, size_t works
   p.bias = d->bias;
   p.a_scale = d->a_scale;
   p.b_scale = d->b_scale;
-  if (d->dtype == GF_F32) return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, float, 0, false>>(p, sms, st);
-  if (d->dtype == GF_BF16) return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, __nv_bfloat16, 0, false>>(p, sms, st);
-  return gfb::launch_gemm<gfb::gemm_kernel<gfb::EPI_INT8, __half, 0, false>>(p, sms, st);
+  if (d->dtype == GF_F32) return gfb::launch_gemm<gfb::EPI_INT8, float, 0, false>(p, pl.shape, sms, st);
+  if (d->dtype == GF_BF16) return gfb::launch_gemm<gfb::EPI_INT8, __nv_bfloat16, 0, false>(p, pl.shape, sms, st);
+  return gfb::launch_gemm<gfb::EPI_INT8, __half, 0, false>(p, pl.shape, sms, st);
 }
 
 gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out) {
