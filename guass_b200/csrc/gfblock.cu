@@ -179,7 +179,7 @@ __device__ __forceinline__ void activate(float g0, float g1, uint64_t& value, ui
 //  the others  epilogue of the other accumulator: warp w reads TMEM lanes
 //              32 * (w % 4) onwards, and the warps of a quarter take its
 //              32-column chunks in turn
-// Each CTA (or pair) walks over tiles and K ranges with a stride of the grid.
+// Each CTA (or pair) walks over a run of tiles and K ranges.
 //
 // Why pairs: a CTA's tile of 128 x 256 takes (128 + 256) * 128 bytes of
 // operands every 512 clocks of products, 96 bytes a clock, and the way from L2
@@ -190,28 +190,32 @@ constexpr int kTileM = 128;   // rows of a CTA
 constexpr int kMaxN = 256;
 constexpr int kABytes = kTileM * 128;
 constexpr int kRowsBytes = 32 * 64;     // staging block: 64 bytes of each of a warp's 32 rows
-constexpr int kWarpVectors = 2 * 32 * 4;  // two vectors of 32 floats (biases, scales)
+constexpr int kVectorBytes = 32 * 4;    // a warp's vector of 32 floats (bias, scale)
 constexpr uint32_t kTmemCols = 512;
 constexpr int kSmemLimit = 232448;
 
 enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
 
-// Warps and shared memory of a variant.  The gated epilogue does about 25
-// instructions for each element of h and hides their latencies behind 16
-// warps; the others do little, and keep 8 warps with room for more registers.
-// Staging blocks: two for results (one fills while the other is written out),
-// and two for the saved rows that the backward's epilogue turns.
-template <int EPI, bool PAIR>
+// Warps and shared memory of a variant.  A chunk's result leaves as one to
+// three staging blocks through TMA stores, which have the next chunk's
+// arithmetic to be read in; the backward's saved rows arrive in two more by
+// TMA loads a chunk ahead (with 227 KB of shared memory in use the L1 cache
+// has too few lines left for that many loads in flight).  What is left holds
+// operand stages.  Eight epilogue warps were as fast as 12 or 16 for the 16-bit
+// products, whose long tiles are bound by the memory they write; the integer
+// results take a conversion each and gain from 12 (16384 x 1280 x 10240: 160 us
+// against 171).
+template <int EPI>
 struct Config {
-  static constexpr int epi_warps = EPI == EPI_GATED ? 16 : 8;
+  static constexpr int epi_warps = EPI == EPI_INT8 ? 12 : 8;
   static constexpr int threads = 64 + 32 * epi_warps;
-  static constexpr int blocks = EPI == EPI_GATED_BWD ? 4 : 2;
-  static constexpr int warp_bytes = blocks * kRowsBytes + kWarpVectors;
-  static constexpr int stage_bytes = kABytes + (PAIR ? kMaxN / 2 : kMaxN) * 128;
-  static constexpr int stages = (kSmemLimit - 512 - epi_warps * warp_bytes) / stage_bytes;
-  static constexpr int smem_bytes = stages * stage_bytes + epi_warps * warp_bytes + 512;
-  static_assert(stages >= 3 && smem_bytes <= kSmemLimit, "shared memory of one SM");
+  static constexpr int out = EPI == EPI_GATED ? 3 : 2;
+  static constexpr int blocks = out + (EPI == EPI_GATED_BWD ? 2 : 0);
+  static constexpr int vectors = EPI == EPI_GATED_BWD ? 0 : EPI == EPI_STORE ? 1 : 2;
+  static constexpr int side_bytes = epi_warps * (blocks * kRowsBytes + vectors * kVectorBytes) + 512;
+  static constexpr int stage_room = (kSmemLimit - side_bytes) / 1024 * 1024;
 };
+constexpr int kMaxEpiWarps = 12;
 constexpr int kMaxStages = 8;
 
 struct alignas(64) GemmParams {
@@ -225,6 +229,7 @@ struct alignas(64) GemmParams {
   int32_t a_mn, b_mn;          // operand is M/N-contiguous
   int32_t gate_row;            // gated: row of B where the gate half starts
   uint32_t idesc, tx_bytes;
+  int32_t stages, stage_bytes;
   int32_t seg_pad, seg;        // result rows come in two runs of `seg` rows, the second starting at seg_pad (0: one run)
   int32_t tma_out;             // the result is written through mo (its rows are 16-byte aligned, in one run)
   int64_t ld_out;
@@ -232,7 +237,7 @@ struct alignas(64) GemmParams {
   float* partial;              // splits > 1: [splits][tiles_m * 128][ld_partial]
   int64_t ld_partial;
   const void* bias;            // [N] (gated: [2 N])
-  void* u;                     // GATED: written (through mu) when not null; GATED_BWD: read
+  void* u;                     // GATED: written through mu when not null
   int32_t hp;                  // gated: padded hidden size
   const float* a_scale;
   const float* b_scale;
@@ -240,25 +245,59 @@ struct alignas(64) GemmParams {
 };
 
 struct Pipe {  // barriers and the abort flag, in shared memory
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], spare, rows[kMaxEpiWarps];
   uint32_t tmem, abort;
 };
 static_assert(sizeof(Pipe) <= 512, "the room behind the staging blocks");
 
-struct Tile {  // m0: first row of this CTA
-  int m0, n0, split, kb0, kb1;
+// The tiles of one CTA or pair, columns first: with few column tiles a run of
+// consecutive ones, so that its rows of A come from memory once and from L2
+// after that; with many, every units-th, so that all units share the rows of
+// a few row tiles and neighbouring columns at a time.  Measured on the loads
+// alone: 10 column tiles (16384 x 320 x 1280 gated) 21 us in runs and 28
+// interleaved; the whole product with 40 (8 bits, 16384 x 1280 x 10240) 177 us
+// in runs and 162 interleaved.  Going on is an addition: a division would
+// stand in every role's way.
+constexpr int kRunColumns = 16;
+struct Tile {
+  int n, m, split;       // tile coordinates
+  int m0, n0, kb0, kb1;  // first row of this CTA, first column, range of k steps
+  int left;              // tiles still to do, this one included
+  int step_n, step_m;    // to the next one
 };
 template <bool PAIR>
-__device__ __forceinline__ Tile tile_of(const GemmParams& p, int64_t item, uint32_t rank) {
-  Tile t;
-  const int n = (int)(item % p.tiles_n);
-  const int64_t rest = item / p.tiles_n;
-  t.m0 = ((int)(rest % p.tiles_m) * (PAIR ? 2 : 1) + rank) * kTileM;
-  t.split = (int)(rest / p.tiles_m);
-  t.n0 = n * p.cols;
+__device__ __forceinline__ void place(const GemmParams& p, Tile& t, uint32_t rank) {
+  t.m0 = (t.m * (PAIR ? 2 : 1) + (int)rank) * kTileM;
+  t.n0 = t.n * p.cols;
   t.kb0 = t.split * p.kb_split;
   t.kb1 = min(t.kb0 + p.kb_split, p.kb_total);
+}
+template <bool PAIR>
+__device__ __forceinline__ Tile first_tile(const GemmParams& p, uint32_t rank) {
+  const uint32_t unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t each = items / units, more = items - each * units;  // the first `more` units take one more
+  const bool run = p.tiles_n <= kRunColumns;
+  const int64_t item = run ? unit * each + (unit < more ? unit : more) : unit;
+  const int64_t rest = item / p.tiles_n;
+  Tile t;
+  t.n = (int)(item - rest * p.tiles_n);
+  t.split = (int)(rest / p.tiles_m);
+  t.m = (int)(rest - (int64_t)t.split * p.tiles_m);
+  t.left = (int)(each + (unit < more));
+  t.step_m = run ? 0 : (int)(units / p.tiles_n);
+  t.step_n = run ? 1 : (int)(units % p.tiles_n);
+  place<PAIR>(p, t, rank);
   return t;
+}
+template <bool PAIR>
+__device__ __forceinline__ void next_tile(const GemmParams& p, Tile& t, uint32_t rank) {
+  --t.left;
+  t.n += t.step_n;
+  t.m += t.step_m;
+  if (t.n >= p.tiles_n) t.n -= p.tiles_n, ++t.m;
+  while (t.m >= p.tiles_m) t.m -= p.tiles_m, ++t.split;
+  place<PAIR>(p, t, rank);
 }
 
 template <int EPI, typename T, int ACT, bool DROP>
@@ -269,107 +308,142 @@ struct EpilogueWarp {
   float* vec1;
   const int lane;
   Philox rng;
-  uint32_t out = 0;  // blocks of rows written
+  float row_scale = 0.0f;
+  const uint32_t rows_bar;      // GATED_BWD: this warp's barrier of the saved rows
+  volatile uint32_t* abort;
+  uint32_t phase = 0;
+  bool rows_due = false;        // they are on their way
 
-  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors)
+  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors, uint32_t bar,
+                                          volatile uint32_t* abort_)
       : p(p_), stage(stage_), vec0(reinterpret_cast<float*>(vectors)), vec1(vec0 + 32), lane(threadIdx.x & 31),
-        rng(p_.drop) {}
+        rng(p_.drop), rows_bar(bar), abort(abort_) {}
 
   // Bias and scale of this lane's column of a chunk, fetched ahead.
   struct Ahead {
     float a, b;
-    uint4 u[2][4];  // GATED_BWD: the chunk's saved rows, four lanes to a row
   };
-  __device__ __forceinline__ void fetch(Ahead& x, int m, int n) const {
-    const int left = p.N - n;
-    x.a = x.b = 0.0f;
+  __device__ __forceinline__ void fetch(Ahead& x, int m, int n) {
     if constexpr (EPI == EPI_GATED_BWD) {
-      const char* u = static_cast<const char*>(p.u) + 2 * ((int64_t)m * 2 * p.hp + n);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + (lane >> 2);
-        const char* at = u + r * 4 * (int64_t)p.hp + (lane & 3) * 16;
-        const bool in = m + r < p.M;
-        x.u[0][i] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
-        x.u[1][i] = in ? *reinterpret_cast<const uint4*>(at + 2 * (int64_t)p.hp) : make_uint4(0, 0, 0, 0);
+      __syncwarp();  // every lane has read the rows before
+      if (lane == 0) {
+        tc::mbar_expect_tx(rows_bar, 2 * kRowsBytes);
+        tc::tma_load(block(C::out), &p.mu, rows_bar, n, m);
+        tc::tma_load(block(C::out + 1), &p.mu, rows_bar, p.hp + n, m);
       }
-    } else if (lane < left) {
-      const T* bias = static_cast<const T*>(p.bias);
-      if (bias) x.a = to_float(bias[n + lane]);
-      if (EPI == EPI_GATED && bias) x.b = to_float(bias[p.N + n + lane]);
-      if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
+      rows_due = true;
+    } else {
+      x.a = x.b = 0.0f;
+      if (lane < p.N - n) {
+        const T* bias = static_cast<const T*>(p.bias);
+        if (bias) x.a = to_float(bias[n + lane]);
+        if (EPI == EPI_GATED && bias) x.b = to_float(bias[p.N + n + lane]);
+        if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
+      }
     }
   }
 
   // One 32-column chunk at result column n of rows m .. m + 31, from the
-  // accumulator columns at `acc`.  `release` runs once they are read.
-  template <typename Release>
-  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int n, const Ahead& ahead, Release release) {
+  // accumulator columns at `acc`.  `release` runs once they are read, and
+  // `fetch_next` once `ahead` is.
+  template <typename Release, typename Next>
+  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int n, const Ahead& ahead, Release release,
+                                        Next fetch_next) {
     uint32_t d[32];
-    if constexpr (EPI != EPI_GATED) tc::tmem_load32(d, acc);
+    if constexpr (EPI == EPI_STORE || EPI == EPI_INT8) tc::tmem_load32(d, acc);
     if constexpr (EPI == EPI_STORE) {
       tc::tmem_wait();
       release();
       if (p.splits > 1) {
         const int row = t.split * p.rows_m + m;
+        fetch_next();
+        begin();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = d[16 * h + i];
-          write(v, &p.mo, n + 16 * h, row);
+          put(h, v);
         }
+        send([&] {
+          tc::tma_store(&p.mo, block(0), n, row);
+          tc::tma_store(&p.mo, block(1), n + 16, row);
+        });
         return;
       }
       vectors(ahead);
+      fetch_next();
       uint32_t v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f(d[2 * i]) + vec0[2 * i], f(d[2 * i + 1]) + vec0[2 * i + 1]);
-      result<2>(v, m, n);
+      begin();
+      put(0, v);
+      result<2>(1, m, n);
     } else if constexpr (EPI == EPI_INT8) {
-      const float s = m + lane < p.M ? p.a_scale[m + lane] : 0.0f;
+      const float s = row_scale;
       vectors(ahead);
+      fetch_next();
       tc::tmem_wait();
       release();
       // |sum| < 2^31: one rounding to fp32, then the two scales and the bias
 #pragma unroll
       for (int i = 0; i < 32; ++i) d[i] = __float_as_uint((float)(int)d[i] * s * vec1[i] + vec0[i]);
       uint32_t v[16];
+      begin();
       if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = d[16 * h + i];
-          result<4>(v, m, n + 16 * h);
+          put(h, v);
         }
+        result<4>(2, m, n);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = pack2<T>(f(d[2 * i]), f(d[2 * i + 1]));
-        result<2>(v, m, n);
+        put(0, v);
+        result<2>(1, m, n);
       }
     } else if constexpr (EPI == EPI_GATED) {
       vectors(ahead);
+      fetch_next();
       if (p.u) gated<true>(acc, m, n, release);
       else gated<false>(acc, m, n, release);
     } else {
       uint32_t v[16], w[16];
-      turn(w, v, ahead.u);
-      tc::tmem_wait();
-      release();
+      read_rows(v, w);
+      fetch_next();
       // du_value = dh * u_value, du_gate = dh * u_gate (see gated)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 a = unpack2<T>(w[i]), g = unpack2<T>(v[i]);
-        w[i] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
-        v[i] = pack2<T>(f(d[2 * i]) * g.x, f(d[2 * i + 1]) * g.y);
+      for (int half = 0; half < 2; ++half) {
+        tc::tmem_load16(d, acc + 16 * half);
+        tc::tmem_wait();
+        if (half == 1) release();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int o = 8 * half + i;
+          const float2 a = unpack2<T>(v[o]), g = unpack2<T>(w[o]);
+          v[o] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
+          w[o] = pack2<T>(f(d[2 * i]) * g.x, f(d[2 * i + 1]) * g.y);
+        }
       }
-      write(w, &p.mo, n, m);
-      write(v, &p.mo, p.hp + n, m);
+      begin();
+      put(0, v);
+      put(1, w);
+      send([&] {
+        tc::tma_store(&p.mo, block(0), n, m);
+        tc::tma_store(&p.mo, block(1), p.hp + n, m);
+      });
     }
   }
 
-  // Every block must be out of shared memory before the CTA ends.
+  // Every block must be out of shared memory, and no copy on its way into it,
+  // before the CTA ends.
   __device__ __forceinline__ void finish() {
+    if (rows_due) {  // after a wait that gave up only
+      volatile uint32_t ignore = 0;
+      tc::mbar_wait(rows_bar, phase, &ignore);
+    }
     if (lane == 0) tc::tma_store_drain();
     __syncwarp();
   }
@@ -380,7 +454,7 @@ struct EpilogueWarp {
   __device__ __forceinline__ void vectors(const Ahead& x) {
     __syncwarp();
     vec0[lane] = x.a;
-    vec1[lane] = x.b;
+    if constexpr (C::vectors == 2) vec1[lane] = x.b;
     __syncwarp();
   }
 
@@ -391,11 +465,10 @@ struct EpilogueWarp {
   // themselves would take.
   template <bool SAVE, typename Release>
   __device__ __forceinline__ void gated(uint32_t acc, int m, int n, Release release) {
-    uint32_t h[16], sv[16], sg[16];
-    const int left = p.N - n;  // the padding columns of h and u are zeros
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t a[16], g[16];
+      uint32_t a[16], g[16], h[8], sv[8], sg[8];
+      const int left = p.N - n - 16 * half;  // the padding columns of h and u are zeros
       tc::tmem_load16(a, acc + 16 * half);
       tc::tmem_load16(g, acc + p.cols + 16 * half);
       tc::tmem_wait();
@@ -414,7 +487,7 @@ struct EpilogueWarp {
         const float4 b1 = *reinterpret_cast<const float4*>(vec1 + 16 * half + 4 * q);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int c = 4 * q + 2 * i, o = 8 * half + 2 * q + i;
+          const int c = 4 * q + 2 * i, o = 2 * q + i;
           uint64_t x = tc::add_f2(tc::pack_f2(f(a[c]), f(a[c + 1])), i ? tc::pack_f2(b0.z, b0.w) : tc::pack_f2(b0.x, b0.y));
           float2 y = tc::unpack_f2(
               tc::add_f2(tc::pack_f2(f(g[c]), f(g[c + 1])), i ? tc::pack_f2(b1.z, b1.w) : tc::pack_f2(b1.x, b1.y)));
@@ -433,68 +506,86 @@ struct EpilogueWarp {
           }
         }
       }
-    }
-    if (left < 32) {
+      if (left < 16) {
 #pragma unroll
-      for (int o = 0; o < 16; ++o) {
-        const uint32_t mask = 2 * o + 1 < left ? 0xFFFFFFFFu : 2 * o < left ? 0xFFFFu : 0u;
-        h[o] &= mask;
-        if constexpr (SAVE) sv[o] &= mask, sg[o] &= mask;
+        for (int o = 0; o < 8; ++o) {
+          const uint32_t mask = 2 * o + 1 < left ? 0xFFFFFFFFu : 2 * o < left ? 0xFFFFu : 0u;
+          h[o] &= mask;
+          if constexpr (SAVE) sv[o] &= mask, sg[o] &= mask;
+        }
+      }
+      if (half == 0) begin();
+      put_half(0, half, h);
+      if constexpr (SAVE) {
+        put_half(1, half, sv);
+        put_half(2, half, sg);
       }
     }
-    write(h, &p.mo, n, m);
-    if constexpr (SAVE) {
-      write(sv, &p.mu, n, m);
-      write(sg, &p.mu, p.hp + n, m);
-    }
+    send([&] {
+      tc::tma_store(&p.mo, block(0), n, m);
+      if constexpr (SAVE) {
+        tc::tma_store(&p.mu, block(1), n, m);
+        tc::tma_store(&p.mu, block(2), p.hp + n, m);
+      }
+    });
   }
 
-  // Writes 64 bytes of each of the 32 rows, lane = row in `v`, through a
-  // staging block whose 16-byte pieces are swizzled as the tensor map says
-  // (piece ^ (row / 2 % 4): eight lanes then cover all banks).
-  __device__ __forceinline__ void write(const uint32_t (&v)[16], const CUtensorMap* map, int x, int y) {
-    char* s = stage + (out & 1) * kRowsBytes;
-    ++out;
-    if (lane == 0) tc::tma_store_wait<1>();
+  // Results leave as blocks of 64 bytes of the 32 rows: begin() waits until
+  // the last chunk's blocks are read, put() writes lane's row with its 16-byte
+  // pieces swizzled as the tensor maps say (piece ^ (row / 2 % 4): eight lanes
+  // then cover all banks), send() stores them.
+  using C = Config<EPI>;
+  __device__ __forceinline__ void begin() {
+    if (lane == 0) tc::tma_store_wait<0>();
     __syncwarp();
+  }
+  __device__ __forceinline__ uint32_t block(int i) const { return tc::smem_addr(stage) + i * kRowsBytes; }
+  __device__ __forceinline__ void put_piece(int b, int i, const uint32_t* v) {
+    *reinterpret_cast<uint4*>(stage + b * kRowsBytes + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  __device__ __forceinline__ void put(int b, const uint32_t (&v)[16]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(s + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    for (int i = 0; i < 4; ++i) put_piece(b, i, v + 4 * i);
+  }
+  __device__ __forceinline__ void put_half(int b, int half, const uint32_t (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) put_piece(b, 2 * half + i, v + 4 * i);
+  }
+  template <typename Stores>
+  __device__ __forceinline__ void send(Stores stores) {
     tc::fence_proxy_async();
     __syncwarp();
     if (lane == 0) {
-      tc::tma_store(map, tc::smem_addr(s), x, y);
+      stores();
       tc::tma_store_commit();
     }
   }
 
-  // The reverse turn of the two blocks of rows that four lanes each fetched
-  // (GATED_BWD), through staging blocks of their own.
-  __device__ __forceinline__ void turn(uint32_t (&v)[16], uint32_t (&w)[16], const uint4 (&u)[2][4]) {
-    char* s = stage + 2 * kRowsBytes;
+  // This lane's row of the two blocks of saved rows (GATED_BWD).
+  __device__ __forceinline__ void read_rows(uint32_t (&v)[16], uint32_t (&w)[16]) {
+    tc::mbar_wait(rows_bar, phase, abort);
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 8 * (i & 3) + (lane >> 2), c = lane & 3;
-      *reinterpret_cast<uint4*>(s + (i >> 2) * kRowsBytes + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = u[i >> 2][i & 3];
-    }
-    __syncwarp();
+    phase ^= 1;
+    rows_due = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const char* at = s + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
+      const char* at = stage + C::out * kRowsBytes + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
       const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + kRowsBytes);
       v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
       w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
     }
   }
 
-  // A piece of the result: 64 bytes of rows m .. m + 31 from column n.
+  // `blocks` blocks of the result, rows m .. m + 31 from column n.
   template <int ES>
-  __device__ __forceinline__ void result(const uint32_t (&v)[16], int m, int n) {
-    if (n >= p.N) return;
+  __device__ __forceinline__ void result(int blocks, int m, int n) {
+    constexpr int per_row = 64 / ES;
     if (p.tma_out) {
-      write(v, &p.mo, n, m);
+      send([&] {
+        tc::tma_store(&p.mo, block(0), n, m);
+        if (blocks > 1 && n + per_row < p.N) tc::tma_store(&p.mo, block(1), n + per_row, m);
+      });
       return;
     }
     // rows off the 16-byte grid, or in two runs (seg_pad is a multiple of 64:
@@ -506,36 +597,31 @@ struct EpilogueWarp {
       rows = min(rows, p.seg - in);
       row = m >= p.seg_pad ? (int64_t)p.seg + in : in;
     }
-    constexpr int per_row = 64 / ES;
-    const int cols = min(per_row, p.N - n);
-    char* dst = static_cast<char*>(p.out) + ES * (row * p.ld_out + n);
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    __syncwarp();
-    for (int i = lane; i < 32 * per_row; i += 32) {
-      const int r = i / per_row, c = i % per_row, b = c * ES;
-      if (r < rows && c < cols) {
-        const char* src = stage + r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
-        if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint16_t*>(src);
-        else *reinterpret_cast<uint32_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint32_t*>(src);
+    for (int k = 0; k < blocks; ++k) {
+      const int at = n + k * per_row, cols = min(per_row, p.N - at);
+      char* dst = static_cast<char*>(p.out) + ES * (row * p.ld_out + at);
+      for (int i = lane; i < 32 * per_row; i += 32) {
+        const int r = i / per_row, c = i % per_row, b = c * ES;
+        if (r < rows && c < cols) {
+          const char* src = stage + k * kRowsBytes + r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
+          if constexpr (ES == 2)
+            *reinterpret_cast<uint16_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint16_t*>(src);
+          else
+            *reinterpret_cast<uint32_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint32_t*>(src);
+        }
       }
     }
-    __syncwarp();
   }
 };
 
 template <int EPI, typename T, int ACT, bool DROP, bool PAIR>
-__global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  using C = Config<EPI, PAIR>;
-  constexpr int kStages = C::stages;
-  static_assert(kStages <= kMaxStages, "barriers");
+__global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  using C = Config<EPI>;
   extern __shared__ __align__(1024) char smem[];
-  char* staging = smem + kStages * C::stage_bytes;
+  char* staging = smem + C::stage_room;
   char* vectors = staging + C::epi_warps * C::blocks * kRowsBytes;
-  Pipe* pipe = reinterpret_cast<Pipe*>(vectors + C::epi_warps * kWarpVectors);
+  Pipe* pipe = reinterpret_cast<Pipe*>(vectors + C::epi_warps * C::vectors * kVectorBytes);
   const uint32_t base = tc::smem_addr(smem);
   if (base & 1023u) {  // the operand tiles' swizzle needs it; the kernel has no other shared memory
     if (threadIdx.x == 0) atomicOr(&g_status, GF_FLAG_TIMEOUT);
@@ -546,13 +632,11 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
   volatile uint32_t* abort = &pipe->abort;
   const int warp = threadIdx.x >> 5;
   const uint32_t rank = PAIR ? tc::cluster_rank() : 0;
-  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  const int64_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     tc::tma_prefetch(&p.ma);
     tc::tma_prefetch(&p.mb);
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(full + 8 * i, 1);
       tc::mbar_init(empty + 8 * i, 1);
     }
@@ -560,6 +644,7 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
       tc::mbar_init(acc_full + 8 * i, 1);
       tc::mbar_init(acc_empty + 8 * i, C::epi_warps * (PAIR ? 2 : 1));
     }
+    for (int i = 0; i < C::epi_warps; ++i) tc::mbar_init(tc::smem_addr(&pipe->rows[i]), 1);
     pipe->abort = 0;
     tc::fence_barrier_init();
     tc::fence_proxy_async();
@@ -575,7 +660,7 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
   if (warp == 0) {
     // Both CTAs of a pair load; the copies of both count on the first one's barrier.
     if (tc::elect_one()) {
-      uint32_t n = 0;  // stages filled
+      uint32_t s = 0, phase = 0, n = 0;  // stage, its phase, stages filled
       bool ok = true;
       const uint32_t full0 = PAIR ? tc::peer_addr(full, 0) : full;
       const int b_cols = PAIR ? p.bn / 2 : p.bn;
@@ -583,14 +668,12 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
         if constexpr (PAIR) tc::tma_load_pair(dst, map, bar, x, y);
         else tc::tma_load(dst, map, bar, x, y);
       };
-      for (int64_t item = first; ok && item < items; item += stride) {
-        const Tile t = tile_of<PAIR>(p, item, rank);
+      for (Tile t = first_tile<PAIR>(p, rank); ok && t.left > 0; next_tile<PAIR>(p, t, rank)) {
         const int n0 = t.n0 + (PAIR ? (int)rank * b_cols : 0);
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-          const int s = n % kStages;
-          ok = tc::mbar_wait(empty + 8 * s, ((n / kStages) & 1) ^ 1, abort);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          ok = tc::mbar_wait(empty + 8 * s, phase ^ 1, abort);
           if (!ok) break;
-          const uint32_t bar = full0 + 8 * s, a = base + s * C::stage_bytes, b = a + kABytes;
+          const uint32_t bar = full0 + 8 * s, a = base + s * p.stage_bytes, b = a + kABytes;
           if (rank == 0) tc::mbar_expect_tx(full + 8 * s, p.tx_bytes);
           const int k0 = kb * (EPI == EPI_INT8 ? 128 : 64);
           if (p.a_mn) {
@@ -607,39 +690,40 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
           } else {
             load(b, &p.mb, bar, k0, n0);
           }
+          ++n;
+          if (++s == p.stages) s = 0, phase ^= 1;
         }
       }
       // The copies in flight must land before the CTA ends.  Every product
       // waits for its copies, so this matters after a wait that gave up only.
       if (!ok && rank == 0) {
         volatile uint32_t ignore = 0;
-        const uint32_t from = n > kStages ? n - kStages : 0;
-        for (uint32_t i = from; i < n; ++i) tc::mbar_wait(full + 8 * (i % kStages), (i / kStages) & 1, &ignore);
+        const uint32_t from = n > (uint32_t)p.stages ? n - p.stages : 0;
+        for (uint32_t i = from; i < n; ++i) tc::mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1, &ignore);
       }
     }
   } else if (warp == 1) {
     if (rank == 0 && tc::elect_one()) {
-      uint32_t n = 0, it = 0;
+      uint32_t s = 0, phase = 0, it = 0;
       bool ok = true;
       const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      for (int64_t item = first; ok && item < items; item += stride, ++it) {
-        const Tile t = tile_of<PAIR>(p, item, rank);
+      for (Tile t = first_tile<PAIR>(p, rank); ok && t.left > 0; next_tile<PAIR>(p, t, rank), ++it) {
         const uint32_t buf = it & 1;
         ok = tc::mbar_wait(acc_empty + 8 * buf, ((it >> 1) & 1) ^ 1, abort);
         if (!ok) break;
         tc::fence_after();
         const uint32_t d = tmem + buf * kMaxN;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-          const int s = n % kStages;
-          ok = tc::mbar_wait(full + 8 * s, (n / kStages) & 1, abort);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          ok = tc::mbar_wait(full + 8 * s, phase, abort);
           if (!ok) break;
           tc::fence_after();
-          const uint32_t a = base + s * C::stage_bytes;
+          const uint32_t a = base + s * p.stage_bytes;
           const uint64_t da = tc::operand_desc(a, p.a_mn), db = tc::operand_desc(a + kABytes, p.b_mn);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             tc::mma<PAIR, EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, p.idesc, kb > t.kb0 || i > 0);
           tc::mma_commit<PAIR>(empty + 8 * s);
+          if (++s == p.stages) s = 0, phase ^= 1;
         }
         if (!ok) break;
         tc::mma_commit<PAIR>(acc_full + 8 * buf);
@@ -649,18 +733,19 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
     constexpr int kSets = C::epi_warps / 4;  // warps of a quarter
     const int quarter = warp & 3, set = (warp - 2) >> 2;
     EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * C::blocks * kRowsBytes,
-                                        vectors + (warp - 2) * kWarpVectors);
+                                        vectors + (warp - 2) * C::vectors * kVectorBytes,
+                                        tc::smem_addr(&pipe->rows[warp - 2]), abort);
     const uint32_t empty0 = PAIR ? tc::peer_addr(acc_empty, 0) : acc_empty;
     // gated: the padding columns of h, u and du are written too (zeros)
     const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
     uint32_t it = 0;
-    for (int64_t item = first; item < items; item += stride, ++it) {
-      const Tile t = tile_of<PAIR>(p, item, rank);
+    for (Tile t = first_tile<PAIR>(p, rank); t.left > 0; next_tile<PAIR>(p, t, rank), ++it) {
       const uint32_t buf = it & 1;
       const int m = t.m0 + 32 * quarter;
       const int c_end = m < p.M ? min(p.cols, n_end - t.n0) : 0;
       const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + buf * kMaxN;
       int c = 32 * set;
+      if (EPI == EPI_INT8) epi.row_scale = m + (int)(threadIdx.x & 31) < p.M ? p.a_scale[m + (threadIdx.x & 31)] : 0.0f;
       typename decltype(epi)::Ahead ahead;
       if (c < c_end) epi.fetch(ahead, m, t.n0 + c);
       if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
@@ -676,10 +761,9 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
       };
       if (c >= c_end) release(true);  // no chunk of this tile is this warp's
       for (; c < c_end; c += 32 * kSets) {
-        const bool last = c + 32 * kSets >= c_end;
-        const auto now = ahead;
-        if (!last) epi.fetch(ahead, m, t.n0 + c + 32 * kSets);
-        epi.chunk(acc + c, t, m, t.n0 + c, now, [&] { release(last); });
+        const int next = c + 32 * kSets;
+        epi.chunk(acc + c, t, m, t.n0 + c, ahead, [&] { release(next >= c_end); },
+                  [&] { if (next < c_end) epi.fetch(ahead, m, t.n0 + next); });
       }
     }
     epi.finish();
@@ -693,8 +777,7 @@ __global__ void __launch_bounds__(Config<EPI, PAIR>::threads, 1) gemm_kernel(con
     if (*abort && rank == 0) {  // products may still be running: their end is a commit away
       if (tc::elect_one()) {
         volatile uint32_t ignore = 0;
-        const uint32_t spare = tc::smem_addr(&pipe->empty[kMaxStages - 1]);  // no variant has that many stages
-        static_assert(kStages < kMaxStages, "a spare barrier");
+        const uint32_t spare = tc::smem_addr(&pipe->spare);
         tc::mbar_init(spare, 1);
         tc::mma_commit<false>(spare);
         tc::mbar_wait(spare, 0, &ignore);
@@ -1013,9 +1096,9 @@ int sm_count() {
 // Pairs or single CTAs, tile width, K ranges: whichever gives the least
 // estimated time.  A tile takes the longest of its products (2 clocks a
 // column and 64 k), its operands' way into the SM (70 bytes a clock) and its
-// epilogue; the grid's time is that of the CTA with most tiles, the fill of
-// its pipeline and one epilogue; K ranges add the partial products' way to
-// memory and back.
+// result's way to memory (about 11 bytes a clock for each SM when all write);
+// the grid's time is that of the CTA with most tiles, the fill of its pipeline
+// and one epilogue; K ranges add the partial products' way to memory and back.
 struct Shape {
   bool pair;
   int bn, splits, kb_split, tiles_m, tiles_n;
@@ -1026,10 +1109,12 @@ Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, in
   double best_cost = 0;
   const bool gated = epi == EPI_GATED;
   const int step = gated ? 64 : 32;
-  const double per_col = epi == EPI_GATED ? 34.0 : epi == EPI_GATED_BWD ? 20.0 : epi == EPI_INT8 ? 12.0 : 8.0;
+  const double per_col = epi == EPI_GATED ? 72.0 : epi == EPI_GATED_BWD ? 80.0 : 24.0;
   for (int pair = 0; pair < 2; ++pair) {
     const int64_t tm = ceil_div(M, pair ? 2 * kTileM : kTileM), units = pair ? sms / 2 : sms;
-    for (int bn = step; bn <= kMaxN; bn += step) {
+    // a single CTA's gated variants have room for enough stages of at most 128 columns
+    const bool narrow = !pair && (gated || epi == EPI_GATED_BWD);
+    for (int bn = step; bn <= (narrow ? kMaxN / 2 : kMaxN); bn += step) {
       const int cols = gated ? bn / 2 : bn;
       if (cols > 32 && cols - 32 >= N) break;  // wider than the result
       const int64_t tn = ceil_div(N, cols);
@@ -1039,7 +1124,7 @@ Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, in
         const int64_t per = ceil_div(kb, s);
         if (ceil_div(kb, per) != s) continue;
         const double waves = (double)ceil_div(tm * tn * s, units), epilogue = per_col * cols, main = per * step_cost;
-        double cost = waves * ((main > epilogue ? main : epilogue) + 100.0) + 1500.0 + epilogue;
+        double cost = waves * ((main > epilogue ? main : epilogue) + 600.0) + 1500.0 + epilogue;
         if (s > 1) cost += 4000.0 + (double)(s + 1) * M * N * 4 / 3000.0;
         if (best.bn == 0 || cost < best_cost) {
           best_cost = cost;
@@ -1056,21 +1141,25 @@ inline size_t partial_bytes(const Shape& s, int64_t N) {
 }
 
 template <int EPI, typename T, int ACT, bool DROP, bool PAIR>
-gf_status launch_gemm(const GemmParams& p, int sms, cudaStream_t st) {
-  using C = Config<EPI, PAIR>;
+gf_status launch_gemm(GemmParams p, int sms, cudaStream_t st) {
+  using C = Config<EPI>;
+  constexpr int smem_bytes = C::stage_room + C::side_bytes;
+  static_assert(smem_bytes <= kSmemLimit && C::stage_room >= 3 * 32768, "shared memory of one SM");
   const auto kernel = gemm_kernel<EPI, T, ACT, DROP, PAIR>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
   int dev = 0;
   GFB_CUDA(cudaGetDevice(&dev));
   if (dev > 63 || !(ready.load() >> dev & 1)) {
-    GFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem_bytes));
+    GFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes));
     if (dev <= 63) ready.fetch_or(uint64_t(1) << dev);
   }
+  p.stage_bytes = kABytes + 128 * round_up(PAIR ? p.bn / 2 : p.bn, 64);
+  p.stages = C::stage_room / p.stage_bytes < kMaxStages ? C::stage_room / p.stage_bytes : kMaxStages;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits, units = PAIR ? sms / 2 : sms;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(items < units ? items : units) * (PAIR ? 2 : 1));
   cfg.blockDim = dim3(C::threads);
-  cfg.dynamicSmemBytes = C::smem_bytes;
+  cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   if (PAIR) {
@@ -1375,8 +1464,8 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
     p.N = (int)pl.F;
     p.hp = (int)pl.Hp;
     p.kb_total = (int)ceil_div(pl.O, 64);
-    p.u = f.u;
     GFB_TRY(make_out_map(&p.mo, du, map_type<T>(), 2));
+    GFB_TRY(make_out_map(&p.mu, Operand{f.u, pl.M, 2 * pl.Hp, 2 * pl.Hp}, map_type<T>(), 2));
     GFB_TRY((launch_gemm<EPI_GATED_BWD, T, 0, false>(p, pl.dh, sms, st)));
   }
   if (f.dx)
