@@ -15,7 +15,8 @@ DTYPES = {torch.float32: _lib.GF_F32, torch.bfloat16: _lib.GF_BF16, torch.float1
 
 # Every symbol include/gfblock.h declares.
 EXPORTED = ("gf_gated_ff_workspace_bytes", "gf_gated_ff_forward", "gf_gated_ff_backward", "gf_dropout",
-            "gf_quantize_rows", "gf_int8_product_workspace_bytes", "gf_int8_matmul", "gf_block_status")
+            "gf_quantize_rows", "gf_int8_product_workspace_bytes", "gf_int8_matmul",
+            "gf_int8_linear_workspace_bytes", "gf_int8_linear", "gf_block_status")
 
 
 class GfDropoutRule(ctypes.Structure):
@@ -95,6 +96,10 @@ def lib() -> ctypes.CDLL:
     L.gf_int8_product_workspace_bytes.restype = size
     L.gf_int8_matmul.argtypes = [prod, ptr, size, ptr]
     L.gf_int8_matmul.restype = ctypes.c_int
+    L.gf_int8_linear_workspace_bytes.argtypes = [prod]
+    L.gf_int8_linear_workspace_bytes.restype = size
+    L.gf_int8_linear.argtypes = [prod, ptr, i64, i32, ptr, size, ptr]
+    L.gf_int8_linear.restype = ctypes.c_int
     L.gf_block_status.argtypes = [ptr, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
     L.gf_block_status.restype = ctypes.c_int
     _ready = L
@@ -128,16 +133,24 @@ def check_tensor(name: str, t, dtypes, device=None) -> None:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
 
 
-def on_device(t: torch.Tensor):
-    """Context that makes the tensor's device current."""
-    return torch.cuda.device(t.device)
+def call(device, fn, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``device`` with that
+    device current.  (The raw calls behind torch.cuda.current_stream and
+    torch.cuda.device: those objects cost more than a small launch.)"""
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
     """``t`` as [rows, cols] with unit column stride and rows that do not
     overlap: a view where its strides allow one, else a copy."""
-    v = t.reshape(-1, cols)
-    if cols > 1 and v.stride(1) != 1 or v.shape[0] > 1 and v.stride(0) < cols:
+    v = t if t.dim() == 2 else t.reshape(-1, cols)
+    row, col = v.stride()
+    if cols > 1 and col != 1 or v.shape[0] > 1 and row < cols:
         v = v.contiguous()
     return v
 
@@ -147,16 +160,15 @@ def ld(v: torch.Tensor) -> int:
     return v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
 
-def fill_rule(rule: GfDropoutRule, p: float, seed, site: int, device) -> None:
+def make_rule(p: float, seed, site: int, device) -> GfDropoutRule:
     """``seed``: an int, or a one-element int64 CUDA tensor that the kernel reads."""
-    p = float(p)
-    require(0.0 <= p < 1.0, f"dropout probability must be in [0, 1), got {p}")
-    site = int(site)
-    require(0 <= site < 1 << 32, f"site must be in [0, 2**32), got {site}")
-    rule.p, rule.site = p, site
+    p, site = float(p), int(site)
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"dropout probability must be in [0, 1), got {p}")
+    if not 0 <= site < 1 << 32:
+        raise ValueError(f"site must be in [0, 2**32), got {site}")
     if isinstance(seed, torch.Tensor):
         check_tensor("seed", seed, (torch.int64,), device)
         require(seed.numel() == 1, f"a seed tensor has one element, got {tuple(seed.shape)}")
-        rule.seed_ptr = seed.data_ptr()
-    else:
-        rule.seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+        return GfDropoutRule(p, 0, seed.data_ptr(), site, 0)
+    return GfDropoutRule(p, int(seed) & 0xFFFFFFFFFFFFFFFF, None, site, 0)

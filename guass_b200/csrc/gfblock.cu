@@ -1104,7 +1104,7 @@ struct Shape {
   int bn, splits, kb_split, tiles_m, tiles_n;
   int rows_m() const { return tiles_m * kTileM * (pair ? 2 : 1); }
 };
-Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
+Shape search_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
   Shape best{};
   double best_cost = 0;
   const bool gated = epi == EPI_GATED;
@@ -1134,6 +1134,22 @@ Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, in
     }
   }
   return best;
+}
+
+// The search takes some microseconds: a thread remembers the last shapes it asked for.
+Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
+  struct Entry {
+    int64_t M, N, kb;
+    int epi, may_split, sms;
+    Shape shape;
+  };
+  thread_local Entry seen[64];  // zero: no size is
+  const uint64_t hash = (uint64_t)M * 0x9E3779B97F4A7C15u ^ (uint64_t)N * 0xC2B2AE3D27D4EB4Fu ^ (uint64_t)kb * 0x165667B19E3779F9u ^
+                        (uint64_t)(4 * epi + may_split) * 0xD6E8FEB86659FD93u;
+  Entry& e = seen[hash >> 58];
+  if (e.M != M || e.N != N || e.kb != kb || e.epi != epi || e.may_split != may_split || e.sms != sms)
+    e = Entry{M, N, kb, epi, may_split, sms, search_shape(M, N, kb, epi, may_split, sms)};
+  return e.shape;
 }
 
 inline size_t partial_bytes(const Shape& s, int64_t N) {
@@ -1518,21 +1534,20 @@ struct Int8Plan {
   void *a, *b;
   size_t bytes;
 };
-gf_status check_int8(const gf_int8_product* p) {
-  const char* who = "gf_int8_matmul";
+gf_status check_int8(const char* who, const gf_int8_product* p, bool quantised) {
   if (!p) return fail(GF_ERR_INVALID_ARG, "%s: the description must be non-null", who);
   if (p->m < 0 || p->n <= 0 || p->k <= 0) return fail(GF_ERR_INVALID_ARG, "%s: sizes must be positive (m may be 0)", who);
   if (p->m > kMaxDim || p->n > kMaxDim) return fail(GF_ERR_UNSUPPORTED, "%s: a size is above 2^31 - 512", who);
   if (p->k > 131071) return fail(GF_ERR_UNSUPPORTED, "%s: k must be at most 131071 (the sums are 32-bit integers)", who);
   if (!known_dtype(p->dtype)) return fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_F32, GF_BF16 or GF_F16", who);
   if (p->reserved != 0) return fail(GF_ERR_INVALID_ARG, "%s: reserved fields must be 0", who);
-  if (p->ld_a < p->k || p->ld_b < p->k || p->ld_out < p->n)
+  if ((quantised && p->ld_a < p->k) || p->ld_b < p->k || p->ld_out < p->n)
     return fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
   return GF_OK;
 }
-Int8Plan plan_int8(const gf_int8_product& p, char* ws) {
+Int8Plan plan_int8(const gf_int8_product& p, char* ws, size_t used) {
   Int8Plan pl{};
-  Bump b{ws};
+  Bump b{ws, used};
   pl.copy_a = !aligned_rows(p.a, p.m, p.ld_a, 1);
   pl.copy_b = !aligned_rows(p.b, p.n, p.ld_b, 1);
   const int64_t ld = round_up<int64_t>(p.k, 16);
@@ -1541,6 +1556,67 @@ Int8Plan plan_int8(const gf_int8_product& p, char* ws) {
   pl.shape = choose_shape(p.m, p.n, ceil_div(p.k, 128), EPI_INT8, false, sm_count());
   pl.bytes = b.used > 256 ? b.used : 256;
   return pl;
+}
+
+// The quantised activations of gf_int8_linear, at the workspace's start.
+struct Quantised {
+  int64_t ld;
+  int8_t* q;
+  float* scale;
+  size_t bytes;
+};
+Quantised place_quantised(const gf_int8_product& p, void* ws) {
+  Quantised q{};
+  Bump b{static_cast<char*>(ws)};
+  q.ld = round_up<int64_t>(p.k, 16);
+  q.q = static_cast<int8_t*>(b.take(p.m * q.ld));
+  q.scale = static_cast<float*>(b.take(4 * p.m));
+  q.bytes = b.used;
+  return q;
+}
+
+gf_status int8_product(const gf_int8_product& d, const Int8Plan& pl, cudaStream_t st) {
+  const int sms = sm_count(), es = dtype_size(d.dtype);
+  Operand a{d.a, d.m, d.k, d.ld_a}, b{d.b, d.n, d.k, d.ld_b};
+  const int64_t ld = round_up<int64_t>(d.k, 16);
+  if (pl.copy_a) {
+    GFB_TRY(align_copy<uint8_t>(d.a, d.ld_a, d.m, d.k, pl.a, ld, d.m, 0, 0, sms, st));
+    a = Operand{pl.a, d.m, d.k, ld};
+  }
+  if (pl.copy_b) {
+    GFB_TRY(align_copy<uint8_t>(d.b, d.ld_b, d.n, d.k, pl.b, ld, d.n, 0, 0, sms, st));
+    b = Operand{pl.b, d.n, d.k, ld};
+  }
+  GemmParams p{};
+  GFB_TRY(set_operands(p, pl.shape, a, false, b, false, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, tc::kAccS32, tc::kFmtS8, false));
+  p.M = (int)d.m;
+  p.N = (int)d.n;
+  p.kb_total = (int)ceil_div(d.k, 128);
+  p.out = d.out;
+  p.ld_out = d.ld_out;
+  p.tma_out = aligned_rows(d.out, d.m, d.ld_out, es);
+  if (p.tma_out)
+    GFB_TRY(make_out_map(&p.mo, Operand{d.out, d.m, d.n, d.ld_out},
+                         d.dtype == GF_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                         : d.dtype == GF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         es));
+  p.bias = d.bias;
+  p.a_scale = d.a_scale;
+  p.b_scale = d.b_scale;
+  if (d.dtype == GF_F32) return launch_gemm<EPI_INT8, float, 0, false>(p, pl.shape, sms, st);
+  if (d.dtype == GF_BF16) return launch_gemm<EPI_INT8, __nv_bfloat16, 0, false>(p, pl.shape, sms, st);
+  return launch_gemm<EPI_INT8, __half, 0, false>(p, pl.shape, sms, st);
+}
+
+gf_status quantise(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q,
+                   float* scale, cudaStream_t st) {
+  const int sms = sm_count();
+  if (dtype == GF_F32) launch_quantize<float>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (dtype == GF_BF16) launch_quantize<__nv_bfloat16>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else launch_quantize<__half>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  GFB_CUDA(cudaGetLastError());
+  return GF_OK;
 }
 
 }  // namespace gfb
@@ -1640,62 +1716,56 @@ gf_status gf_quantize_rows(int64_t rows, int64_t cols, int32_t dtype, const void
   if (rows == 0) return GF_OK;
   if (!x || !q || !scale) return gf::fail(GF_ERR_INVALID_ARG, "%s: x, q and scale must be non-null", who);
   gfb::Range range("gfblock.quantize_rows");
-  const int sms = gfb::sm_count();
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GF_F32) gfb::launch_quantize<float>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (dtype == GF_BF16) gfb::launch_quantize<__nv_bfloat16>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else gfb::launch_quantize<__half>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  GFB_CUDA(cudaGetLastError());
-  return GF_OK;
+  return gfb::quantise(rows, cols, dtype, x, ld_x, q, ld_q, scale, reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t gf_int8_product_workspace_bytes(const gf_int8_product* p) {
-  if (gfb::check_int8(p) != GF_OK) return 0;
-  return p->m == 0 ? 256 : gfb::plan_int8(*p, nullptr).bytes;
+  if (gfb::check_int8("gf_int8_product_workspace_bytes", p, true) != GF_OK) return 0;
+  return p->m == 0 ? 256 : gfb::plan_int8(*p, nullptr, 0).bytes;
 }
 
 gf_status gf_int8_matmul(const gf_int8_product* d, void* workspace, size_t workspace_bytes, gf_stream stream) {
   const char* who = "gf_int8_matmul";
-  GFB_TRY(gfb::check_int8(d));
+  GFB_TRY(gfb::check_int8(who, d, true));
   if (d->m == 0) return GF_OK;
   if (!d->a || !d->b || !d->a_scale || !d->b_scale || !d->out)
     return gf::fail(GF_ERR_INVALID_ARG, "%s: a, b, a_scale, b_scale and out must be non-null", who);
-  const gfb::Int8Plan pl = gfb::plan_int8(*d, static_cast<char*>(workspace));
+  const gfb::Int8Plan pl = gfb::plan_int8(*d, static_cast<char*>(workspace), 0);
   GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
   gfb::Range range("gfblock.int8_matmul");
-  const int sms = gfb::sm_count(), es = gfb::dtype_size(d->dtype);
+  return gfb::int8_product(*d, pl, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t gf_int8_linear_workspace_bytes(const gf_int8_product* p) {
+  if (gfb::check_int8("gf_int8_linear_workspace_bytes", p, false) != GF_OK) return 0;
+  if (p->m == 0) return 256;
+  gf_int8_product d = *p;
+  const gfb::Quantised q = gfb::place_quantised(d, nullptr);
+  d.a = nullptr;  // aligned, as the workspace is
+  d.ld_a = q.ld;
+  return gfb::plan_int8(d, nullptr, q.bytes).bytes;
+}
+
+gf_status gf_int8_linear(const gf_int8_product* p, const void* x, int64_t ld_x, int32_t x_dtype, void* workspace,
+                         size_t workspace_bytes, gf_stream stream) {
+  const char* who = "gf_int8_linear";
+  GFB_TRY(gfb::check_int8(who, p, false));
+  if (!gfb::known_dtype(x_dtype)) return gf::fail(GF_ERR_UNSUPPORTED, "%s: x_dtype must be GF_F32, GF_BF16 or GF_F16", who);
+  if (ld_x < p->k) return gf::fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
+  if (p->m == 0) return GF_OK;
+  if (!x || !p->b || !p->b_scale || !p->out)
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: x, b, b_scale and out must be non-null", who);
+  gf_int8_product d = *p;
+  const gfb::Quantised q = gfb::place_quantised(d, workspace);
+  d.a = q.q;
+  d.ld_a = q.ld;
+  d.a_scale = q.scale;
+  const gfb::Int8Plan pl = gfb::plan_int8(d, static_cast<char*>(workspace), q.bytes);
+  GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
+  gfb::Range range("gfblock.int8_linear");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  gfb::Operand a{d->a, d->m, d->k, d->ld_a}, b{d->b, d->n, d->k, d->ld_b};
-  const int64_t ld = gfb::round_up<int64_t>(d->k, 16);
-  if (pl.copy_a) {
-    GFB_TRY(gfb::align_copy<uint8_t>(d->a, d->ld_a, d->m, d->k, pl.a, ld, d->m, 0, 0, sms, st));
-    a = gfb::Operand{pl.a, d->m, d->k, ld};
-  }
-  if (pl.copy_b) {
-    GFB_TRY(gfb::align_copy<uint8_t>(d->b, d->ld_b, d->n, d->k, pl.b, ld, d->n, 0, 0, sms, st));
-    b = gfb::Operand{pl.b, d->n, d->k, ld};
-  }
-  gfb::GemmParams p{};
-  GFB_TRY(gfb::set_operands(p, pl.shape, a, false, b, false, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, tc::kAccS32, tc::kFmtS8,
-                            false));
-  p.M = (int)d->m;
-  p.N = (int)d->n;
-  p.kb_total = (int)gfb::ceil_div(d->k, 128);
-  p.out = d->out;
-  p.ld_out = d->ld_out;
-  p.tma_out = gfb::aligned_rows(d->out, d->m, d->ld_out, es);
-  if (p.tma_out)
-    GFB_TRY(gfb::make_out_map(&p.mo, gfb::Operand{d->out, d->m, d->n, d->ld_out},
-                              d->dtype == GF_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                              : d->dtype == GF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                              es));
-  p.bias = d->bias;
-  p.a_scale = d->a_scale;
-  p.b_scale = d->b_scale;
-  if (d->dtype == GF_F32) return gfb::launch_gemm<gfb::EPI_INT8, float, 0, false>(p, pl.shape, sms, st);
-  if (d->dtype == GF_BF16) return gfb::launch_gemm<gfb::EPI_INT8, __nv_bfloat16, 0, false>(p, pl.shape, sms, st);
-  return gfb::launch_gemm<gfb::EPI_INT8, __half, 0, false>(p, pl.shape, sms, st);
+  GFB_TRY(gfb::quantise(d.m, d.k, x_dtype, x, ld_x, q.q, q.ld, q.scale, st));
+  return gfb::int8_product(d, pl, st);
 }
 
 gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out) {

@@ -6,43 +6,45 @@ import ctypes
 
 import torch
 
-from guass_b200 import _block, _lib
+from guass_b200 import _block
 
 
-def _run(x, p, seed, site, residual):
-    rule = _block.GfDropoutRule()
-    _block.fill_rule(rule, p, seed, site, x.device)
+def _rows(t):
+    """(tensor, rows, columns, row stride, column stride) of ``t`` as [rows,
+    last dimension], whatever its strides (a copy only where its leading
+    dimensions cannot be one)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
+    return t, *t.shape, *t.stride()
+
+
+def _run(x, rule, residual):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    r = residual if residual is not None else x
-    with _block.on_device(x):
-        _lib.check(_block.lib().gf_dropout(
-            x.shape[0], x.shape[1], _block.DTYPES[x.dtype], ctypes.byref(rule), x.data_ptr(), *x.stride(),
-            residual.data_ptr() if residual is not None else None, *r.stride(), y.data_ptr(),
-            torch.cuda.current_stream(x.device).cuda_stream))
+    x, rows, cols, row_stride, col_stride = _rows(x)
+    ptr, r_row, r_col = None, 0, 0
+    if residual is not None:
+        residual, _, _, r_row, r_col = _rows(residual)
+        ptr = residual.data_ptr()
+    _block.call(x.device, _block.lib().gf_dropout, rows, cols, _block.DTYPES[x.dtype], ctypes.byref(rule), x.data_ptr(),
+                row_stride, col_stride, ptr, r_row, r_col, y.data_ptr())
     return y
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site):
-        on_device = isinstance(seed, torch.Tensor)
-        ctx.save_for_backward(seed if on_device else None)
-        ctx.rule = (p, None if on_device else seed, site)
-        return _run(x, p, seed, site, residual)
+        rule = _block.make_rule(p, seed, site, x.device)
+        if isinstance(seed, torch.Tensor):
+            ctx.save_for_backward(seed)  # autograd then refuses one that has changed
+        ctx.rule = rule
+        return _run(x, rule, residual)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        seed, = ctx.saved_tensors
-        p, number, site = ctx.rule
-        dx = _run(dy, p, number if seed is None else seed, site, None) if ctx.needs_input_grad[0] else None
+        ctx.saved_tensors
+        dx = _run(dy, ctx.rule, None) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
-
-
-def _as_rows(t):
-    """[rows, last dimension] with whatever strides the tensor has (a copy
-    only where its leading dimensions cannot be one)."""
-    return t.reshape(-1, t.shape[-1]) if t.dim() else t.reshape(1, 1)
 
 
 def dropout(x, p: float, seed, *, site: int = 0, residual=None):
@@ -63,8 +65,7 @@ def dropout(x, p: float, seed, *, site: int = 0, residual=None):
     if residual is not None:
         _block.check_tensor("residual", residual, (x.dtype,), x.device)
         _block.require(residual.shape == x.shape, f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
-    _block.fill_rule(_block.GfDropoutRule(), p, seed, site, x.device)
     if x.numel() == 0:
+        _block.make_rule(p, seed, site, x.device)
         return x.clone() if residual is None else residual + x
-    y = _Dropout.apply(_as_rows(x), None if residual is None else _as_rows(residual), p, seed, site)
-    return y.view(x.shape)
+    return _Dropout.apply(x, residual, p, seed, site)

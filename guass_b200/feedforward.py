@@ -23,83 +23,92 @@ from guass_b200 import _block, _lib
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _describe(x, w_in, w_out, b_in, b_out, activation, p, seed, site):
+def _describe(x, w_in, w_out, b_in, b_out, activation, rule):
     f = _block.GfGatedFf()
     f.tokens, f.in_features = x.shape
-    f.hidden, f.out_features = w_out.shape[1], w_out.shape[0]
+    f.out_features, f.hidden = w_out.shape
     f.dtype = _block.DTYPES[x.dtype]
     f.activation = _block.ACTIVATIONS[activation]
-    _block.fill_rule(f.dropout, p, seed, site, x.device)
+    f.dropout = rule
     f.x, f.ld_x = x.data_ptr(), _block.ld(x)
     f.w_in, f.ld_w_in = w_in.data_ptr(), _block.ld(w_in)
     f.w_out, f.ld_w_out = w_out.data_ptr(), _block.ld(w_out)
-    f.b_in = b_in.data_ptr() if b_in is not None else None
-    f.b_out = b_out.data_ptr() if b_out is not None else None
+    if b_in is not None:
+        f.b_in = b_in.data_ptr()
+    if b_out is not None:
+        f.b_out = b_out.data_ptr()
     return f
 
 
-def _launch(L, f, backward: bool, device) -> None:
+def _workspace(L, f, backward: bool) -> int:
     n = L.gf_gated_ff_workspace_bytes(ctypes.byref(f), int(backward))
     if n == 0:
         raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
-    ws = torch.empty(n, dtype=torch.uint8, device=device)
-    fn = L.gf_gated_ff_backward if backward else L.gf_gated_ff_forward
-    _lib.check(fn(ctypes.byref(f), ws.data_ptr(), n, torch.cuda.current_stream(device).cuda_stream))
+    return n
 
 
-def _forward(x, w_in, w_out, b_in, b_out, activation, p, seed, site, keep):
+def _forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
+    """(y, h, u): h and u are the saved state, None without ``keep``."""
     L = _block.lib()
-    f = _describe(x, w_in, w_out, b_in, b_out, activation, p, seed, site)
-    hp = -(-f.hidden // 64) * 64
-    y = torch.empty(f.tokens, f.out_features, dtype=x.dtype, device=x.device)
-    h = torch.empty(f.tokens, hp, dtype=x.dtype, device=x.device)
-    u = torch.empty(f.tokens, 2 * hp, dtype=x.dtype, device=x.device) if keep else None
-    f.y, f.ld_y, f.h = y.data_ptr(), f.out_features, h.data_ptr()
-    f.u = u.data_ptr() if keep else None
+    d, (out, hidden) = x.shape[-1], w_out.shape
+    shape = x.shape
+    x, w_in, w_out = _block.rows_of(x, d), _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
+    b_in, b_out = (None if b is None else b.contiguous() for b in (b_in, b_out))
+    f = _describe(x, w_in, w_out, b_in, b_out, activation, rule)
+    y = torch.empty(*shape[:-1], out, dtype=x.dtype, device=x.device)
+    f.y, f.ld_y = y.data_ptr(), out
+    hp = -(-hidden // 64) * 64
+    h = u = None
+    if keep:
+        h = torch.empty(f.tokens, hp, dtype=x.dtype, device=x.device)
+        u = torch.empty(f.tokens, 2 * hp, dtype=x.dtype, device=x.device)
+        f.h, f.u = h.data_ptr(), u.data_ptr()
     if f.tokens:
-        _launch(L, f, False, x.device)
+        n = _workspace(L, f, False)
+        ws = torch.empty(n + (0 if keep else 2 * f.tokens * hp), dtype=torch.uint8, device=x.device)
+        if not keep:
+            f.h = ws.data_ptr() + n
+        _block.call(x.device, L.gf_gated_ff_forward, ctypes.byref(f), ws.data_ptr(), n)
     return y, h, u
 
 
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation, p, seed, site):
-        with _block.on_device(x):
-            y, h, u = _forward(x, w_in, w_out, b_in, b_out, activation, p, seed, site, True)
-        wants_w_out = ctx.needs_input_grad[2]
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, w_in, w_out, u, h if wants_w_out else None,
-                              seed if isinstance(seed, torch.Tensor) else None)
-        ctx.rule = (activation, p, None if isinstance(seed, torch.Tensor) else seed, site)
-        ctx.shape = x.shape
+        y, h, u = _forward(x, w_in, w_out, b_in, b_out, activation, _block.make_rule(p, seed, site, x.device), True)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(x if need[1] else None, w_in, w_out, u, h if need[2] else None)
+        ctx.activation, ctx.shape = activation, x.shape
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w_in, w_out, u, h, seed = ctx.saved_tensors
-        activation, p, number, site = ctx.rule
-        need = ctx.needs_input_grad
-        dy = _block.rows_of(dy, w_out.shape[0])
-        with _block.on_device(dy):
-            L = _block.lib()
-            stand_in = x if x is not None else dy.new_empty(0, ctx.shape[1])
-            f = _describe(stand_in, w_in, w_out, None, None, activation, p, number if seed is None else seed, site)
-            f.tokens = ctx.shape[0]
-            f.u = u.data_ptr()
-            f.h = h.data_ptr() if h is not None else None
-            f.dy, f.ld_dy = dy.data_ptr(), _block.ld(dy)
+        x, w_in, w_out, u, h = ctx.saved_tensors
+        need, (out, hidden), d = ctx.needs_input_grad, w_out.shape, w_in.shape[1]
+        dy = _block.rows_of(dy, out)
+        w_in, w_out = _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
+        x = dy.new_empty(0, d) if x is None else _block.rows_of(x, d)
+        L = _block.lib()
+        # the saved factors hold the dropout: the backward has no rule of its own
+        f = _describe(x, w_in, w_out, None, None, ctx.activation, _block.GfDropoutRule())
+        f.tokens = dy.shape[0]
+        f.u = u.data_ptr()
+        f.dy, f.ld_dy = dy.data_ptr(), _block.ld(dy)
+        if h is not None:
+            f.h = h.data_ptr()
 
-            def grad(wanted, *shape):
-                return torch.empty(*shape, dtype=dy.dtype, device=dy.device) if wanted else None
+        def grad(wanted, *shape):
+            return torch.empty(shape, dtype=dy.dtype, device=dy.device) if wanted else None
 
-            dx = grad(need[0], f.tokens, f.in_features)
-            dw_in = grad(need[1], 2 * f.hidden, f.in_features)
-            dw_out = grad(need[2], f.out_features, f.hidden)
-            db_in = grad(need[3], 2 * f.hidden)
-            db_out = grad(need[4], f.out_features)
-            for name, g in (("dx", dx), ("dw_in", dw_in), ("dw_out", dw_out), ("db_in", db_in), ("db_out", db_out)):
-                setattr(f, name, g.data_ptr() if g is not None else None)
-            _launch(L, f, True, dy.device)
+        dx, dw_in, dw_out = grad(need[0], *ctx.shape), grad(need[1], 2 * hidden, d), grad(need[2], out, hidden)
+        db_in, db_out = grad(need[3], 2 * hidden), grad(need[4], out)
+        for name, g in (("dx", dx), ("dw_in", dw_in), ("dw_out", dw_out), ("db_in", db_in), ("db_out", db_out)):
+            if g is not None:
+                setattr(f, name, g.data_ptr())
+        n = _workspace(L, f, True)
+        ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
+        _block.call(dy.device, L.gf_gated_ff_backward, ctypes.byref(f), ws.data_ptr(), n)
         return dx, dw_in, dw_out, db_in, db_out, None, None, None, None
 
 
@@ -114,8 +123,8 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str
     start on 16-byte boundaries cost a copy).  ``activation``: ``"gelu"`` (the
     error-function form) or ``"silu"``.  ``dropout_p``, ``seed`` and ``site``
     drop hidden activations by the rule of :func:`guass_b200.dropout.dropout`
-    on the hidden ``[rows, hidden]``; a seed tensor must not change between
-    the forward and its backward.  Returns [..., out].
+    on the hidden ``[rows, hidden]``; the backward uses the mask of its
+    forward, whatever becomes of a seed tensor.  Returns [..., out].
 
     Differentiable once in every tensor.  Work goes to the current stream of
     ``x``'s device; nothing synchronises, and both passes can be captured."""
@@ -134,12 +143,7 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str
     _block.require(b_out is None or tuple(b_out.shape) == (w_out.shape[0],), "b_out must be [out]")
     _block.require(activation in _block.ACTIVATIONS,
                    f"activation must be one of {sorted(_block.ACTIVATIONS)}, got {activation!r}")
-    _block.fill_rule(_block.GfDropoutRule(), dropout_p, seed, site, x.device)
-    flat, wi, wo = _block.rows_of(x, d), _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
-    bi, bo = (b.contiguous() if b is not None else None for b in (b_in, b_out))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (flat, wi, wo, bi, bo)):
-        y = _GatedFeedForward.apply(flat, wi, wo, bi, bo, activation, dropout_p, seed, site)
-    else:
-        with _block.on_device(x):
-            y = _forward(flat, wi, wo, bi, bo, activation, dropout_p, seed, site, False)[0]
-    return y.view(*x.shape[:-1], w_out.shape[0])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out)):
+        return _GatedFeedForward.apply(x, w_in, w_out, b_in, b_out, activation, dropout_p, seed, site)
+    rule = _block.make_rule(dropout_p, seed, site, x.device)
+    return _forward(x, w_in, w_out, b_in, b_out, activation, rule, False)[0]

@@ -33,11 +33,40 @@ def quantize_rows(x):
     kp = -(-k // 16) * 16
     q = torch.empty(v.shape[0], kp, dtype=torch.int8, device=x.device)
     scale = torch.empty(v.shape[0], dtype=torch.float32, device=x.device)
-    with _block.on_device(x):
-        _lib.check(_block.lib().gf_quantize_rows(v.shape[0], k, _block.DTYPES[x.dtype], v.data_ptr(), _block.ld(v),
-                                                 q.data_ptr(), kp, scale.data_ptr(),
-                                                 torch.cuda.current_stream(x.device).cuda_stream))
+    _block.call(x.device, _block.lib().gf_quantize_rows, v.shape[0], k, _block.DTYPES[x.dtype], v.data_ptr(),
+                _block.ld(v), q.data_ptr(), kp, scale.data_ptr())
     return q.view(*x.shape[:-1], kp)[..., :k], scale.view(x.shape[:-1])
+
+
+def _check_weight(b, b_scale, bias, out_dtype, device):
+    """[N, K] int8 with [N] scales and bias: (n, k)."""
+    _block.check_tensor("b" if bias is None else "q_weight", b, (torch.int8,), device)
+    _block.check_tensor("weight scales", b_scale, (torch.float32,), device)
+    _block.require(out_dtype in _block.DTYPES, f"out_dtype must be one of {list(_block.DTYPES)}, got {out_dtype}")
+    _block.require(b.dim() == 2, f"the int8 weight must be [N, K], got {tuple(b.shape)}")
+    n, k = b.shape
+    _block.require(n > 0 and 0 < k <= _MAX_K, f"N must be positive and K in 1..{_MAX_K}, got N={n}, K={k}")
+    _block.require(b_scale.dim() == 1 and b_scale.shape[0] == n, f"weight scales must be [{n}]")
+    if bias is not None:
+        _block.check_tensor("bias", bias, (out_dtype,), device)
+        _block.require(bias.dim() == 1 and bias.shape[0] == n, f"bias must be [{n}]")
+    return n, k
+
+
+def _describe(m, n, k, b, b_scale, bias, out):
+    d = _block.GfInt8Product()
+    d.m, d.n, d.k, d.dtype = m, n, k, _block.DTYPES[out.dtype]
+    d.b, d.ld_b, d.b_scale = b.data_ptr(), _block.ld(b), b_scale.data_ptr()
+    if bias is not None:
+        d.bias = bias.data_ptr()
+    d.out, d.ld_out = out.data_ptr(), n
+    return d
+
+
+def _workspace(size, device):
+    if size == 0:
+        raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
+    return torch.empty(size, dtype=torch.uint8, device=device)
 
 
 def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
@@ -48,55 +77,48 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
     ``out_dtype`` or None.  Any row strides; rows that do not start on 16-byte
     boundaries cost a copy."""
     _block.check_tensor("a", a, (torch.int8,))
-    _block.check_tensor("b", b, (torch.int8,), a.device)
     _block.check_tensor("a_scale", a_scale, (torch.float32,), a.device)
-    _block.check_tensor("b_scale", b_scale, (torch.float32,), a.device)
-    _block.require(out_dtype in _block.DTYPES, f"out_dtype must be one of {list(_block.DTYPES)}, got {out_dtype}")
-    _block.require(a.dim() == 2 and b.dim() == 2 and a.shape[1] == b.shape[1],
-                   f"a is {tuple(a.shape)}, b {tuple(b.shape)}: expected [M, K] and [N, K]")
-    m, k = a.shape
-    n = b.shape[0]
-    _block.require(n > 0 and 0 < k <= _MAX_K, f"N must be positive and K in 1..{_MAX_K}, got N={n}, K={k}")
-    _block.require(tuple(a_scale.shape) == (m,) and tuple(b_scale.shape) == (n,), "a_scale must be [M], b_scale [N]")
-    if bias is not None:
-        _block.check_tensor("bias", bias, (out_dtype,), a.device)
-        _block.require(tuple(bias.shape) == (n,), "bias must be [N]")
-        bias = bias.contiguous()
+    n, k = _check_weight(b, b_scale, bias, out_dtype, a.device)
+    _block.require(a.dim() == 2 and a.shape[1] == k, f"a is {tuple(a.shape)}, b {tuple(b.shape)}: expected [M, K] and [N, K]")
+    m = a.shape[0]
+    _block.require(tuple(a_scale.shape) == (m,), "a_scale must be [M]")
     a, b, a_scale, b_scale = _block.rows_of(a, k), _block.rows_of(b, k), a_scale.contiguous(), b_scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
     out = torch.empty(m, n, dtype=out_dtype, device=a.device)
     if m == 0:
         return out
-    d = _block.GfInt8Product()
-    d.m, d.n, d.k, d.dtype = m, n, k, _block.DTYPES[out_dtype]
-    d.a, d.ld_a, d.b, d.ld_b = a.data_ptr(), _block.ld(a), b.data_ptr(), _block.ld(b)
-    d.a_scale, d.b_scale = a_scale.data_ptr(), b_scale.data_ptr()
-    d.bias = bias.data_ptr() if bias is not None else None
-    d.out, d.ld_out = out.data_ptr(), n
+    d = _describe(m, n, k, b, b_scale, bias, out)
+    d.a, d.ld_a, d.a_scale = a.data_ptr(), _block.ld(a), a_scale.data_ptr()
     L = _block.lib()
-    with _block.on_device(a):
-        size = L.gf_int8_product_workspace_bytes(ctypes.byref(d))
-        if size == 0:
-            raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
-        ws = torch.empty(size, dtype=torch.uint8, device=a.device)
-        _lib.check(L.gf_int8_matmul(ctypes.byref(d), ws.data_ptr(), size,
-                                    torch.cuda.current_stream(a.device).cuda_stream))
+    ws = _workspace(L.gf_int8_product_workspace_bytes(ctypes.byref(d)), a.device)
+    _block.call(a.device, L.gf_int8_matmul, ctypes.byref(d), ws.data_ptr(), ws.shape[0])
     return out
 
 
 def int8_linear(x, q_weight, weight_scale, bias=None, *, out_dtype=None):
     """``linear(x, q_weight * weight_scale[:, None], bias)`` with ``x`` [..., K]
-    quantised row by row (:func:`quantize_rows`); ``out_dtype`` defaults to
-    ``x``'s.  Forward only: refuses an ``x`` that needs a gradient."""
+    (fp32, bf16 or fp16) quantised row by row as :func:`quantize_rows` does;
+    ``q_weight`` [N, K] int8, ``weight_scale`` [N] fp32, ``bias`` [N] of
+    ``out_dtype``, which defaults to ``x``'s.  Forward only: refuses an ``x``
+    that needs a gradient."""
     _block.check_tensor("x", x, tuple(_block.DTYPES))
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("int8_linear has no backward: call it under torch.no_grad() or on a detached input")
-    _block.check_tensor("q_weight", q_weight, (torch.int8,), x.device)
-    _block.require(x.dim() >= 1 and q_weight.dim() == 2 and x.shape[-1] == q_weight.shape[1],
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    n, k = _check_weight(q_weight, weight_scale, bias, out_dtype, x.device)
+    _block.require(x.dim() >= 1 and x.shape[-1] == k,
                    f"x is {tuple(x.shape)}, q_weight {tuple(q_weight.shape)}: expected [..., K] and [N, K]")
-    q, scale = quantize_rows(x)
-    y = int8_matmul(q.reshape(-1, q.shape[-1]), scale.reshape(-1), q_weight, weight_scale, bias,
-                    out_dtype=x.dtype if out_dtype is None else out_dtype)
-    return y.view(*x.shape[:-1], q_weight.shape[0])
+    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    x, q_weight, weight_scale = _block.rows_of(x, k), _block.rows_of(q_weight, k), weight_scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    d = _describe(x.shape[0], n, k, q_weight, weight_scale, bias, out)
+    L = _block.lib()
+    ws = _workspace(L.gf_int8_linear_workspace_bytes(ctypes.byref(d)), x.device)
+    _block.call(x.device, L.gf_int8_linear, ctypes.byref(d), x.data_ptr(), _block.ld(x), _block.DTYPES[x.dtype],
+                ws.data_ptr(), ws.shape[0])
+    return out
 
 
 class Int8Linear(nn.Module):

@@ -125,6 +125,12 @@ typedef struct gf_int8_product {
 size_t gf_int8_product_workspace_bytes(const gf_int8_product* p);
 gf_status gf_int8_matmul(const gf_int8_product* p, void* workspace, size_t workspace_bytes, gf_stream stream);
 
+/* out = quantise(x) b^T with x [m, k] of x_dtype, quantised row by row as
+ * gf_quantize_rows does; a, ld_a and a_scale of the product are not used. */
+size_t gf_int8_linear_workspace_bytes(const gf_int8_product* p);
+gf_status gf_int8_linear(const gf_int8_product* p, const void* x, int64_t ld_x, int32_t x_dtype, void* workspace,
+                         size_t workspace_bytes, gf_stream stream);
+
 /* Synchronises `stream` and returns the condition bits that these operators
  * set on the current device since the last reset. */
 gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out);

@@ -138,6 +138,13 @@ def test_dropout_and_int8_descriptions_refused():
     assert product(size=8) == bad and "too small" in _lib.last_error()
     assert product(k=131072, ld_a=131072, ld_b=131072) == no and product(dtype=9) == no and product(m=1 << 31) == no
     assert product(m=0, a=None) == _lib.GF_OK
+
+    def linear(ws=FAKE, size=1 << 20, x=FAKE, ld_x=16, x_dtype=0, **kw):
+        d = dict(m=2, n=2, k=16, b=FAKE, b_scale=FAKE, out=FAKE, ld_b=16, ld_out=2)
+        return L.gf_int8_linear(ctypes.byref(_block.GfInt8Product(**{**d, **kw})), x, ld_x, x_dtype, ws, size, None)
+
+    assert linear(x=None) == bad and linear(ld_x=15) == bad and linear(b=None) == bad and linear(size=256) == bad
+    assert linear(x_dtype=5) == no and linear(ws=None) == bad and linear(m=0, x=None) == _lib.GF_OK
     assert L.gf_block_status(None, 0, None) == bad
 
 
@@ -153,13 +160,12 @@ def test_python_entry_points_refuse_cpu_tensors_and_wrong_types():
         int8_linear(x, x, x)
     with pytest.raises(TypeError, match="torch.Tensor"):
         int8_matmul([1], None, None, None)
-    rule = _block.GfDropoutRule()
     for p in (-0.1, 1.0, float("nan")):
         with pytest.raises(ValueError, match="probability"):
-            _block.fill_rule(rule, p, 0, 0, None)
+            _block.make_rule(p, 0, 0, None)
     with pytest.raises(ValueError, match="site"):
-        _block.fill_rule(rule, 0.1, 0, 1 << 32, None)
-    _block.fill_rule(rule, 0.1, -1, 3, None)
+        _block.make_rule(0.1, 0, 1 << 32, None)
+    rule = _block.make_rule(0.1, -1, 3, None)
     assert (rule.seed, rule.site) == (0xFFFFFFFFFFFFFFFF, 3)
 
 
