@@ -825,57 +825,228 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
 }
 
 // ---------------------------------------------------------------------------
-// column sums (bias gradients): rows cut into `parts` runs, each summed in
-// order, the runs then added in order
+// column sums (bias gradients): rows cut into runs, each summed in order, the
+// runs then added in order.  One launch does up to two matrices (blockIdx.z).
+
+struct SumJob {
+  const void* src;
+  int64_t ld;
+  int32_t rows, cols, run, parts;
+  int32_t seg_pad, seg;  // results: `seg` columns from 0 and from seg_pad (0: all columns)
+  float* partial;        // [parts][cols]
+  void* out;
+};
+struct SumJobs {
+  SumJob job[2];
+};
 
 template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const T* src, int64_t ld, int rows, int cols, int run,
-                                                          float* partial) {
+__global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ SumJobs jobs) {
+  const SumJob& j = jobs.job[blockIdx.z];
   const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
-  const int64_t r0 = (int64_t)blockIdx.y * run, r1 = min((int64_t)rows, r0 + run);
+  if ((int)blockIdx.x * 32 >= j.cols || (int)blockIdx.y >= j.parts) return;
+  const T* src = static_cast<const T*>(j.src);
+  const int64_t r0 = (int64_t)blockIdx.y * j.run, r1 = min((int64_t)j.rows, r0 + j.run);
   float s = 0.0f;
-  if (c < cols)
-    for (int64_t r = r0 + w; r < r1; r += 8) s += to_float(src[r * ld + c]);
+  if (c < j.cols)
+    for (int64_t r = r0 + w; r < r1; r += 8) s += to_float(src[r * j.ld + c]);
   __shared__ float sums[8][32];
   sums[w][threadIdx.x % 32] = s;
   __syncthreads();
-  if (w == 0 && c < cols) {
+  if (w == 0 && c < j.cols) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-    partial[(int64_t)blockIdx.y * cols + c] = s;
+    j.partial[(int64_t)blockIdx.y * j.cols + c] = s;
   }
 }
-// out[c] = sum over the runs; `seg` columns from 0 and from seg_pad (0: all)
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(const float* partial, int parts, int cols, int seg_pad, int seg,
-                                                          T* out) {
+__global__ void __launch_bounds__(256) column_join_kernel(const __grid_constant__ SumJobs jobs) {
+  const SumJob& j = jobs.job[blockIdx.z];
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  const int n = seg_pad ? 2 * seg : cols;
-  if (i >= n) return;
-  const int c = seg_pad && i >= seg ? seg_pad + i - seg : i;
+  if (i >= (j.seg_pad ? 2 * j.seg : j.cols)) return;
+  const int c = j.seg_pad && i >= j.seg ? j.seg_pad + i - j.seg : i;
   float s = 0.0f;
-  for (int k = 0; k < parts; ++k) s += partial[(int64_t)k * cols + c];
-  out[i] = from_float<T>(s);
+  for (int k = 0; k < j.parts; ++k) s += j.partial[(int64_t)k * j.cols + c];
+  static_cast<T*>(j.out)[i] = from_float<T>(s);
 }
 
 // ---------------------------------------------------------------------------
-// copies into 16-byte aligned rows: dst row r holds src row r (or, with two
-// runs of rows, src rows 0 .. seg - 1 and seg .. 2 seg - 1 at 0 and seg_pad);
-// everything else is zero
+// copies into 16-byte aligned rows, up to four in one launch (blockIdx.y): dst
+// row r holds src row r (or, with two runs of rows, src rows 0 .. seg - 1 and
+// seg .. 2 seg - 1 at 0 and seg_pad); everything else is zero
+
+struct AlignJob {
+  const void* src;
+  void* dst;
+  int64_t ld, src_rows, dst_rows;
+  int32_t cols, ld_dst, seg_pad, seg;
+};
+struct AlignJobs {
+  AlignJob job[4];
+  int n;
+};
 
 template <typename E>
-__global__ void __launch_bounds__(256) align_kernel(const E* src, int64_t ld, int64_t src_rows, int cols, E* dst,
-                                                    int ld_dst, int64_t dst_rows, int seg_pad, int seg) {
-  const int64_t total = dst_rows * ld_dst;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ld_dst;
-    const int c = (int)(i - r * ld_dst);
+__global__ void __launch_bounds__(256) align_kernel(const __grid_constant__ AlignJobs jobs) {
+  const AlignJob& j = jobs.job[blockIdx.y];
+  // a warp copies whole rows
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < j.dst_rows; r += (int64_t)gridDim.x * 8) {
     int64_t from = r;
-    if (seg_pad) {
-      const int64_t in = r >= seg_pad ? r - seg_pad : r;
-      from = in < seg ? (r >= seg_pad ? seg + in : in) : src_rows;
+    if (j.seg_pad) {
+      const int64_t in = r >= j.seg_pad ? r - j.seg_pad : r;
+      from = in < j.seg ? (r >= j.seg_pad ? j.seg + in : in) : j.src_rows;
     }
-    dst[i] = from < src_rows && c < cols ? src[from * ld + c] : E(0);
+    const E* src = static_cast<const E*>(j.src) + from * j.ld;
+    E* dst = static_cast<E*>(j.dst) + r * j.ld_dst;
+    const int cols = from < j.src_rows ? j.cols : 0;
+    for (int c = lane; c < j.ld_dst; c += 32) dst[c] = c < cols ? src[c] : E(0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The block for a few tokens, where it is a walk over the weights: a warp
+// takes a column of h (both its rows of w_in) or of y, four warps sharing a
+// long row; each lane holds 16 bytes of the row at a time against the tokens'
+// same columns in shared memory.  Rows are 16-byte aligned.
+
+constexpr int kSkinnyTokens = 8;
+constexpr int kSkinnyWarps = 8;
+
+struct SkinnyParams {
+  const void *x, *w, *bias;  // x [tokens, k], w [n or two runs of n, k]
+  int64_t ld_x, ld_w, gate_row;
+  int32_t tokens, n, k, hp;
+  void *out, *u;
+  int64_t ld_out;
+  int32_t act;
+  DropArgs drop;
+};
+
+template <typename T, int TOKENS, bool GATED>
+__global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_constant__ SkinnyParams p) {
+  constexpr int kRows = GATED ? 2 : 1;
+  constexpr int kShare = GATED ? 1 : 4;             // warps of a column
+  constexpr int kChunk = 2048;                      // columns of x in shared memory at a time
+  __shared__ __align__(16) T xs[TOKENS][kChunk];
+  __shared__ float part[kSkinnyWarps][TOKENS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = blockIdx.x * (kSkinnyWarps / kShare) + warp / kShare;
+  const bool live = n < p.n;
+  float sum[kRows][TOKENS] = {};
+  for (int k0 = 0; k0 < p.k; k0 += kChunk) {
+    const int len = min(kChunk, p.k - k0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < TOKENS * (kChunk / 8); i += 32 * kSkinnyWarps) {
+      const int m = i / (kChunk / 8), c = i % (kChunk / 8) * 8;
+      if (c >= len) continue;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      const T* src = static_cast<const T*>(p.x) + m * p.ld_x + k0 + c;
+      if (m < p.tokens && c + 8 <= len) v = *reinterpret_cast<const uint4*>(src);
+      *reinterpret_cast<uint4*>(&xs[m][c]) = v;
+      if (m < p.tokens && c + 8 > len)
+        for (int j = 0; c + j < len; ++j) xs[m][c + j] = src[j];
+    }
+    __syncthreads();
+    if (!live) continue;
+    const T* w = static_cast<const T*>(p.w) + n * p.ld_w + k0;
+    auto add = [&](const uint4 (&v)[kRows], int c) {
+#pragma unroll
+      for (int m = 0; m < TOKENS; ++m) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(&xs[m][c]);
+        const uint32_t* xw = reinterpret_cast<const uint32_t*>(&xv);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          const uint32_t* ww = reinterpret_cast<const uint32_t*>(&v[r]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 a = unpack2<T>(xw[j]), b = unpack2<T>(ww[j]);
+            sum[r][m] = fmaf(a.x, b.x, fmaf(a.y, b.y, sum[r][m]));
+          }
+        }
+      }
+    };
+    constexpr int kStep = 256 * kShare, kAhead = 4;  // loads in flight
+    const int whole = len & ~7;
+    int c = 8 * (lane + 32 * (warp % kShare));
+    for (; c + (kAhead - 1) * kStep < whole; c += kAhead * kStep) {
+      uint4 v[kAhead][kRows];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) v[i][r] = *reinterpret_cast<const uint4*>(w + r * p.gate_row * p.ld_w + c + i * kStep);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add(v[i], c + i * kStep);
+    }
+    for (; c < len; c += kStep) {
+      uint4 v[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const T* at = w + r * p.gate_row * p.ld_w + c;
+        if (c < whole) {
+          v[r] = *reinterpret_cast<const uint4*>(at);
+        } else {  // the row's last few: what follows is not its own
+          T tail[8];
+          for (int j = 0; j < 8; ++j) tail[j] = c + j < len ? at[j] : T(0.0f);
+          v[r] = *reinterpret_cast<const uint4*>(tail);
+        }
+      }
+      add(v, c);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m)
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum[r][m] += __shfl_xor_sync(0xFFFFFFFFu, sum[r][m], d);
+  const T* bias = static_cast<const T*>(p.bias);
+  if constexpr (GATED) {
+    // lane m finishes token m; the padding columns of h and u are zeros
+    float a = 0.0f, g = 0.0f;
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m)
+      if (lane == m) a = sum[0][m], g = sum[1][m];
+    if (live && lane < p.tokens) {
+      if (bias) a += to_float(bias[n]), g += to_float(bias[p.n + n]);
+      uint64_t value, slope;
+      if (p.act == GF_ACT_GELU) activate<GF_ACT_GELU, true>(g, g, value, slope);
+      else activate<GF_ACT_SILU, true>(g, g, value, slope);
+      float v = tc::unpack_f2(value).x, s = tc::unpack_f2(slope).x * a;
+      if (p.drop.on) {
+        const uint4 w = Philox(p.drop)((uint32_t)n >> 2, (uint32_t)lane);
+        const uint32_t word = (n & 3) == 0 ? w.x : (n & 3) == 1 ? w.y : (n & 3) == 2 ? w.z : w.w;
+        const float keep = word >= p.drop.threshold ? p.drop.scale : 0.0f;
+        v = keep * v;
+        s = keep * s;
+      }
+      T* out = static_cast<T*>(p.out) + lane * p.ld_out + n;
+      *out = from_float<T>(a * v);
+      if (p.u) {
+        T* u = static_cast<T*>(p.u) + lane * 2 * (int64_t)p.hp + n;
+        u[0] = from_float<T>(v);
+        u[p.hp] = from_float<T>(s);
+      }
+    } else if (!live && n < p.hp && lane < p.tokens) {
+      static_cast<T*>(p.out)[lane * p.ld_out + n] = T(0.0f);
+      if (p.u) {
+        T* u = static_cast<T*>(p.u) + lane * 2 * (int64_t)p.hp + n;
+        u[0] = u[p.hp] = T(0.0f);
+      }
+    }
+  } else {
+    float y = 0.0f;
+#pragma unroll
+    for (int m = 0; m < TOKENS; ++m)
+      if (lane == m) y = sum[0][m];
+    if (lane < TOKENS) part[warp][lane] = y;
+    __syncthreads();
+    if (live && warp % kShare == 0 && lane < p.tokens) {
+      y = bias ? to_float(bias[n]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) y += part[warp + i][lane];
+      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(y);
+    }
   }
 }
 
@@ -1237,10 +1408,10 @@ struct Bump {  // workspace layout: offsets first (null base), pointers when it 
 
 struct FfPlan {
   int64_t M, D, F, O, Hp;
-  bool copy_x, copy_w_in, copy_w_out, copy_dy;
+  bool skinny, copy_x, copy_w_in, copy_w_out, copy_dy;
   Shape in, out, dh, dx, dw_in, dw_out;
   int in_parts, in_run, out_parts, out_run;  // column sums
-  void *x, *w_in, *w_out, *dy, *du, *partial, *sums;
+  void *x, *w_in, *w_out, *dy, *du, *partial, *in_sums, *out_sums;
   size_t bytes;
 };
 
@@ -1260,6 +1431,12 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
   p.M = f.tokens, p.D = f.in_features, p.F = f.hidden, p.O = f.out_features;
   p.Hp = round_up<int64_t>(p.F, 64);
   const bool back = pass == GF_PASS_BACKWARD;
+  p.skinny = !back && p.M <= kSkinnyTokens && aligned_rows(f.x, p.M, f.ld_x, 2) &&
+             aligned_rows(f.w_in, 2 * p.F, f.ld_w_in, 2) && aligned_rows(f.w_out, p.O, f.ld_w_out, 2);
+  if (p.skinny) {
+    p.bytes = 256;
+    return p;
+  }
   const bool use_x = !back || f.dw_in, use_w_in = !back || f.dx;
   const bool use_du = back && (f.dx || f.dw_in || f.db_in);
   const bool use_w_out = !back || use_du, use_dy = back && (use_du || f.dw_out);
@@ -1272,7 +1449,7 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
   if (p.copy_w_in) p.w_in = b.take(2 * 2 * p.Hp * round_up<int64_t>(p.D, 8));
   if (p.copy_w_out) p.w_out = b.take(2 * p.O * round_up<int64_t>(p.F, 8));
   if (p.copy_dy) p.dy = b.take(2 * p.M * round_up<int64_t>(p.O, 8));
-  size_t partial = 0, sums = 0;
+  size_t partial = 0;
   auto need = [&](const Shape& s, int64_t N) {
     const size_t n = partial_bytes(s, N);
     if (n > partial) partial = n;
@@ -1300,16 +1477,14 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
     }
     if (f.db_in) {
       column_runs(p.M, 2 * p.Hp, sms, &p.in_parts, &p.in_run);
-      sums = (size_t)4 * p.in_parts * 2 * p.Hp;
+      p.in_sums = b.take((size_t)4 * p.in_parts * 2 * p.Hp);
     }
     if (f.db_out) {
       column_runs(p.M, p.O, sms, &p.out_parts, &p.out_run);
-      const size_t n = (size_t)4 * p.out_parts * p.O;
-      if (n > sums) sums = n;
+      p.out_sums = b.take((size_t)4 * p.out_parts * p.O);
     }
   }
   if (partial) p.partial = b.take(partial);
-  if (sums) p.sums = b.take(sums);
   p.bytes = b.used > 256 ? b.used : 256;
   return p;
 }
@@ -1336,11 +1511,16 @@ gf_status check_workspace(const char* who, const void* ws, size_t have, size_t w
   return GF_OK;
 }
 
+void add_align(AlignJobs& jobs, const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ld_dst,
+               int64_t dst_rows, int64_t seg_pad, int64_t seg) {
+  jobs.job[jobs.n++] = AlignJob{src, dst, ld, rows, dst_rows, (int)cols, (int)ld_dst, (int)seg_pad, (int)seg};
+}
 template <typename E>
-gf_status align_copy(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ld_dst, int64_t dst_rows,
-                     int64_t seg_pad, int64_t seg, int sms, cudaStream_t st) {
-  align_kernel<E><<<grid_for(dst_rows * ld_dst, 256, sms), 256, 0, st>>>(
-      static_cast<const E*>(src), ld, rows, (int)cols, static_cast<E*>(dst), (int)ld_dst, dst_rows, (int)seg_pad, (int)seg);
+gf_status run_align(const AlignJobs& jobs, int sms, cudaStream_t st) {
+  if (jobs.n == 0) return GF_OK;
+  int64_t rows = 0;
+  for (int i = 0; i < jobs.n; ++i) rows = jobs.job[i].dst_rows > rows ? jobs.job[i].dst_rows : rows;
+  align_kernel<E><<<dim3(grid_for(rows, 8, sms), jobs.n), 256, 0, st>>>(jobs);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(GF_ERR_CUDA, "align_kernel: %s", cudaGetErrorString(e));
   return GF_OK;
@@ -1363,23 +1543,24 @@ gf_status align_ff(const gf_gated_ff& f, const FfPlan& p, FfOperands* o, int sms
   o->w_out = Operand{f.w_out, p.O, p.F, f.ld_w_out};
   o->dy = Operand{f.dy, p.M, p.O, f.ld_dy};
   const int64_t ld_d = round_up<int64_t>(p.D, 8), ld_f = round_up<int64_t>(p.F, 8), ld_o = round_up<int64_t>(p.O, 8);
+  AlignJobs jobs{};
   if (p.copy_x) {
-    GFB_TRY(align_copy<uint16_t>(f.x, f.ld_x, p.M, p.D, p.x, ld_d, p.M, 0, 0, sms, st));
+    add_align(jobs, f.x, f.ld_x, p.M, p.D, p.x, ld_d, p.M, 0, 0);
     o->x = Operand{p.x, p.M, p.D, ld_d};
   }
   if (p.copy_w_in) {
-    GFB_TRY(align_copy<uint16_t>(f.w_in, f.ld_w_in, 2 * p.F, p.D, p.w_in, ld_d, 2 * p.Hp, p.Hp, p.F, sms, st));
+    add_align(jobs, f.w_in, f.ld_w_in, 2 * p.F, p.D, p.w_in, ld_d, 2 * p.Hp, p.Hp, p.F);
     o->w_in = Operand{p.w_in, 2 * p.Hp, p.D, ld_d};
   }
   if (p.copy_w_out) {
-    GFB_TRY(align_copy<uint16_t>(f.w_out, f.ld_w_out, p.O, p.F, p.w_out, ld_f, p.O, 0, 0, sms, st));
+    add_align(jobs, f.w_out, f.ld_w_out, p.O, p.F, p.w_out, ld_f, p.O, 0, 0);
     o->w_out = Operand{p.w_out, p.O, p.F, ld_f};
   }
   if (p.copy_dy) {
-    GFB_TRY(align_copy<uint16_t>(f.dy, f.ld_dy, p.M, p.O, p.dy, ld_o, p.M, 0, 0, sms, st));
+    add_align(jobs, f.dy, f.ld_dy, p.M, p.O, p.dy, ld_o, p.M, 0, 0);
     o->dy = Operand{p.dy, p.M, p.O, ld_o};
   }
-  return GF_OK;
+  return run_align<uint16_t>(jobs, sms, st);
 }
 
 template <typename T>
@@ -1431,8 +1612,41 @@ gf_status gated(const GemmParams& p, const Shape& s, int act, int sms, cudaStrea
                    : launch_gemm<EPI_GATED, T, GF_ACT_SILU, false>(p, s, sms, st);
 }
 
+template <typename T, bool GATED>
+gf_status skinny(const SkinnyParams& p, cudaStream_t st) {
+  // (gated: a warp per column of h, padding included; else four per column of y)
+  const int cols = GATED ? p.hp : p.n, per = GATED ? kSkinnyWarps : kSkinnyWarps / 4;
+  const int grid = (int)ceil_div(cols, per);
+  if (p.tokens == 1) skinny_kernel<T, 1, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
+  else if (p.tokens <= 4) skinny_kernel<T, 4, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
+  else skinny_kernel<T, kSkinnyTokens, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
+  GFB_CUDA(cudaGetLastError());
+  return GF_OK;
+}
+
+template <typename T>
+gf_status ff_skinny(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
+  SkinnyParams p{};
+  p.x = f.x, p.ld_x = f.ld_x;
+  p.w = f.w_in, p.ld_w = f.ld_w_in, p.gate_row = pl.F;
+  p.bias = f.b_in;
+  p.tokens = (int)pl.M, p.n = (int)pl.F, p.k = (int)pl.D, p.hp = (int)pl.Hp;
+  p.out = f.h, p.ld_out = pl.Hp;
+  p.u = f.u;
+  p.act = f.activation;
+  p.drop = drop_args(f.dropout);
+  GFB_TRY((skinny<T, true>(p, st)));
+  p.x = f.h, p.ld_x = pl.Hp;
+  p.w = f.w_out, p.ld_w = f.ld_w_out;
+  p.bias = f.b_out;
+  p.n = (int)pl.O, p.k = (int)pl.F;
+  p.out = f.y, p.ld_out = f.ld_y;
+  return skinny<T, false>(p, st);
+}
+
 template <typename T>
 gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
+  if (pl.skinny) return ff_skinny<T>(f, pl, st);
   const int sms = sm_count();
   FfOperands o;
   GFB_TRY(align_ff(f, pl, &o, sms, st));
@@ -1454,15 +1668,16 @@ gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
 }
 
 template <typename T>
-gf_status column_sums(const void* src, int64_t ld, int64_t rows, int64_t cols, int parts, int run, void* partial,
-                      int64_t seg_pad, int64_t seg, void* out, cudaStream_t st) {
-  const dim3 grid((unsigned)ceil_div(cols, 32), (unsigned)parts);
-  column_sums_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(src), ld, (int)rows, (int)cols, run,
-                                              static_cast<float*>(partial));
+gf_status column_sums(const SumJobs& jobs, int n, cudaStream_t st) {
+  int64_t cols = 0;
+  int parts = 0;
+  for (int i = 0; i < n; ++i) {
+    cols = jobs.job[i].cols > cols ? jobs.job[i].cols : cols;
+    parts = jobs.job[i].parts > parts ? jobs.job[i].parts : parts;
+  }
+  column_sums_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), parts, n), 256, 0, st>>>(jobs);
   GFB_CUDA(cudaGetLastError());
-  const int64_t n = seg_pad ? 2 * seg : cols;
-  column_join_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(static_cast<const float*>(partial), parts, (int)cols,
-                                                                    (int)seg_pad, (int)seg, static_cast<T*>(out));
+  column_join_kernel<T><<<dim3((unsigned)ceil_div(cols, 256), 1, n), 256, 0, st>>>(jobs);
   GFB_CUDA(cudaGetLastError());
   return GF_OK;
 }
@@ -1492,12 +1707,15 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   if (f.dw_out)
     GFB_TRY(product<T>(pl.dw_out, o.dy, true, Operand{f.h, pl.M, pl.Hp, pl.Hp}, true, pl.O, pl.F, pl.M, f.dw_out, pl.F,
                        nullptr, 0, 0, pl.partial, sms, st));
+  SumJobs sums{};
+  int n = 0;
   if (f.db_in)
-    GFB_TRY(column_sums<T>(pl.du, 2 * pl.Hp, pl.M, 2 * pl.Hp, pl.in_parts, pl.in_run, pl.sums, pl.Hp == pl.F ? 0 : pl.Hp,
-                           pl.F, f.db_in, st));
+    sums.job[n++] = SumJob{pl.du, 2 * pl.Hp, (int)pl.M, (int)(2 * pl.Hp), pl.in_run, pl.in_parts,
+                           pl.Hp == pl.F ? 0 : (int)pl.Hp, (int)pl.F, static_cast<float*>(pl.in_sums), f.db_in};
   if (f.db_out)
-    GFB_TRY(column_sums<T>(f.dy, f.ld_dy, pl.M, pl.O, pl.out_parts, pl.out_run, pl.sums, 0, 0, f.db_out, st));
-  return GF_OK;
+    sums.job[n++] = SumJob{f.dy, f.ld_dy, (int)pl.M, (int)pl.O, pl.out_run, pl.out_parts, 0, 0,
+                           static_cast<float*>(pl.out_sums), f.db_out};
+  return n ? column_sums<T>(sums, n, st) : GF_OK;
 }
 
 // ---- dropout and the 8-bit product
@@ -1579,14 +1797,16 @@ gf_status int8_product(const gf_int8_product& d, const Int8Plan& pl, cudaStream_
   const int sms = sm_count(), es = dtype_size(d.dtype);
   Operand a{d.a, d.m, d.k, d.ld_a}, b{d.b, d.n, d.k, d.ld_b};
   const int64_t ld = round_up<int64_t>(d.k, 16);
+  AlignJobs jobs{};
   if (pl.copy_a) {
-    GFB_TRY(align_copy<uint8_t>(d.a, d.ld_a, d.m, d.k, pl.a, ld, d.m, 0, 0, sms, st));
+    add_align(jobs, d.a, d.ld_a, d.m, d.k, pl.a, ld, d.m, 0, 0);
     a = Operand{pl.a, d.m, d.k, ld};
   }
   if (pl.copy_b) {
-    GFB_TRY(align_copy<uint8_t>(d.b, d.ld_b, d.n, d.k, pl.b, ld, d.n, 0, 0, sms, st));
+    add_align(jobs, d.b, d.ld_b, d.n, d.k, pl.b, ld, d.n, 0, 0);
     b = Operand{pl.b, d.n, d.k, ld};
   }
+  GFB_TRY(run_align<uint8_t>(jobs, sms, st));
   GemmParams p{};
   GFB_TRY(set_operands(p, pl.shape, a, false, b, false, 1, CU_TENSOR_MAP_DATA_TYPE_UINT8, tc::kAccS32, tc::kFmtS8, false));
   p.M = (int)d.m;

@@ -449,3 +449,19 @@ def test_seed_changed_before_backward_is_refused():
     seed.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("size", [(320, 1280, 320), (2056, 72, 40), (77, 130, 9), (1280, 4100, 24)])
+def test_ff_few_tokens(size, tokens, dtype):
+    """The walk over the weights (up to 8 tokens) and its border, rows of any length on 16-byte boundaries."""
+    d, f, o = size
+    t = ff_inputs(tokens, d, f, o, dtype, bias=True)
+    for n in ("x", "w_in", "w_out"):  # rows padded to whole 16 bytes, with values that must not be read as theirs
+        rows, cols = t[n].shape
+        wide = torch.full((rows, -(-cols // 8) * 8 + 8), float("nan"), dtype=dtype, device="cuda")
+        wide[:, :cols] = t[n]
+        t[n] = wide[:, :cols]
+    ff_check(t, "gelu", p=0.25, seed=4, site=2)
+    ff_check(t, "silu", wants=())
