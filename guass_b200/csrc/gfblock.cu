@@ -1065,88 +1065,118 @@ struct DropoutParams {
 };
 
 // One thread takes V columns of a row at a time: 16 bytes of aligned rows, or
-// (VEC false) four elements through any strides.  ROWS: neighbouring threads
-// take neighbouring rows, for inputs whose rows are the contiguous dimension.
-template <typename T, bool VEC, bool ROWS>
+// (VEC false) four elements through any strides; two such groups per turn, so
+// that the loads of both are on their way while the generator works.  ROWS:
+// neighbouring threads take neighbouring rows, for inputs whose rows are the
+// contiguous dimension.  I: the type that holds rows * groups.
+template <typename T, bool VEC, bool ROWS, bool RES, typename I>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
-  constexpr int V = VEC ? 16 / sizeof(T) : 4;
+  constexpr int V = VEC ? 16 / sizeof(T) : 4, U = 2;
   const Philox rng(p.drop);
-  const int64_t inner = ROWS ? p.rows : p.groups, outer = ROWS ? p.groups : p.rows;
-  const int64_t step = (int64_t)gridDim.x * blockDim.x;
-  const int64_t step_o = step / inner, step_i = step - step_o * inner;
-  int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  int64_t o = i / inner;
+  const I inner = (I)(ROWS ? p.rows : p.groups), outer = (I)(ROWS ? p.groups : p.rows);
+  const I step = (I)gridDim.x * blockDim.x;
+  const I step_o = step / inner, step_i = step - step_o * inner;
+  I i = (I)blockIdx.x * blockDim.x + threadIdx.x;
+  I o = i / inner;
   i -= o * inner;
   while (o < outer) {
-    const int64_t row = ROWS ? i : o, group = ROWS ? o : i;
-    const int64_t col = group * V;
-    const T* x = static_cast<const T*>(p.x) + row * p.x_rs + col * p.x_cs;
-    const T* res = p.res ? static_cast<const T*>(p.res) + row * p.r_rs + col * p.r_cs : nullptr;
-    T* y = static_cast<T*>(p.y) + row * p.cols + col;
-    T in[V], add[V], out[V];
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(in) = *reinterpret_cast<const uint4*>(x);
-      if (res) *reinterpret_cast<uint4*>(add) = *reinterpret_cast<const uint4*>(res);
-    } else {
+    T in[U][V], add[U][V];
+    int64_t rows[U], cols[U];
+    bool live[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (col + j < p.cols) {
-          in[j] = x[j * p.x_cs];
-          if (res) add[j] = res[j * p.r_cs];
+    for (int u = 0; u < U; ++u) {
+      live[u] = o < outer;
+      const int64_t row = rows[u] = ROWS ? i : o, col = cols[u] = (int64_t)(ROWS ? o : i) * V;
+      if (live[u]) {
+        const T* x = static_cast<const T*>(p.x) + row * p.x_rs + col * p.x_cs;
+        const T* res = static_cast<const T*>(p.res) + row * p.r_rs + col * p.r_cs;
+        if constexpr (VEC) {
+          *reinterpret_cast<uint4*>(in[u]) = *reinterpret_cast<const uint4*>(x);
+          if constexpr (RES) *reinterpret_cast<uint4*>(add[u]) = *reinterpret_cast<const uint4*>(res);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (col + j < p.cols) {
+              in[u][j] = x[j * p.x_cs];
+              if constexpr (RES) add[u][j] = res[j * p.r_cs];
+            }
         }
+      }
+      o += step_o;
+      i += step_i;
+      if (i >= inner) i -= inner, ++o;
     }
 #pragma unroll
-    for (int b = 0; b < V / 4; ++b) {
-      const uint4 w = rng((uint32_t)(col / 4 + b), (uint64_t)row);
-      const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+    for (int u = 0; u < U; ++u) {
+      if (!live[u]) continue;
+      T out[V];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v = word[j] >= p.drop.threshold ? to_float(in[4 * b + j]) * p.drop.scale : 0.0f;
-        if (res) v += to_float(add[4 * b + j]);
-        out[4 * b + j] = from_float<T>(v);
+      for (int b = 0; b < V / 4; ++b) {
+        const uint4 w = rng((uint32_t)(cols[u] / 4 + b), (uint64_t)rows[u]);
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v = word[j] >= p.drop.threshold ? to_float(in[u][4 * b + j]) * p.drop.scale : 0.0f;
+          if constexpr (RES) v += to_float(add[u][4 * b + j]);
+          out[4 * b + j] = from_float<T>(v);
+        }
+      }
+      T* y = static_cast<T*>(p.y) + rows[u] * p.cols + cols[u];
+      if constexpr (VEC) {
+        *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(out);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (cols[u] + j < p.cols) y[j] = out[j];
       }
     }
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(out);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (col + j < p.cols) y[j] = out[j];
-    }
-    o += step_o;
-    i += step_i;
-    if (i >= inner) i -= inner, ++o;
   }
 }
 
 // ---------------------------------------------------------------------------
-// row quantisation: TPR threads per row, two passes over the row (the second
-// finds it in L1 or L2)
+// row quantisation: TPR threads per row.  VPL > 0: rows of 16-byte aligned
+// pieces, VPL pieces of 8 values per thread held in registers between the
+// maximum and the rounding; VPL = 0: any row, read twice (the second time from
+// L1 or L2).
+//
+// Rounding to even by one fp32 addition: 1.5 * 2^23 + v has v's nearest whole
+// number, as two's complement, in its low bits for |v| < 2^22.
 
 constexpr float kTinyRow = 7.8886090522101181e-31f;  // 2^-100: below it 127 / max could overflow
 
-template <typename T, int TPR>
+__device__ __forceinline__ uint32_t round_to_int(float v, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.0f));
+}
+
+template <typename T, int TPR, int VPL>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int cols, const T* x, int64_t ld, int8_t* q,
-                                                            int64_t ld_q, float* scale, int vec) {
+                                                            int64_t ld_q, float* scale) {
   const int t = threadIdx.x % TPR;
-  const int64_t per_block = 256 / TPR;
+  constexpr int64_t per_block = 256 / TPR;
+  constexpr int kHeld = VPL > 0 ? VPL : 1;
   __shared__ uint32_t warp_max[8];
   for (int64_t base = blockIdx.x * per_block; base < rows; base += gridDim.x * per_block) {
     const int64_t r = base + threadIdx.x / TPR;
     const bool live = r < rows;
     const T* row = x + r * ld;
+    __align__(16) T held[kHeld][8];
     // magnitudes compare like their bits, with infinity and NaN above every finite value
     uint32_t top = 0;
     auto see = [&](float v) { top = max(top, __float_as_uint(v) & 0x7FFFFFFFu); };
     if (live) {
-      if (vec) {
-        for (int c = 8 * t; c < cols; c += 8 * TPR) {
-          T v[8];
-          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + c);
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(row + c + 4);
+      if constexpr (VPL > 0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) see(to_float(v[j]));
+        for (int i = 0; i < VPL; ++i) {
+          const int c = 8 * (t + i * TPR);
+#pragma unroll
+          for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+            reinterpret_cast<uint4*>(held[i])[k] =
+                c < cols ? reinterpret_cast<const uint4*>(row + c)[k] : make_uint4(0, 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) see(to_float(held[i][j]));
       } else {
         for (int c = t; c < cols; c += TPR) see(to_float(row[c]));
       }
@@ -1163,28 +1193,28 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
     if (!live) continue;
     const float most = __uint_as_float(top);
     float s = __fdiv_rn(most, 127.0f), inv = __fdiv_rn(127.0f, most);
-    bool zero = false;
-    if (most < kTinyRow) s = 0.0f, zero = true;
-    if (top >= 0x7F800000u) s = __uint_as_float(0x7FFFFFFFu), zero = true;
+    uint32_t mask = 0xFFFFFFFFu;
+    if (most < kTinyRow) s = 0.0f, mask = 0;
+    if (top >= 0x7F800000u) s = __uint_as_float(0x7FFFFFFFu), mask = 0;
     if (t == 0) scale[r] = s;
-    auto quant = [&](float v) -> int {
-      return zero ? 0 : (int)(int8_t)__float2int_rn(__fmul_rn(v, inv));
-    };
     int8_t* out = q + r * ld_q;
-    if (vec) {
-      for (int c = 8 * t; c < ld_q; c += 8 * TPR) {
-        uint32_t w[2] = {0, 0};
-        if (c < cols) {
-          T v[8];
-          *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + c);
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(row + c + 4);
+    if constexpr (VPL > 0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[j / 4] |= (uint32_t)(quant(to_float(v[j])) & 0xFF) << (8 * (j % 4));
-        }
-        *reinterpret_cast<uint2*>(out + c) = make_uint2(w[0], w[1]);
+      for (int i = 0; i < VPL; ++i) {
+        const int c = 8 * (t + i * TPR);
+        uint32_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = round_to_int(to_float(held[i][j]), inv);
+        auto join = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
+          return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
+        };
+        if (c < cols)
+          *reinterpret_cast<uint2*>(out + c) = make_uint2(join(b[0], b[1], b[2], b[3]) & mask, join(b[4], b[5], b[6], b[7]) & mask);
       }
+      for (int64_t c = cols + t; c < ld_q; c += TPR) out[c] = 0;
     } else {
-      for (int c = t; c < ld_q; c += TPR) out[c] = c < cols ? (int8_t)quant(to_float(row[c])) : (int8_t)0;
+      for (int64_t c = t; c < ld_q; c += TPR)
+        out[c] = c < cols ? (int8_t)(round_to_int(to_float(row[c]), inv) & mask) : (int8_t)0;
     }
   }
 }
@@ -1720,27 +1750,46 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
 
 // ---- dropout and the 8-bit product
 
+template <typename T, bool RES, typename I>
+void launch_dropout(const DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
+  const int grid = grid_for(ceil_div(p.rows * p.groups, 2), 256, sms);
+  if (vec) dropout_kernel<T, true, false, RES, I><<<grid, 256, 0, st>>>(p);
+  else if (by_rows) dropout_kernel<T, false, true, RES, I><<<grid, 256, 0, st>>>(p);
+  else dropout_kernel<T, false, false, RES, I><<<grid, 256, 0, st>>>(p);
+}
 template <typename T>
 void launch_dropout(DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
   p.groups = ceil_div(p.cols, vec ? 16 / (int64_t)sizeof(T) : 4);
-  const int grid = grid_for(p.rows * p.groups, 256, sms);
-  if (vec) dropout_kernel<T, true, false><<<grid, 256, 0, st>>>(p);
-  else if (by_rows) dropout_kernel<T, false, true><<<grid, 256, 0, st>>>(p);
-  else dropout_kernel<T, false, false><<<grid, 256, 0, st>>>(p);
+  // positions pass their end by up to two strides of the grid
+  const bool narrow = p.rows * p.groups < (int64_t(1) << 31);
+  if (p.res) {
+    if (narrow) launch_dropout<T, true, uint32_t>(p, vec, by_rows, sms, st);
+    else launch_dropout<T, true, uint64_t>(p, vec, by_rows, sms, st);
+  } else {
+    if (narrow) launch_dropout<T, false, uint32_t>(p, vec, by_rows, sms, st);
+    else launch_dropout<T, false, uint64_t>(p, vec, by_rows, sms, st);
+  }
 }
 
+template <typename T, int TPR, int VPL>
+void launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
+                     cudaStream_t st) {
+  quantize_rows_kernel<T, TPR, VPL><<<grid_for(rows, 256 / TPR, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x),
+                                                                                  ld_x, q, ld_q, scale);
+}
 template <typename T>
 void launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
                      cudaStream_t st) {
-  const int vec = aligned_rows(x, rows, ld_x, sizeof(T)) && cols % 8 == 0 && ld_q % 8 == 0 &&
-                  (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  // a warp for a row of up to 2048 values, a CTA for a longer one
-  if (cols <= 2048)
-    quantize_rows_kernel<T, 32><<<grid_for(rows, 8, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x), ld_x, q,
-                                                                        ld_q, scale, vec);
-  else
-    quantize_rows_kernel<T, 256><<<grid_for(rows, 1, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x), ld_x, q,
-                                                                         ld_q, scale, vec);
+  const bool vec = aligned_rows(x, rows, ld_x, sizeof(T)) && cols % 8 == 0 && ld_q % 8 == 0 &&
+                   (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+  // a warp for a row of up to 2048 values, a CTA for a longer one; aligned rows
+  // of up to 16384 stay in registers
+  if (vec && cols <= 512) launch_quantize<T, 32, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (vec && cols <= 1280) launch_quantize<T, 32, 5>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (vec && cols <= 4096) launch_quantize<T, 256, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (vec && cols <= 16384) launch_quantize<T, 256, 8>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else if (cols <= 2048) launch_quantize<T, 32, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  else launch_quantize<T, 256, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
 }
 
 bool known_dtype(int d) { return d == GF_F32 || d == GF_BF16 || d == GF_F16; }
