@@ -43,7 +43,6 @@ class GfGatedFf(ctypes.Structure):
         ("b_in", ctypes.c_void_p),
         ("w_out", ctypes.c_void_p), ("ld_w_out", ctypes.c_int64),
         ("b_out", ctypes.c_void_p),
-        ("u", ctypes.c_void_p),
         ("h", ctypes.c_void_p),
         ("y", ctypes.c_void_p), ("ld_y", ctypes.c_int64),
         ("dy", ctypes.c_void_p), ("ld_dy", ctypes.c_int64),

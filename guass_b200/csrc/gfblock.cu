@@ -194,33 +194,35 @@ constexpr int kVectorBytes = 32 * 4;    // a warp's vector of 32 floats (bias, s
 constexpr uint32_t kTmemCols = 512;
 constexpr int kSmemLimit = 232448;
 
+#ifndef GFB_W1
+#define GFB_W1 8
+#endif
+#ifndef GFB_W2
+#define GFB_W2 8
+#endif
 enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
 
-// Warps and shared memory of a variant.  A chunk's result leaves as one to
-// three staging blocks through TMA stores, which have the next chunk's
-// arithmetic to be read in; the backward's saved rows arrive in two more by
-// TMA loads a chunk ahead (with 227 KB of shared memory in use the L1 cache
-// has too few lines left for that many loads in flight).  What is left holds
-// operand stages.  Eight epilogue warps were as fast as 12 or 16 for the 16-bit
-// products, whose long tiles are bound by the memory they write; the integer
-// results take a conversion each and gain from 12 (16384 x 1280 x 10240: 160 us
-// against 171).
+// Warps and shared memory of a variant.  A chunk's result leaves as staging
+// blocks through TMA stores, which have the next chunk's arithmetic to be read
+// in; what is left holds operand stages.  Eight epilogue warps were as fast as
+// 12 or 16 for the 16-bit products, whose long tiles are bound by the memory
+// they write; the integer results take a conversion each and gain from 12
+// (16384 x 1280 x 10240: 160 us against 171).
 template <int EPI>
 struct Config {
-  static constexpr int epi_warps = EPI == EPI_INT8 ? 12 : 8;
+  static constexpr int epi_warps = EPI == EPI_INT8 ? 12 : EPI == EPI_GATED_BWD ? GFB_W2 : EPI == EPI_GATED ? GFB_W1 : 8;
   static constexpr int threads = 64 + 32 * epi_warps;
-  static constexpr int out = EPI == EPI_GATED ? 3 : 2;
-  static constexpr int blocks = out + (EPI == EPI_GATED_BWD ? 2 : 0);
-  static constexpr int vectors = EPI == EPI_GATED_BWD ? 0 : EPI == EPI_STORE ? 1 : 2;
+  static constexpr int blocks = EPI == EPI_GATED ? 1 : 2;
+  static constexpr int vectors = EPI == EPI_STORE ? 1 : 2;
   static constexpr int side_bytes = epi_warps * (blocks * kRowsBytes + vectors * kVectorBytes) + 512;
   static constexpr int stage_room = (kSmemLimit - side_bytes) / 1024 * 1024;
 };
-constexpr int kMaxEpiWarps = 12;
 constexpr int kMaxStages = 8;
 
 struct alignas(64) GemmParams {
   CUtensorMap ma, mb;
-  CUtensorMap mo, mu;            // tiles of 64 bytes x 32 rows: result (or partial products), and u
+  CUtensorMap ma2, mb2;          // GATED_BWD: operands of dh, dy (m, k) and w_out (k, n)
+  CUtensorMap mo;                // tiles of 64 bytes x 32 rows of the result (or of the partial products)
   int32_t M, N;                // rows and columns of the result (gated: columns of h, without padding)
   int32_t tiles_m, tiles_n, splits, kb_total, kb_split;
   int32_t rows_m;              // rows of all tiles of M
@@ -229,6 +231,8 @@ struct alignas(64) GemmParams {
   int32_t a_mn, b_mn;          // operand is M/N-contiguous
   int32_t gate_row;            // gated: row of B where the gate half starts
   uint32_t idesc, tx_bytes;
+  uint32_t idesc2, tx_bytes2;  // GATED_BWD: of dh
+  int32_t kb2;                 // and its k steps
   int32_t stages, stage_bytes;
   int32_t seg_pad, seg;        // result rows come in two runs of `seg` rows, the second starting at seg_pad (0: one run)
   int32_t tma_out;             // the result is written through mo (its rows are 16-byte aligned, in one run)
@@ -236,8 +240,7 @@ struct alignas(64) GemmParams {
   void* out;                   // STORE, INT8: result
   float* partial;              // splits > 1: [splits][tiles_m * 128][ld_partial]
   int64_t ld_partial;
-  const void* bias;            // [N] (gated: [2 N])
-  void* u;                     // GATED: written through mu when not null
+  const void* bias;            // [N] (gated, forward and backward: [2 N])
   int32_t hp;                  // gated: padded hidden size
   const float* a_scale;
   const float* b_scale;
@@ -245,7 +248,7 @@ struct alignas(64) GemmParams {
 };
 
 struct Pipe {  // barriers and the abort flag, in shared memory
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], spare, rows[kMaxEpiWarps];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], spare;
   uint32_t tmem, abort;
 };
 static_assert(sizeof(Pipe) <= 512, "the room behind the staging blocks");
@@ -309,45 +312,30 @@ struct EpilogueWarp {
   const int lane;
   Philox rng;
   float row_scale = 0.0f;
-  const uint32_t rows_bar;      // GATED_BWD: this warp's barrier of the saved rows
-  volatile uint32_t* abort;
-  uint32_t phase = 0;
-  bool rows_due = false;        // they are on their way
 
-  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors, uint32_t bar,
-                                          volatile uint32_t* abort_)
+  __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors)
       : p(p_), stage(stage_), vec0(reinterpret_cast<float*>(vectors)), vec1(vec0 + 32), lane(threadIdx.x & 31),
-        rng(p_.drop), rows_bar(bar), abort(abort_) {}
+        rng(p_.drop) {}
 
   // Bias and scale of this lane's column of a chunk, fetched ahead.
   struct Ahead {
     float a, b;
   };
-  __device__ __forceinline__ void fetch(Ahead& x, int m, int n) {
-    if constexpr (EPI == EPI_GATED_BWD) {
-      __syncwarp();  // every lane has read the rows before
-      if (lane == 0) {
-        tc::mbar_expect_tx(rows_bar, 2 * kRowsBytes);
-        tc::tma_load(block(C::out), &p.mu, rows_bar, n, m);
-        tc::tma_load(block(C::out + 1), &p.mu, rows_bar, p.hp + n, m);
-      }
-      rows_due = true;
-    } else {
-      x.a = x.b = 0.0f;
-      if (lane < p.N - n) {
-        const T* bias = static_cast<const T*>(p.bias);
-        if (bias) x.a = to_float(bias[n + lane]);
-        if (EPI == EPI_GATED && bias) x.b = to_float(bias[p.N + n + lane]);
-        if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
-      }
+  __device__ __forceinline__ void fetch(Ahead& x, int n) const {
+    x.a = x.b = 0.0f;
+    if (lane < p.N - n) {
+      const T* bias = static_cast<const T*>(p.bias);
+      if (bias) x.a = to_float(bias[n + lane]);
+      if ((EPI == EPI_GATED || EPI == EPI_GATED_BWD) && bias) x.b = to_float(bias[p.N + n + lane]);
+      if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
     }
   }
 
   // One 32-column chunk at result column n of rows m .. m + 31, from the
-  // accumulator columns at `acc`.  `release` runs once they are read, and
+  // accumulator columns at `acc` (dh: at `acc2`).  `release` runs once they are read, and
   // `fetch_next` once `ahead` is.
   template <typename Release, typename Next>
-  __device__ __forceinline__ void chunk(uint32_t acc, const Tile& t, int m, int n, const Ahead& ahead, Release release,
+  __device__ __forceinline__ void chunk(uint32_t acc, uint32_t acc2, const Tile& t, int m, int n, const Ahead& ahead, Release release,
                                         Next fetch_next) {
     uint32_t d[32];
     if constexpr (EPI == EPI_STORE || EPI == EPI_INT8) tc::tmem_load32(d, acc);
@@ -404,46 +392,15 @@ struct EpilogueWarp {
         put(0, v);
         result<2>(1, m, n);
       }
-    } else if constexpr (EPI == EPI_GATED) {
+    } else {
       vectors(ahead);
       fetch_next();
-      if (p.u) gated<true>(acc, m, n, release);
-      else gated<false>(acc, m, n, release);
-    } else {
-      uint32_t v[16], w[16];
-      read_rows(v, w);
-      fetch_next();
-      // du_value = dh * u_value, du_gate = dh * u_gate (see gated)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        tc::tmem_load16(d, acc + 16 * half);
-        tc::tmem_wait();
-        if (half == 1) release();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int o = 8 * half + i;
-          const float2 a = unpack2<T>(v[o]), g = unpack2<T>(w[o]);
-          v[o] = pack2<T>(f(d[2 * i]) * a.x, f(d[2 * i + 1]) * a.y);
-          w[o] = pack2<T>(f(d[2 * i]) * g.x, f(d[2 * i + 1]) * g.y);
-        }
-      }
-      begin();
-      put(0, v);
-      put(1, w);
-      send([&] {
-        tc::tma_store(&p.mo, block(0), n, m);
-        tc::tma_store(&p.mo, block(1), p.hp + n, m);
-      });
+      gated(acc, acc2, m, n, release);
     }
   }
 
-  // Every block must be out of shared memory, and no copy on its way into it,
-  // before the CTA ends.
+  // Every block must be out of shared memory before the CTA ends.
   __device__ __forceinline__ void finish() {
-    if (rows_due) {  // after a wait that gave up only
-      volatile uint32_t ignore = 0;
-      tc::mbar_wait(rows_bar, phase, &ignore);
-    }
     if (lane == 0) tc::tma_store_drain();
     __syncwarp();
   }
@@ -458,19 +415,23 @@ struct EpilogueWarp {
     __syncwarp();
   }
 
-  // h = keep * value * act(gate); saved for the backward (SAVE): what the
-  // gradient of h is multiplied with, keep * act(gate) and keep * value *
-  // act'(gate).  keep is 1 / (1 - p) or 0, so that the backward needs neither
-  // the activation nor the mask again, for the bytes that value and gate
-  // themselves would take.
-  template <bool SAVE, typename Release>
-  __device__ __forceinline__ void gated(uint32_t acc, int m, int n, Release release) {
+  // The forward's chunk, h = keep * value * act(gate), or the backward's,
+  // du_value = keep * dh * act(gate) and du_gate = keep * dh * value *
+  // act'(gate), from the same value and gate in fp32: the backward computes
+  // them again instead of reading them.  That is 4 * tokens * hidden *
+  // in_features more operations against 8 bytes written and read for every
+  // element of h, half the activation memory of the block, and one rounding
+  // less in every gradient.  keep is 1 / (1 - p) or 0, 1 without dropout.
+  template <typename Release>
+  __device__ __forceinline__ void gated(uint32_t acc, uint32_t acc2, int m, int n, Release release) {
+    constexpr bool kBack = EPI == EPI_GATED_BWD;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t a[16], g[16], h[8], sv[8], sg[8];
-      const int left = p.N - n - 16 * half;  // the padding columns of h and u are zeros
+      uint32_t a[16], g[16], dh[16], o0[8], o1[8];
+      const int left = p.N - n - 16 * half;  // the padding columns of h and du are zeros
       tc::tmem_load16(a, acc + 16 * half);
       tc::tmem_load16(g, acc + p.cols + 16 * half);
+      if constexpr (kBack) tc::tmem_load16(dh, acc2 + 16 * half);
       tc::tmem_wait();
       if (half == 1) release();
 #pragma unroll
@@ -488,21 +449,23 @@ struct EpilogueWarp {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int c = 4 * q + 2 * i, o = 2 * q + i;
-          uint64_t x = tc::add_f2(tc::pack_f2(f(a[c]), f(a[c + 1])), i ? tc::pack_f2(b0.z, b0.w) : tc::pack_f2(b0.x, b0.y));
-          float2 y = tc::unpack_f2(
+          const uint64_t x = tc::add_f2(tc::pack_f2(f(a[c]), f(a[c + 1])), i ? tc::pack_f2(b0.z, b0.w) : tc::pack_f2(b0.x, b0.y));
+          const float2 y = tc::unpack_f2(
               tc::add_f2(tc::pack_f2(f(g[c]), f(g[c + 1])), i ? tc::pack_f2(b1.z, b1.w) : tc::pack_f2(b1.x, b1.y)));
           uint64_t value, slope = 0;
-          activate<ACT, SAVE>(y.x, y.y, value, slope);
-          if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
-          float2 r = tc::unpack_f2(tc::mul_f2(x, value));
-          h[o] = pack2<T>(r.x, r.y);
-          if constexpr (SAVE) {
-            slope = tc::mul_f2(x, slope);
-            if constexpr (DROP) slope = tc::mul_f2(slope, keep[i]);
-            r = tc::unpack_f2(value);
-            sv[o] = pack2<T>(r.x, r.y);
-            r = tc::unpack_f2(slope);
-            sg[o] = pack2<T>(r.x, r.y);
+          activate<ACT, kBack>(y.x, y.y, value, slope);
+          float2 r;
+          if constexpr (kBack) {
+            uint64_t d = tc::pack_f2(f(dh[c]), f(dh[c + 1]));
+            if constexpr (DROP) d = tc::mul_f2(d, keep[i]);
+            r = tc::unpack_f2(tc::mul_f2(d, value));
+            o0[o] = pack2<T>(r.x, r.y);
+            r = tc::unpack_f2(tc::mul_f2(tc::mul_f2(d, x), slope));
+            o1[o] = pack2<T>(r.x, r.y);
+          } else {
+            if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
+            r = tc::unpack_f2(tc::mul_f2(x, value));
+            o0[o] = pack2<T>(r.x, r.y);
           }
         }
       }
@@ -510,23 +473,17 @@ struct EpilogueWarp {
 #pragma unroll
         for (int o = 0; o < 8; ++o) {
           const uint32_t mask = 2 * o + 1 < left ? 0xFFFFFFFFu : 2 * o < left ? 0xFFFFu : 0u;
-          h[o] &= mask;
-          if constexpr (SAVE) sv[o] &= mask, sg[o] &= mask;
+          o0[o] &= mask;
+          if constexpr (kBack) o1[o] &= mask;
         }
       }
       if (half == 0) begin();
-      put_half(0, half, h);
-      if constexpr (SAVE) {
-        put_half(1, half, sv);
-        put_half(2, half, sg);
-      }
+      put_half(0, half, o0);
+      if constexpr (kBack) put_half(1, half, o1);
     }
     send([&] {
       tc::tma_store(&p.mo, block(0), n, m);
-      if constexpr (SAVE) {
-        tc::tma_store(&p.mu, block(1), n, m);
-        tc::tma_store(&p.mu, block(2), p.hp + n, m);
-      }
+      if constexpr (kBack) tc::tma_store(&p.mo, block(1), p.hp + n, m);
     });
   }
 
@@ -559,21 +516,6 @@ struct EpilogueWarp {
     if (lane == 0) {
       stores();
       tc::tma_store_commit();
-    }
-  }
-
-  // This lane's row of the two blocks of saved rows (GATED_BWD).
-  __device__ __forceinline__ void read_rows(uint32_t (&v)[16], uint32_t (&w)[16]) {
-    tc::mbar_wait(rows_bar, phase, abort);
-    __syncwarp();
-    phase ^= 1;
-    rows_due = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const char* at = stage + C::out * kRowsBytes + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
-      const uint4 x = *reinterpret_cast<const uint4*>(at), y = *reinterpret_cast<const uint4*>(at + kRowsBytes);
-      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
-      w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
     }
   }
 
@@ -636,6 +578,10 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
   if (threadIdx.x == 0) {
     tc::tma_prefetch(&p.ma);
     tc::tma_prefetch(&p.mb);
+    if constexpr (EPI == EPI_GATED_BWD) {
+      tc::tma_prefetch(&p.ma2);
+      tc::tma_prefetch(&p.mb2);
+    }
     for (int i = 0; i < p.stages; ++i) {
       tc::mbar_init(full + 8 * i, 1);
       tc::mbar_init(empty + 8 * i, 1);
@@ -644,7 +590,6 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       tc::mbar_init(acc_full + 8 * i, 1);
       tc::mbar_init(acc_empty + 8 * i, C::epi_warps * (PAIR ? 2 : 1));
     }
-    for (int i = 0; i < C::epi_warps; ++i) tc::mbar_init(tc::smem_addr(&pipe->rows[i]), 1);
     pipe->abort = 0;
     tc::fence_barrier_init();
     tc::fence_proxy_async();
@@ -668,31 +613,44 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
         if constexpr (PAIR) tc::tma_load_pair(dst, map, bar, x, y);
         else tc::tma_load(dst, map, bar, x, y);
       };
+      // one stage: fill(its A, its B, the barrier) once the stage is free
+      auto stage = [&](uint32_t bytes, auto fill) {
+        ok = tc::mbar_wait(empty + 8 * s, phase ^ 1, abort);
+        if (!ok) return;
+        const uint32_t a = base + s * p.stage_bytes;
+        if (rank == 0) tc::mbar_expect_tx(full + 8 * s, bytes);
+        fill(a, a + kABytes, full0 + 8 * s);
+        ++n;
+        if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+      };
       for (Tile t = first_tile<PAIR>(p, rank); ok && t.left > 0; next_tile<PAIR>(p, t, rank)) {
-        const int n0 = t.n0 + (PAIR ? (int)rank * b_cols : 0);
-        for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          ok = tc::mbar_wait(empty + 8 * s, phase ^ 1, abort);
-          if (!ok) break;
-          const uint32_t bar = full0 + 8 * s, a = base + s * p.stage_bytes, b = a + kABytes;
-          if (rank == 0) tc::mbar_expect_tx(full + 8 * s, p.tx_bytes);
-          const int k0 = kb * (EPI == EPI_INT8 ? 128 : 64);
-          if (p.a_mn) {
-            load(a, &p.ma, bar, t.m0, k0);
-            load(a + tc::kMnGroupBytes, &p.ma, bar, t.m0 + 64, k0);
-          } else {
-            load(a, &p.ma, bar, k0, t.m0);
-          }
-          if (EPI == EPI_GATED) {  // value rows, then gate rows: one half of B each
-            if (!PAIR || rank == 0) load(b, &p.mb, bar, k0, t.n0);
-            if (!PAIR || rank == 1) load(b + (PAIR ? 0 : p.cols * 128), &p.mb, bar, k0, p.gate_row + t.n0);
-          } else if (p.b_mn) {
-            for (int i = 0; i < b_cols; i += 64) load(b + 128 * i, &p.mb, bar, n0 + i, k0);
-          } else {
-            load(b, &p.mb, bar, k0, n0);
-          }
-          ++n;
-          if (++s == p.stages) s = 0, phase ^= 1;
+        if constexpr (EPI == EPI_GATED_BWD) {
+          const int half = PAIR ? p.cols / 2 : p.cols, n2 = t.n0 + (PAIR ? (int)rank * half : 0);
+          for (int kb = 0; ok && kb < p.kb2; ++kb)
+            stage(p.tx_bytes2, [&](uint32_t a, uint32_t b, uint32_t bar) {
+              load(a, &p.ma2, bar, 64 * kb, t.m0);
+              for (int i = 0; i < half; i += 64) load(b + 128 * i, &p.mb2, bar, n2 + i, 64 * kb);
+            });
         }
+        const int n0 = t.n0 + (PAIR ? (int)rank * b_cols : 0);
+        for (int kb = t.kb0; ok && kb < t.kb1; ++kb)
+          stage(p.tx_bytes, [&](uint32_t a, uint32_t b, uint32_t bar) {
+            const int k0 = kb * (EPI == EPI_INT8 ? 128 : 64);
+            if (p.a_mn) {
+              load(a, &p.ma, bar, t.m0, k0);
+              load(a + tc::kMnGroupBytes, &p.ma, bar, t.m0 + 64, k0);
+            } else {
+              load(a, &p.ma, bar, k0, t.m0);
+            }
+            if (EPI == EPI_GATED || EPI == EPI_GATED_BWD) {  // value rows, then gate rows: one half of B each
+              if (!PAIR || rank == 0) load(b, &p.mb, bar, k0, t.n0);
+              if (!PAIR || rank == 1) load(b + (PAIR ? 0 : p.cols * 128), &p.mb, bar, k0, p.gate_row + t.n0);
+            } else if (p.b_mn) {
+              for (int i = 0; i < b_cols; i += 64) load(b + 128 * i, &p.mb, bar, n0 + i, k0);
+            } else {
+              load(b, &p.mb, bar, k0, n0);
+            }
+          });
       }
       // The copies in flight must land before the CTA ends.  Every product
       // waits for its copies, so this matters after a wait that gave up only.
@@ -706,25 +664,38 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
     if (rank == 0 && tc::elect_one()) {
       uint32_t s = 0, phase = 0, it = 0;
       bool ok = true;
-      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+      // one k step of products into the accumulator at d
+      auto step = [&](uint32_t d, bool a_mn, bool b_mn, uint32_t idesc, bool fresh) {
+        ok = tc::mbar_wait(full + 8 * s, phase, abort);
+        if (!ok) return;
+        tc::fence_after();
+        const uint32_t a = base + s * p.stage_bytes;
+        const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint64_t da = tc::operand_desc(a, a_mn), db = tc::operand_desc(a + kABytes, b_mn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          tc::mma<PAIR, EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, idesc, !fresh || i > 0);
+        tc::mma_commit<PAIR>(empty + 8 * s);
+        if (++s == (uint32_t)p.stages) s = 0, phase ^= 1;
+      };
       for (Tile t = first_tile<PAIR>(p, rank); ok && t.left > 0; next_tile<PAIR>(p, t, rank), ++it) {
         const uint32_t buf = it & 1;
         ok = tc::mbar_wait(acc_empty + 8 * buf, ((it >> 1) & 1) ^ 1, abort);
         if (!ok) break;
         tc::fence_after();
-        const uint32_t d = tmem + buf * kMaxN;
-        for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          ok = tc::mbar_wait(full + 8 * s, phase, abort);
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t a = base + s * p.stage_bytes;
-          const uint64_t da = tc::operand_desc(a, p.a_mn), db = tc::operand_desc(a + kABytes, p.b_mn);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            tc::mma<PAIR, EPI == EPI_INT8>(d, da + i * a_step, db + i * b_step, p.idesc, kb > t.kb0 || i > 0);
-          tc::mma_commit<PAIR>(empty + 8 * s);
-          if (++s == p.stages) s = 0, phase ^= 1;
+        uint32_t d = tmem + buf * kMaxN;
+        if constexpr (EPI == EPI_GATED_BWD) {
+          // dh in one of two buffers; value and gate, which need the rest of
+          // TMEM, once the epilogue of the tile before is through
+          for (int kb = 0; ok && kb < p.kb2; ++kb)
+            step(tmem + kMaxN + buf * (kMaxN / 2), false, true, p.idesc2, kb == 0);
+          if (ok && it > 0) {
+            ok = tc::mbar_wait(acc_empty + 8 * (buf ^ 1), ((it - 1) >> 1) & 1, abort);
+            tc::fence_after();
+          }
+          d = tmem;
         }
+        for (int kb = t.kb0; ok && kb < t.kb1; ++kb) step(d, p.a_mn, p.b_mn, p.idesc, kb == t.kb0);
         if (!ok) break;
         tc::mma_commit<PAIR>(acc_full + 8 * buf);
       }
@@ -733,8 +704,7 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
     constexpr int kSets = C::epi_warps / 4;  // warps of a quarter
     const int quarter = warp & 3, set = (warp - 2) >> 2;
     EpilogueWarp<EPI, T, ACT, DROP> epi(p, staging + (warp - 2) * C::blocks * kRowsBytes,
-                                        vectors + (warp - 2) * C::vectors * kVectorBytes,
-                                        tc::smem_addr(&pipe->rows[warp - 2]), abort);
+                                        vectors + (warp - 2) * C::vectors * kVectorBytes);
     const uint32_t empty0 = PAIR ? tc::peer_addr(acc_empty, 0) : acc_empty;
     // gated: the padding columns of h, u and du are written too (zeros)
     const int n_end = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? p.hp : p.N;
@@ -743,11 +713,12 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       const uint32_t buf = it & 1;
       const int m = t.m0 + 32 * quarter;
       const int c_end = m < p.M ? min(p.cols, n_end - t.n0) : 0;
-      const uint32_t acc = tmem + ((uint32_t)(32 * quarter) << 16) + buf * kMaxN;
+      const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
+      const uint32_t acc = lanes + (EPI == EPI_GATED_BWD ? 0 : buf * kMaxN), acc2 = lanes + kMaxN + buf * (kMaxN / 2);
       int c = 32 * set;
       if (EPI == EPI_INT8) epi.row_scale = m + (int)(threadIdx.x & 31) < p.M ? p.a_scale[m + (threadIdx.x & 31)] : 0.0f;
       typename decltype(epi)::Ahead ahead;
-      if (c < c_end) epi.fetch(ahead, m, t.n0 + c);
+      if (c < c_end) epi.fetch(ahead, t.n0 + c);
       if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
       tc::fence_after();
       auto release = [&](bool last) {
@@ -762,8 +733,8 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       if (c >= c_end) release(true);  // no chunk of this tile is this warp's
       for (; c < c_end; c += 32 * kSets) {
         const int next = c + 32 * kSets;
-        epi.chunk(acc + c, t, m, t.n0 + c, ahead, [&] { release(next >= c_end); },
-                  [&] { if (next < c_end) epi.fetch(ahead, m, t.n0 + next); });
+        epi.chunk(acc + c, acc2 + c, t, m, t.n0 + c, ahead, [&] { release(next >= c_end); },
+                  [&] { if (next < c_end) epi.fetch(ahead, t.n0 + next); });
       }
     }
     epi.finish();
@@ -917,7 +888,7 @@ struct SkinnyParams {
   const void *x, *w, *bias;  // x [tokens, k], w [n or two runs of n, k]
   int64_t ld_x, ld_w, gate_row;
   int32_t tokens, n, k, hp;
-  void *out, *u;
+  void* out;
   int64_t ld_out;
   int32_t act;
   DropArgs drop;
@@ -1002,7 +973,7 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
       for (int d = 16; d > 0; d >>= 1) sum[r][m] += __shfl_xor_sync(0xFFFFFFFFu, sum[r][m], d);
   const T* bias = static_cast<const T*>(p.bias);
   if constexpr (GATED) {
-    // lane m finishes token m; the padding columns of h and u are zeros
+    // lane m finishes token m; the padding columns of h are zeros
     float a = 0.0f, g = 0.0f;
 #pragma unroll
     for (int m = 0; m < TOKENS; ++m)
@@ -1010,29 +981,18 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
     if (live && lane < p.tokens) {
       if (bias) a += to_float(bias[n]), g += to_float(bias[p.n + n]);
       uint64_t value, slope;
-      if (p.act == GF_ACT_GELU) activate<GF_ACT_GELU, true>(g, g, value, slope);
-      else activate<GF_ACT_SILU, true>(g, g, value, slope);
-      float v = tc::unpack_f2(value).x, s = tc::unpack_f2(slope).x * a;
+      if (p.act == GF_ACT_GELU) activate<GF_ACT_GELU, false>(g, g, value, slope);
+      else activate<GF_ACT_SILU, false>(g, g, value, slope);
+      float v = tc::unpack_f2(value).x;
       if (p.drop.on) {
         const uint4 w = Philox(p.drop)((uint32_t)n >> 2, (uint32_t)lane);
         const uint32_t word = (n & 3) == 0 ? w.x : (n & 3) == 1 ? w.y : (n & 3) == 2 ? w.z : w.w;
         const float keep = word >= p.drop.threshold ? p.drop.scale : 0.0f;
         v = keep * v;
-        s = keep * s;
       }
-      T* out = static_cast<T*>(p.out) + lane * p.ld_out + n;
-      *out = from_float<T>(a * v);
-      if (p.u) {
-        T* u = static_cast<T*>(p.u) + lane * 2 * (int64_t)p.hp + n;
-        u[0] = from_float<T>(v);
-        u[p.hp] = from_float<T>(s);
-      }
+      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(a * v);
     } else if (!live && n < p.hp && lane < p.tokens) {
       static_cast<T*>(p.out)[lane * p.ld_out + n] = T(0.0f);
-      if (p.u) {
-        T* u = static_cast<T*>(p.u) + lane * 2 * (int64_t)p.hp + n;
-        u[0] = u[p.hp] = T(0.0f);
-      }
     }
   } else {
     float y = 0.0f;
@@ -1305,27 +1265,31 @@ struct Shape {
   int bn, splits, kb_split, tiles_m, tiles_n;
   int rows_m() const { return tiles_m * kTileM * (pair ? 2 : 1); }
 };
-Shape search_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
+Shape search_shape(int64_t M, int64_t N, int64_t kb, int64_t kb2, int epi, bool may_split, int sms) {
   Shape best{};
   double best_cost = 0;
-  const bool gated = epi == EPI_GATED;
-  const int step = gated ? 64 : 32;
-  const double per_col = epi == EPI_GATED ? 72.0 : epi == EPI_GATED_BWD ? 80.0 : 24.0;
+  const bool gated = epi == EPI_GATED || epi == EPI_GATED_BWD;
+  // bytes a result element takes, over 11 bytes a clock, for 128 rows
+  const double per_col = epi == EPI_GATED_BWD ? 48.0 : 24.0;
   for (int pair = 0; pair < 2; ++pair) {
     const int64_t tm = ceil_div(M, pair ? 2 * kTileM : kTileM), units = pair ? sms / 2 : sms;
-    // a single CTA's gated variants have room for enough stages of at most 128 columns
-    const bool narrow = !pair && (gated || epi == EPI_GATED_BWD);
-    for (int bn = step; bn <= (narrow ? kMaxN / 2 : kMaxN); bn += step) {
+    const int step = gated ? 64 : 32;
+    for (int bn = step; bn <= kMaxN; bn += step) {
       const int cols = gated ? bn / 2 : bn;
       if (cols > 32 && cols - 32 >= N) break;  // wider than the result
       const int64_t tn = ceil_div(N, cols);
-      const double loads = (kTileM + (pair ? bn / 2 : bn)) * 128 / 70.0, products = 2.0 * bn;
-      const double step_cost = loads > products ? loads : products;
+      const auto k_step = [&](int n) {  // clocks of 64 k: operands or products of n columns
+        const double loads = (kTileM + (pair ? n / 2 : n)) * 128 / 70.0, products = 2.0 * n;
+        return loads > products ? loads : products;
+      };
       for (int64_t s = 1; s <= (may_split ? kb : 1) && s <= 64; s = s < 4 ? s + 1 : s + s / 4) {
         const int64_t per = ceil_div(kb, s);
         if (ceil_div(kb, per) != s) continue;
-        const double waves = (double)ceil_div(tm * tn * s, units), epilogue = per_col * cols, main = per * step_cost;
-        double cost = waves * ((main > epilogue ? main : epilogue) + 600.0) + 1500.0 + epilogue;
+        const double waves = (double)ceil_div(tm * tn * s, units), epilogue = per_col * cols, main = per * k_step(bn);
+        // the backward's dh overlaps the epilogue before it, value and gate do not
+        const double under = epi == EPI_GATED_BWD ? kb2 * k_step(cols) : main;
+        const double tile = (under > epilogue ? under : epilogue) + (epi == EPI_GATED_BWD ? main : 0.0);
+        double cost = waves * (tile + 600.0) + 1500.0 + epilogue;
         if (s > 1) cost += 4000.0 + (double)(s + 1) * M * N * 4 / 3000.0;
         if (best.bn == 0 || cost < best_cost) {
           best_cost = cost;
@@ -1338,18 +1302,18 @@ Shape search_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, in
 }
 
 // The search takes some microseconds: a thread remembers the last shapes it asked for.
-Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms) {
+Shape choose_shape(int64_t M, int64_t N, int64_t kb, int epi, bool may_split, int sms, int64_t kb2 = 0) {
   struct Entry {
-    int64_t M, N, kb;
+    int64_t M, N, kb, kb2;
     int epi, may_split, sms;
     Shape shape;
   };
   thread_local Entry seen[64];  // zero: no size is
   const uint64_t hash = (uint64_t)M * 0x9E3779B97F4A7C15u ^ (uint64_t)N * 0xC2B2AE3D27D4EB4Fu ^ (uint64_t)kb * 0x165667B19E3779F9u ^
-                        (uint64_t)(4 * epi + may_split) * 0xD6E8FEB86659FD93u;
+                        (uint64_t)(8 * kb2 + 2 * epi + may_split) * 0xD6E8FEB86659FD93u;
   Entry& e = seen[hash >> 58];
-  if (e.M != M || e.N != N || e.kb != kb || e.epi != epi || e.may_split != may_split || e.sms != sms)
-    e = Entry{M, N, kb, epi, may_split, sms, search_shape(M, N, kb, epi, may_split, sms)};
+  if (e.M != M || e.N != N || e.kb != kb || e.kb2 != kb2 || e.epi != epi || e.may_split != may_split || e.sms != sms)
+    e = Entry{M, N, kb, kb2, epi, may_split, sms, search_shape(M, N, kb, kb2, epi, may_split, sms)};
   return e.shape;
 }
 
@@ -1361,7 +1325,7 @@ template <int EPI, typename T, int ACT, bool DROP, bool PAIR>
 gf_status launch_gemm(GemmParams p, int sms, cudaStream_t st) {
   using C = Config<EPI>;
   constexpr int smem_bytes = C::stage_room + C::side_bytes;
-  static_assert(smem_bytes <= kSmemLimit && C::stage_room >= 3 * 32768, "shared memory of one SM");
+  static_assert(smem_bytes <= kSmemLimit && C::stage_room >= 3 * 49152, "shared memory of one SM");
   const auto kernel = gemm_kernel<EPI, T, ACT, DROP, PAIR>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is set
   int dev = 0;
@@ -1467,8 +1431,8 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
     p.bytes = 256;
     return p;
   }
-  const bool use_x = !back || f.dw_in, use_w_in = !back || f.dx;
   const bool use_du = back && (f.dx || f.dw_in || f.db_in);
+  const bool use_x = !back || use_du, use_w_in = use_x;
   const bool use_w_out = !back || use_du, use_dy = back && (use_du || f.dw_out);
   p.copy_x = use_x && !aligned_rows(f.x, p.M, f.ld_x, 2);
   p.copy_w_in = use_w_in && (p.Hp != p.F || !aligned_rows(f.w_in, 2 * p.F, f.ld_w_in, 2));
@@ -1491,7 +1455,7 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
   } else {
     if (use_du) {
       p.du = b.take(2 * p.M * 2 * p.Hp);
-      p.dh = choose_shape(p.M, p.Hp, ceil_div(p.O, 64), EPI_GATED_BWD, false, sms);
+      p.dh = choose_shape(p.M, p.Hp, ceil_div(p.D, 64), EPI_GATED_BWD, false, sms, ceil_div(p.O, 64));
     }
     if (f.dx) {
       p.dx = choose_shape(p.M, p.D, 2 * p.Hp / 64, EPI_STORE, true, sms);
@@ -1633,13 +1597,13 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
   return GF_OK;
 }
 
-template <typename T>
+template <int EPI, typename T>
 gf_status gated(const GemmParams& p, const Shape& s, int act, int sms, cudaStream_t st) {
   if (act == GF_ACT_GELU)
-    return p.drop.on ? launch_gemm<EPI_GATED, T, GF_ACT_GELU, true>(p, s, sms, st)
-                     : launch_gemm<EPI_GATED, T, GF_ACT_GELU, false>(p, s, sms, st);
-  return p.drop.on ? launch_gemm<EPI_GATED, T, GF_ACT_SILU, true>(p, s, sms, st)
-                   : launch_gemm<EPI_GATED, T, GF_ACT_SILU, false>(p, s, sms, st);
+    return p.drop.on ? launch_gemm<EPI, T, GF_ACT_GELU, true>(p, s, sms, st)
+                     : launch_gemm<EPI, T, GF_ACT_GELU, false>(p, s, sms, st);
+  return p.drop.on ? launch_gemm<EPI, T, GF_ACT_SILU, true>(p, s, sms, st)
+                   : launch_gemm<EPI, T, GF_ACT_SILU, false>(p, s, sms, st);
 }
 
 template <typename T, bool GATED>
@@ -1662,7 +1626,6 @@ gf_status ff_skinny(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   p.bias = f.b_in;
   p.tokens = (int)pl.M, p.n = (int)pl.F, p.k = (int)pl.D, p.hp = (int)pl.Hp;
   p.out = f.h, p.ld_out = pl.Hp;
-  p.u = f.u;
   p.act = f.activation;
   p.drop = drop_args(f.dropout);
   GFB_TRY((skinny<T, true>(p, st)));
@@ -1688,11 +1651,9 @@ gf_status ff_forward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   p.gate_row = (int)pl.Hp;
   p.kb_total = (int)ceil_div(pl.D, 64);
   p.bias = f.b_in;
-  p.u = f.u;
   p.drop = drop_args(f.dropout);
   GFB_TRY(make_out_map(&p.mo, Operand{f.h, pl.M, pl.Hp, pl.Hp}, map_type<T>(), 2));
-  if (f.u) GFB_TRY(make_out_map(&p.mu, Operand{f.u, pl.M, 2 * pl.Hp, 2 * pl.Hp}, map_type<T>(), 2));
-  GFB_TRY(gated<T>(p, pl.in, f.activation, sms, st));
+  GFB_TRY((gated<EPI_GATED, T>(p, pl.in, f.activation, sms, st)));
   return product<T>(pl.out, Operand{f.h, pl.M, pl.Hp, pl.Hp}, false, o.w_out, false, pl.M, pl.O, pl.F, f.y, f.ld_y, f.b_out,
                     0, 0, pl.partial, sms, st);
 }
@@ -1720,14 +1681,23 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
   const Operand du{pl.du, pl.M, 2 * pl.Hp, 2 * pl.Hp};
   if (pl.du) {
     GemmParams p{};
-    GFB_TRY(set_operands(p, pl.dh, o.dy, false, o.w_out, true, 2, map_type<T>(), tc::kAccF32, mma_format<T>(), false));
+    GFB_TRY(set_operands(p, pl.dh, o.x, false, o.w_in, false, 2, map_type<T>(), tc::kAccF32, mma_format<T>(), true));
     p.M = (int)pl.M;
     p.N = (int)pl.F;
     p.hp = (int)pl.Hp;
-    p.kb_total = (int)ceil_div(pl.O, 64);
+    p.gate_row = (int)pl.Hp;
+    p.kb_total = (int)ceil_div(pl.D, 64);
+    p.bias = f.b_in;
+    p.drop = drop_args(f.dropout);
+    // dh: dy as stored, w_out with its columns along N
+    const int half = pl.dh.pair ? p.cols / 2 : p.cols;
+    p.kb2 = (int)ceil_div(pl.O, 64);
+    p.idesc2 = tc::instruction_desc(tc::kAccF32, mma_format<T>(), false, true, p.cols, pl.dh.pair);
+    p.tx_bytes2 = (kABytes + 128 * round_up(half, 64)) * (pl.dh.pair ? 2 : 1);
+    GFB_TRY(make_map(&p.ma2, o.dy, map_type<T>(), 2, 64, kTileM));
+    GFB_TRY(make_map(&p.mb2, o.w_out, map_type<T>(), 2, 64, 64));
     GFB_TRY(make_out_map(&p.mo, du, map_type<T>(), 2));
-    GFB_TRY(make_out_map(&p.mu, Operand{f.u, pl.M, 2 * pl.Hp, 2 * pl.Hp}, map_type<T>(), 2));
-    GFB_TRY((launch_gemm<EPI_GATED_BWD, T, 0, false>(p, pl.dh, sms, st)));
+    GFB_TRY((gated<EPI_GATED_BWD, T>(p, pl.dh, f.activation, sms, st)));
   }
   if (f.dx)
     GFB_TRY(product<T>(pl.dx, du, false, o.w_in, true, pl.M, pl.D, 2 * pl.Hp, f.dx, pl.D, nullptr, 0, 0, pl.partial, sms, st));
@@ -1907,8 +1877,7 @@ gf_status gf_gated_ff_forward(const gf_gated_ff* ff, void* workspace, size_t wor
   if (ff->tokens == 0) return GF_OK;
   if (!ff->x || !ff->w_in || !ff->w_out || !ff->h || !ff->y)
     return gf::fail(GF_ERR_INVALID_ARG, "%s: x, w_in, w_out, h and y must be non-null", who);
-  if ((reinterpret_cast<uintptr_t>(ff->u) | reinterpret_cast<uintptr_t>(ff->h)) & 15u)
-    return gf::fail(GF_ERR_INVALID_ARG, "%s: u and h must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(ff->h) & 15u) return gf::fail(GF_ERR_INVALID_ARG, "%s: h must be 16-byte aligned", who);
   const gfb::FfPlan pl = gfb::plan_ff(*ff, GF_PASS_FORWARD, static_cast<char*>(workspace));
   GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
   gfb::Range r("gfblock.gated_ff_forward");
@@ -1929,12 +1898,11 @@ gf_status gf_gated_ff_backward(const gf_gated_ff* ff, void* workspace, size_t wo
     if (ff->db_out) GFB_CUDA(cudaMemsetAsync(ff->db_out, 0, 2 * o, st));
     return GF_OK;
   }
-  if (!ff->dy || !ff->w_out || !ff->u) return gf::fail(GF_ERR_INVALID_ARG, "%s: dy, w_out and u must be non-null", who);
-  if (ff->dx && !ff->w_in) return gf::fail(GF_ERR_INVALID_ARG, "%s: dx needs w_in", who);
-  if (ff->dw_in && !ff->x) return gf::fail(GF_ERR_INVALID_ARG, "%s: dw_in needs x", who);
+  if (!ff->dy) return gf::fail(GF_ERR_INVALID_ARG, "%s: dy must be non-null", who);
+  if ((ff->dx || ff->dw_in || ff->db_in) && (!ff->x || !ff->w_in || !ff->w_out))
+    return gf::fail(GF_ERR_INVALID_ARG, "%s: dx, dw_in and db_in need x, w_in and w_out", who);
   if (ff->dw_out && !ff->h) return gf::fail(GF_ERR_INVALID_ARG, "%s: dw_out needs h", who);
-  if ((reinterpret_cast<uintptr_t>(ff->u) | reinterpret_cast<uintptr_t>(ff->h)) & 15u)
-    return gf::fail(GF_ERR_INVALID_ARG, "%s: u and h must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(ff->h) & 15u) return gf::fail(GF_ERR_INVALID_ARG, "%s: h must be 16-byte aligned", who);
   const gfb::FfPlan pl = gfb::plan_ff(*ff, GF_PASS_BACKWARD, static_cast<char*>(workspace));
   GFB_TRY(gfb::check_workspace(who, workspace, workspace_bytes, pl.bytes));
   gfb::Range r("gfblock.gated_ff_backward");

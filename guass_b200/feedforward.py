@@ -7,10 +7,11 @@ input projections, the activation, the product and the dropout are one kernel;
 the output projection is a second.  Matrices are bf16 or fp16, products
 accumulate in fp32.
 
-The training forward saves, in the room the two projections would take, what
-the backward multiplies with: the activation and its slope times the value,
-each with the dropout folded in.  The backward computes only the gradients that are asked for: with frozen weights (how
-the Gaussian adapters are trained) that is two kernels.
+The backward computes the projections and the dropout mask again from the
+block's input, so that a training forward keeps the input alone (and the
+hidden activations where ``w_out`` is trained).  It computes only the gradients
+that are asked for: with frozen weights (how the Gaussian adapters are
+trained) that is two kernels.
 """
 from __future__ import annotations
 
@@ -48,7 +49,7 @@ def _workspace(L, f, backward: bool) -> int:
 
 
 def _forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
-    """(y, h, u): h and u are the saved state, None without ``keep``."""
+    """(y, h): h is the saved state, None without ``keep``."""
     L = _block.lib()
     d, (out, hidden) = x.shape[-1], w_out.shape
     shape = x.shape
@@ -58,42 +59,40 @@ def _forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
     y = torch.empty(*shape[:-1], out, dtype=x.dtype, device=x.device)
     f.y, f.ld_y = y.data_ptr(), out
     hp = -(-hidden // 64) * 64
-    h = u = None
+    h = None
     if keep:
         h = torch.empty(f.tokens, hp, dtype=x.dtype, device=x.device)
-        u = torch.empty(f.tokens, 2 * hp, dtype=x.dtype, device=x.device)
-        f.h, f.u = h.data_ptr(), u.data_ptr()
+        f.h = h.data_ptr()
     if f.tokens:
         n = _workspace(L, f, False)
         ws = torch.empty(n + (0 if keep else 2 * f.tokens * hp), dtype=torch.uint8, device=x.device)
         if not keep:
             f.h = ws.data_ptr() + n
         _block.call(x.device, L.gf_gated_ff_forward, ctypes.byref(f), ws.data_ptr(), n)
-    return y, h, u
+    return y, h
 
 
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_in, w_out, b_in, b_out, activation, p, seed, site):
-        y, h, u = _forward(x, w_in, w_out, b_in, b_out, activation, _block.make_rule(p, seed, site, x.device), True)
         need = ctx.needs_input_grad
-        ctx.save_for_backward(x if need[1] else None, w_in, w_out, u, h if need[2] else None)
-        ctx.activation, ctx.shape = activation, x.shape
+        rule = _block.make_rule(p, seed, site, x.device)
+        y, h = _forward(x, w_in, w_out, b_in, b_out, activation, rule, need[2])
+        # (a saved seed tensor: autograd refuses one that has changed)
+        ctx.save_for_backward(x, w_in, w_out, b_in, h, seed if isinstance(seed, torch.Tensor) else None)
+        ctx.activation, ctx.rule = activation, rule
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w_in, w_out, u, h = ctx.saved_tensors
-        need, (out, hidden), d = ctx.needs_input_grad, w_out.shape, w_in.shape[1]
-        dy = _block.rows_of(dy, out)
+        x, w_in, w_out, b_in, h, _ = ctx.saved_tensors
+        need, (out, hidden), d, shape = ctx.needs_input_grad, w_out.shape, w_in.shape[1], x.shape
+        dy, x = _block.rows_of(dy, out), _block.rows_of(x, d)
         w_in, w_out = _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
-        x = dy.new_empty(0, d) if x is None else _block.rows_of(x, d)
+        b_in = None if b_in is None else b_in.contiguous()
         L = _block.lib()
-        # the saved factors hold the dropout: the backward has no rule of its own
-        f = _describe(x, w_in, w_out, None, None, ctx.activation, _block.GfDropoutRule())
-        f.tokens = dy.shape[0]
-        f.u = u.data_ptr()
+        f = _describe(x, w_in, w_out, b_in, None, ctx.activation, ctx.rule)
         f.dy, f.ld_dy = dy.data_ptr(), _block.ld(dy)
         if h is not None:
             f.h = h.data_ptr()
@@ -101,7 +100,7 @@ class _GatedFeedForward(torch.autograd.Function):
         def grad(wanted, *shape):
             return torch.empty(shape, dtype=dy.dtype, device=dy.device) if wanted else None
 
-        dx, dw_in, dw_out = grad(need[0], *ctx.shape), grad(need[1], 2 * hidden, d), grad(need[2], out, hidden)
+        dx, dw_in, dw_out = grad(need[0], *shape), grad(need[1], 2 * hidden, d), grad(need[2], out, hidden)
         db_in, db_out = grad(need[3], 2 * hidden), grad(need[4], out)
         for name, g in (("dx", dx), ("dw_in", dw_in), ("dw_out", dw_out), ("db_in", db_in), ("db_out", db_out)):
             if g is not None:
@@ -123,8 +122,8 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str
     start on 16-byte boundaries cost a copy).  ``activation``: ``"gelu"`` (the
     error-function form) or ``"silu"``.  ``dropout_p``, ``seed`` and ``site``
     drop hidden activations by the rule of :func:`guass_b200.dropout.dropout`
-    on the hidden ``[rows, hidden]``; the backward uses the mask of its
-    forward, whatever becomes of a seed tensor.  Returns [..., out].
+    on the hidden ``[rows, hidden]``; a seed tensor must not change between
+    the forward and its backward.  Returns [..., out].
 
     Differentiable once in every tensor.  Work goes to the current stream of
     ``x``'s device; nothing synchronises, and both passes can be captured."""

@@ -53,16 +53,13 @@ typedef struct gf_dropout_rule {
  *   u = x w_in^T + b_in          [tokens, 2 * hidden]: value half, gate half
  *   h = dropout(u_value * act(u_gate))
  *   y = h w_out^T + b_out        [tokens, out_features]
- * Products accumulate in fp32; h, what is saved in u and the gradient of u are
- * rounded to `dtype` where they are stored (tensor-core operands), y and the
- * gradients once at the end.
+ * Products accumulate in fp32; h and the gradient of u are rounded to `dtype`
+ * where they are stored (tensor-core operands), y and the gradients once at
+ * the end.
  *
- * h, and for a training forward u, are the saved state, with leading
- * dimensions Hp and 2 * Hp, Hp = hidden rounded up to a multiple of 64.  u
- * holds what the gradient of h is multiplied with, keep * act(u_gate) and, Hp
- * columns on, keep * u_value * act'(u_gate), keep being 0 or 1 / (1 - p).  The
- * forward always writes h and writes u when it is not NULL; the backward reads
- * u, and h when dw_out is wanted. */
+ * The forward writes h, with leading dimension Hp = hidden rounded up to a
+ * multiple of 64.  The backward takes the forward's inputs, computes u and the
+ * dropout again from them, and needs the saved h when dw_out is wanted only. */
 typedef struct gf_gated_ff {
   int64_t tokens, in_features, hidden, out_features; /* tokens >= 0, the others > 0, each < 2^31 - 512 */
   int32_t dtype;      /* GF_BF16 or GF_F16, of every matrix and vector */
@@ -73,7 +70,6 @@ typedef struct gf_gated_ff {
   const void* b_in;                    /* [2 * hidden] or NULL */
   const void* w_out; int64_t ld_w_out; /* [out_features, hidden] */
   const void* b_out;                   /* [out_features] or NULL */
-  void* u;                             /* [tokens, 2 * Hp] saved factors, or NULL; 16-byte aligned */
   void* h;                             /* [tokens, Hp]; 16-byte aligned */
   void* y;           int64_t ld_y;     /* [tokens, out_features] (forward) */
   /* backward: the gradient of y, and the wanted gradients (NULL = not wanted; contiguous) */

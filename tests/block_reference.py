@@ -84,8 +84,6 @@ def feed_forward(x, w_in, w_out, b_in, b_out, act, keep, dy, dtype):
     out = dict(y=(y, SLACK * (ey + rounding(y, dtype))))
     if dy is None:
         return out
-    # the backward reads the rounded u
-    ev, eg = ev + rounding(v, dtype), eg + rounding(g, dtype)
     dh = dy @ w_out * keep
     edh = keep * (o * SUM_ERR * (dy.abs() @ w_out.abs())) + dh.abs() * 2.0 ** -22
     dv, dg = dh * a, dh * v * slope

@@ -47,7 +47,7 @@ def test_struct_layout_matches_c(tmp_path):
 def _ff(**kw):
     f = _block.GfGatedFf(tokens=4, in_features=8, hidden=16, out_features=8, dtype=_lib.GF_BF16, ld_x=8, ld_w_in=8,
                          ld_w_out=16, ld_y=8, ld_dy=8)
-    for name in ("x", "w_in", "w_out", "u", "h", "y", "dy"):
+    for name in ("x", "w_in", "w_out", "h", "y", "dy"):
         setattr(f, name, FAKE)
     for k, v in kw.items():
         setattr(f.dropout if k in ("p", "reserved", "seed_ptr") else f, k, v)
@@ -93,7 +93,7 @@ def test_feed_forward_pointers_and_workspace_refused():
     assert forward(ws=FAKE + 16)[0] == bad
     assert forward(size=16)[0] == bad and "too small" in _lib.last_error()
     assert forward(ld_y=7)[0] == bad
-    for name in ("dy", "w_out", "u", "w_in"):
+    for name in ("dy", "w_out", "x", "w_in"):
         assert backward(**{name: None})[0] == bad
     assert backward(size=16)[0] == bad and "too small" in _lib.last_error()
     assert backward(ld_dy=7)[0] == bad
