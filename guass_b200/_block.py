@@ -137,11 +137,30 @@ def call(device, fn, *args) -> None:
     device current.  (The raw calls behind torch.cuda.current_stream and
     torch.cuda.device: those objects cost more than a small launch.)"""
     index = device.index
-    if index is None or index == torch._C._cuda_getDevice():
-        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice() if index is None else index)))
+    if index == torch._C._cuda_getDevice():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
         with torch.cuda.device(index):
             _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def run(device, size_fn, fn, desc, *args, room: int = 0, use_room=None, query=()) -> None:
+    """``fn(desc, *args, workspace, bytes, stream)`` with the workspace that
+    ``size_fn(desc, *query)`` asks for, on ``device`` as :func:`call`.
+    ``use_room(pointer)`` gets ``room`` further bytes behind it."""
+    index = device.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return run(device, size_fn, fn, desc, *args, room=room, use_room=use_room, query=query)
+    ref = ctypes.byref(desc)
+    n = size_fn(ref, *query)
+    if n == 0:
+        raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
+    ws = torch.empty(n + room, dtype=torch.uint8, device=device)
+    ptr = ws.data_ptr()
+    if use_room is not None:
+        use_room(ptr + n)
+    _lib.check(fn(ref, *args, ptr, n, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:

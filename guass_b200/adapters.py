@@ -229,6 +229,7 @@ class BatchedAdapters:
             self.n_off.append(self.n_off[-1] + o * i)
         self._current = None
         self._orig = {}
+        self._int8 = None
 
     def _packed_params(self):
         mu = torch.cat([torch.tanh(m.mu_raw) for m in self.modules])  # gaussian_linear.py:153-154
@@ -316,7 +317,7 @@ class BatchedAdapters:
         weights; undo with :meth:`unquantize`."""
         from guass_b200.int8 import Int8Linear
 
-        if getattr(self, "_int8", None):
+        if self._int8:
             raise RuntimeError("quantize_merged: the layers are already served in 8 bits")
         self._int8 = []
         for m, d in zip(self.modules, self.render()):
@@ -326,7 +327,7 @@ class BatchedAdapters:
             m.forward = layer.forward
 
     def unquantize(self):
-        for m, forward, _ in getattr(self, "_int8", None) or []:
+        for m, forward, _ in self._int8 or []:
             if forward is None:
                 m.__dict__.pop("forward", None)
             else:
@@ -412,6 +413,7 @@ class BatchedAdapters:
             m.compute_delta_weight = cdw
 
     def uninstall(self):
+        self.unquantize()
         for m in self.modules:
             orig = self._orig.pop(id(m), None)
             if orig is not None:
@@ -450,7 +452,8 @@ class ModelRenderer:
     def _before_forward(self, module, args):
         if self.bank.shapes_changed():
             self.bank = self.bank.rebuilt()
-        self.bank.render()
+        if not self.bank._int8:  # served in 8 bits: nothing to render
+            self.bank.render()
 
     def remove(self) -> None:
         self._handle.remove()

@@ -194,23 +194,18 @@ constexpr int kVectorBytes = 32 * 4;    // a warp's vector of 32 floats (bias, s
 constexpr uint32_t kTmemCols = 512;
 constexpr int kSmemLimit = 232448;
 
-#ifndef GFB_W1
-#define GFB_W1 8
-#endif
-#ifndef GFB_W2
-#define GFB_W2 8
-#endif
 enum Epilogue { EPI_STORE, EPI_GATED, EPI_GATED_BWD, EPI_INT8 };
 
 // Warps and shared memory of a variant.  A chunk's result leaves as staging
 // blocks through TMA stores, which have the next chunk's arithmetic to be read
-// in; what is left holds operand stages.  Eight epilogue warps were as fast as
-// 12 or 16 for the 16-bit products, whose long tiles are bound by the memory
-// they write; the integer results take a conversion each and gain from 12
-// (16384 x 1280 x 10240: 160 us against 171).
+// in; what is left holds operand stages.  The gate's arithmetic hides behind
+// 16 warps (16384 x 320 x 1280 forward: 34 us, with 8 warps 39), the integer
+// results, a conversion each, behind 12 (16384 x 1280 x 10240: 160 us, with 8
+// warps 171); the backward, whose products take longer, is no faster with more
+// than 8 (1024 x 1280 x 5120: 37 us, with 16 warps and fewer stages 42).
 template <int EPI>
 struct Config {
-  static constexpr int epi_warps = EPI == EPI_INT8 ? 12 : EPI == EPI_GATED_BWD ? GFB_W2 : EPI == EPI_GATED ? GFB_W1 : 8;
+  static constexpr int epi_warps = EPI == EPI_GATED ? 16 : EPI == EPI_INT8 ? 12 : 8;
   static constexpr int threads = 64 + 32 * epi_warps;
   static constexpr int blocks = EPI == EPI_GATED ? 1 : 2;
   static constexpr int vectors = EPI == EPI_STORE ? 1 : 2;
@@ -332,11 +327,11 @@ struct EpilogueWarp {
   }
 
   // One 32-column chunk at result column n of rows m .. m + 31, from the
-  // accumulator columns at `acc` (dh: at `acc2`).  `release` runs once they are read, and
-  // `fetch_next` once `ahead` is.
+  // accumulator columns at `acc` (dh: at `acc2`).  `release` runs once they
+  // are read, `fetch_next` once `ahead` is.
   template <typename Release, typename Next>
-  __device__ __forceinline__ void chunk(uint32_t acc, uint32_t acc2, const Tile& t, int m, int n, const Ahead& ahead, Release release,
-                                        Next fetch_next) {
+  __device__ __forceinline__ void chunk(uint32_t acc, uint32_t acc2, const Tile& t, int m, int n, const Ahead& ahead,
+                                        Release release, Next fetch_next) {
     uint32_t d[32];
     if constexpr (EPI == EPI_STORE || EPI == EPI_INT8) tc::tmem_load32(d, acc);
     if constexpr (EPI == EPI_STORE) {

@@ -15,11 +15,9 @@ trained) that is two kernels.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
-from guass_b200 import _block, _lib
+from guass_b200 import _block
 
 _TYPES = (torch.bfloat16, torch.float16)
 
@@ -41,13 +39,6 @@ def _describe(x, w_in, w_out, b_in, b_out, activation, rule):
     return f
 
 
-def _workspace(L, f, backward: bool) -> int:
-    n = L.gf_gated_ff_workspace_bytes(ctypes.byref(f), int(backward))
-    if n == 0:
-        raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
-    return n
-
-
 def _forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
     """(y, h): h is the saved state, None without ``keep``."""
     L = _block.lib()
@@ -59,16 +50,16 @@ def _forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
     y = torch.empty(*shape[:-1], out, dtype=x.dtype, device=x.device)
     f.y, f.ld_y = y.data_ptr(), out
     hp = -(-hidden // 64) * 64
-    h = None
+    h, use_room = None, None
     if keep:
         h = torch.empty(f.tokens, hp, dtype=x.dtype, device=x.device)
         f.h = h.data_ptr()
+    else:
+        def use_room(pointer):
+            f.h = pointer
     if f.tokens:
-        n = _workspace(L, f, False)
-        ws = torch.empty(n + (0 if keep else 2 * f.tokens * hp), dtype=torch.uint8, device=x.device)
-        if not keep:
-            f.h = ws.data_ptr() + n
-        _block.call(x.device, L.gf_gated_ff_forward, ctypes.byref(f), ws.data_ptr(), n)
+        _block.run(x.device, L.gf_gated_ff_workspace_bytes, L.gf_gated_ff_forward, f, query=(0,),
+                   room=0 if keep else 2 * f.tokens * hp, use_room=use_room)
     return y, h
 
 
@@ -105,9 +96,7 @@ class _GatedFeedForward(torch.autograd.Function):
         for name, g in (("dx", dx), ("dw_in", dw_in), ("dw_out", dw_out), ("db_in", db_in), ("db_out", db_out)):
             if g is not None:
                 setattr(f, name, g.data_ptr())
-        n = _workspace(L, f, True)
-        ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
-        _block.call(dy.device, L.gf_gated_ff_backward, ctypes.byref(f), ws.data_ptr(), n)
+        _block.run(dy.device, L.gf_gated_ff_workspace_bytes, L.gf_gated_ff_backward, f, query=(1,))
         return dx, dw_in, dw_out, db_in, db_out, None, None, None, None
 
 

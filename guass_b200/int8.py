@@ -9,12 +9,10 @@ multiplies.  Forward only.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch import nn
 
-from guass_b200 import _block, _lib
+from guass_b200 import _block
 
 _MAX_K = 131071
 
@@ -63,12 +61,6 @@ def _describe(m, n, k, b, b_scale, bias, out):
     return d
 
 
-def _workspace(size, device):
-    if size == 0:
-        raise _lib.GfieldError(_lib.GF_ERR_INVALID_ARG, _lib.last_error())
-    return torch.empty(size, dtype=torch.uint8, device=device)
-
-
 def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
     """``(a b^T) * a_scale[:, None] * b_scale + bias`` as ``out_dtype``.
 
@@ -90,8 +82,7 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
     d = _describe(m, n, k, b, b_scale, bias, out)
     d.a, d.ld_a, d.a_scale = a.data_ptr(), _block.ld(a), a_scale.data_ptr()
     L = _block.lib()
-    ws = _workspace(L.gf_int8_product_workspace_bytes(ctypes.byref(d)), a.device)
-    _block.call(a.device, L.gf_int8_matmul, ctypes.byref(d), ws.data_ptr(), ws.shape[0])
+    _block.run(a.device, L.gf_int8_product_workspace_bytes, L.gf_int8_matmul, d)
     return out
 
 
@@ -115,9 +106,8 @@ def int8_linear(x, q_weight, weight_scale, bias=None, *, out_dtype=None):
     bias = None if bias is None else bias.contiguous()
     d = _describe(x.shape[0], n, k, q_weight, weight_scale, bias, out)
     L = _block.lib()
-    ws = _workspace(L.gf_int8_linear_workspace_bytes(ctypes.byref(d)), x.device)
-    _block.call(x.device, L.gf_int8_linear, ctypes.byref(d), x.data_ptr(), _block.ld(x), _block.DTYPES[x.dtype],
-                ws.data_ptr(), ws.shape[0])
+    _block.run(x.device, L.gf_int8_linear_workspace_bytes, L.gf_int8_linear, d, x.data_ptr(), _block.ld(x),
+               _block.DTYPES[x.dtype])
     return out
 
 

@@ -405,7 +405,8 @@ def test_captured_step_sees_new_seeds():
     def step():
         y = gated_feed_forward(x, *w, dropout_p=0.2, seed=seed, site=1)
         z = dropout(y, 0.2, seed, site=2, residual=x)
-        return z, torch.autograd.grad(z, [x], dy)[0]
+        grad, = torch.autograd.grad(z, [x], dy)
+        return z.detach(), grad  # a graph of x that lives on would tie the next capture to its stream
 
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
@@ -444,11 +445,68 @@ def test_captured_int8():
 
 def test_seed_changed_before_backward_is_refused():
     x = torch.ones(4, 4, device="cuda", requires_grad=True)
+    t = ff_inputs(4, 8, 16, 8, BF16, False)
+    leaf = t["x"].requires_grad_()
     seed = torch.tensor([1], device="cuda")
-    y = dropout(x, 0.5, seed)
+    made = dropout(x, 0.5, seed), gated_feed_forward(leaf, t["w_in"], t["w_out"], dropout_p=0.5, seed=seed)
     seed.add_(1)
-    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
-        y.sum().backward()
+    for y in made:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_no_second_derivative():
+    x = torch.ones(4, 8, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(dropout(x, 0.5, 1).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [x])
+
+
+def test_ff_long_sums_and_wide_rows():
+    """K ranges joined in order (a long K and few tiles), rows past 2^16 columns."""
+    ff_check(ff_inputs(16, 24, 33000, 40, BF16, True), "gelu", wants=("x", "w_out"))
+    ff_check(ff_inputs(2100, 24, 40, 64, FP16, True), "silu")
+
+
+def test_ff_one_input_in_two_blocks():
+    """Two blocks in a row on the same input, whose gradient is the sum of both."""
+    t, s = (ff_inputs(50, 32, 48, 32, FP16, True, seed=k) for k in (1, 20))
+    x = t["x"].detach().requires_grad_()
+
+    def block(w, v):
+        return gated_feed_forward(v, *(w[n] for n in ("w_in", "w_out", "b_in", "b_out")), dropout_p=0.1, seed=2)
+
+    dy = normal(50, 32, seed=3, dtype=FP16)
+    both, = torch.autograd.grad([block(t, x), block(s, x)], [x], [dy, dy])
+    one, = torch.autograd.grad(block(t, x), [x], dy)
+    two, = torch.autograd.grad(block(s, x), [x], dy)
+    assert torch.equal(both, one + two)
+
+
+def test_dropout_large_positions():
+    """Elements whose offset passes 2^31 (as bytes and as elements), few rows and many."""
+    for rows, cols in ((3, 1 << 30), (1 << 20, 2100)):
+        x = torch.ones(1, 1, dtype=BF16, device="cuda").expand(rows, cols)
+        y = dropout(x, 0.5, 17, site=1)
+        for r in (0, rows - 1):
+            c = min(cols, 4096)
+            mask = ref.keep_mask(1, 8, 0.5, 17, 1)  # row 0: the reference's own start
+            words = [ref.philox([(cols - c + j) // 4, r, 1, 0], [17, 0])[(cols - c + j) % 4] >= 1 << 31 for j in range(c)]
+            assert torch.equal(y[r, cols - c:].cpu() != 0, torch.tensor(words))
+            if r == 0:
+                assert torch.equal(y[0, :8].cpu() != 0, mask[0])
+        del y
+
+
+def test_int8_many_rows_past_2_31_bytes():
+    """A result whose byte offsets pass 2^31."""
+    m, n, k = 300_000, 4096, 32
+    a = torch.ones(m, k, dtype=torch.int8, device="cuda")
+    a[-1] = 3
+    b = torch.ones(n, k, dtype=torch.int8, device="cuda")
+    one = torch.ones(m, device="cuda")
+    y = int8_matmul(a, one, b, one[:n])
+    assert (y[:1000] == 32).all() and (y[-1] == 96).all() and (y[-1000:-1] == 32).all()
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])

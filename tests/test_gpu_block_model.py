@@ -114,3 +114,44 @@ def test_merged_layers_in_8_bits(fused):
         bank.unquantize()
         assert torch.equal(m(x), before)
         assert not any("forward" in q.__dict__ for q in bank.modules) or fused
+
+
+def test_model_renderer_serves_8_bits():
+    """quantize_merged under ModelRenderer: no render per forward; uninstalling leaves 8-bit serving."""
+    from guass_b200.adapters import ModelRenderer
+
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = sd15.SD15UNet(sd15.tiny_config(), dtype=torch.bfloat16)
+    model.cuda()
+    r = ModelRenderer(model, fused_weight=True, out_dtype=torch.bfloat16)
+    inp = inputs()
+    with torch.no_grad():
+        before = model(inp.latents, inp.t, inp.text)
+        r.bank.quantize_merged()
+        r.bank._current = None  # a render would set it
+        a = model(inp.latents, inp.t, inp.text)
+        assert r.bank._current is None and torch.equal(a, model(inp.latents, inp.t, inp.text))
+        assert torch.isfinite(a).all() and not torch.equal(a, before)
+        r.bank.unquantize()
+        assert torch.equal(model(inp.latents, inp.t, inp.text), before)
+        r.bank.quantize_merged()
+        r.remove()
+    assert not any("forward" in m.__dict__ for m in model.adapters().values())
+
+
+def test_8_bits_refuse_training():
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = sd15.SD15UNet(sd15.tiny_config(), dtype=torch.bfloat16)
+    model.cuda()
+    bank = BatchedAdapters(model.adapters(), out_dtype=torch.bfloat16)
+    bank.install()
+    bank.render()
+    bank.quantize_merged()
+    m = bank.modules[0]
+    x = torch.randn(3, m.in_features, device="cuda").bfloat16().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward"):
+        m(x)
+    with torch.no_grad():
+        assert m(x).shape == (3, m.out_features)
