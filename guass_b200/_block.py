@@ -115,13 +115,10 @@ def device_flags(device="cuda", reset: bool = False) -> int:
     return flags.value
 
 
-def require(cond: bool, message: str, kind=ValueError) -> None:
-    if not cond:
-        raise kind(message)
-
-
 def check_tensor(name: str, t, dtypes, device=None) -> None:
     """A CUDA tensor of one of ``dtypes`` (and on ``device``)."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and (device is None or t.device == device):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t)!r}")
     if t.device.type != "cuda":
@@ -187,6 +184,7 @@ def make_rule(p: float, seed, site: int, device) -> GfDropoutRule:
         raise ValueError(f"site must be in [0, 2**32), got {site}")
     if isinstance(seed, torch.Tensor):
         check_tensor("seed", seed, (torch.int64,), device)
-        require(seed.numel() == 1, f"a seed tensor has one element, got {tuple(seed.shape)}")
+        if seed.numel() != 1:
+            raise ValueError(f"a seed tensor has one element, got {tuple(seed.shape)}")
         return GfDropoutRule(p, 0, seed.data_ptr(), site, 0)
     return GfDropoutRule(p, int(seed) & 0xFFFFFFFFFFFFFFFF, None, site, 0)

@@ -64,7 +64,8 @@ def dropout(x, p: float, seed, *, site: int = 0, residual=None):
     _block.check_tensor("x", x, tuple(_block.DTYPES))
     if residual is not None:
         _block.check_tensor("residual", residual, (x.dtype,), x.device)
-        _block.require(residual.shape == x.shape, f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
+        if residual.shape != x.shape:
+            raise ValueError(f"residual is {tuple(residual.shape)}, x {tuple(x.shape)}")
     if x.numel() == 0:
         _block.make_rule(p, seed, site, x.device)
         return x.clone() if residual is None else residual + x

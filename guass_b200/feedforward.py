@@ -100,6 +100,28 @@ class _GatedFeedForward(torch.autograd.Function):
         return dx, dw_in, dw_out, db_in, db_out, None, None, None, None
 
 
+def _check(x, w_in, w_out, b_in, b_out, activation) -> None:
+    _block.check_tensor("x", x, _TYPES)
+    device, dtypes = x.device, (x.dtype,)
+    _block.check_tensor("w_in", w_in, dtypes, device)
+    _block.check_tensor("w_out", w_out, dtypes, device)
+    if x.dim() < 1 or w_in.dim() != 2 or w_out.dim() != 2:
+        raise ValueError("x needs a feature dimension, w_in and w_out two dimensions")
+    d, (out, hidden), (rows, cols) = x.shape[-1], w_out.shape, w_in.shape
+    if rows != 2 * hidden or cols != d:
+        raise ValueError(f"w_in is {(rows, cols)}, expected {(2 * hidden, d)} for x {tuple(x.shape)} and w_out "
+                         f"{(out, hidden)}")
+    if d == 0 or hidden == 0 or out == 0:
+        raise ValueError("feature sizes must be positive")
+    for name, b, n in (("b_in", b_in, rows), ("b_out", b_out, out)):
+        if b is not None:
+            _block.check_tensor(name, b, dtypes, device)
+            if b.dim() != 1 or b.shape[0] != n:
+                raise ValueError(f"{name} must be [{n}], got {tuple(b.shape)}")
+    if activation not in _block.ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_block.ACTIVATIONS)}, got {activation!r}")
+
+
 def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str = "gelu", dropout_p: float = 0.0,
                        seed=0, site: int = 0):
     """``linear(dropout(value * act(gate)), w_out, b_out)`` where
@@ -116,22 +138,10 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str
 
     Differentiable once in every tensor.  Work goes to the current stream of
     ``x``'s device; nothing synchronises, and both passes can be captured."""
-    _block.check_tensor("x", x, _TYPES)
-    for name, t in (("w_in", w_in), ("w_out", w_out), ("b_in", b_in), ("b_out", b_out)):
-        if t is not None or name[0] == "w":
-            _block.check_tensor(name, t, (x.dtype,), x.device)
-    _block.require(x.dim() >= 1 and w_in.dim() == 2 and w_out.dim() == 2, "x needs a feature dimension, w_in and "
-                   "w_out two dimensions")
-    d, hidden = x.shape[-1], w_out.shape[1]
-    _block.require(w_in.shape[0] == 2 * hidden and w_in.shape[1] == d,
-                   f"w_in is {tuple(w_in.shape)}, expected {(2 * hidden, d)} for x {tuple(x.shape)} and w_out "
-                   f"{tuple(w_out.shape)}")
-    _block.require(min(d, hidden, w_out.shape[0]) > 0, "feature sizes must be positive")
-    _block.require(b_in is None or tuple(b_in.shape) == (2 * hidden,), "b_in must be [2 * hidden]")
-    _block.require(b_out is None or tuple(b_out.shape) == (w_out.shape[0],), "b_out must be [out]")
-    _block.require(activation in _block.ACTIVATIONS,
-                   f"activation must be one of {sorted(_block.ACTIVATIONS)}, got {activation!r}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_in, w_out, b_in, b_out)):
+    _check(x, w_in, w_out, b_in, b_out, activation)
+    if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad
+                                    or b_in is not None and b_in.requires_grad
+                                    or b_out is not None and b_out.requires_grad):
         return _GatedFeedForward.apply(x, w_in, w_out, b_in, b_out, activation, dropout_p, seed, site)
     rule = _block.make_rule(dropout_p, seed, site, x.device)
     return _forward(x, w_in, w_out, b_in, b_out, activation, rule, False)[0]

@@ -25,7 +25,8 @@ def quantize_rows(x):
     so that products with it are NaN.  ``q`` [..., K] is a view of rows that
     start on 16-byte boundaries, the layout the product reads in place."""
     _block.check_tensor("x", x, tuple(_block.DTYPES))
-    _block.require(x.dim() >= 1 and x.shape[-1] > 0, "x needs a last dimension of at least 1")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("x needs a last dimension of at least 1")
     k = x.shape[-1]
     v = _block.rows_of(x.detach(), k)
     kp = -(-k // 16) * 16
@@ -38,16 +39,21 @@ def quantize_rows(x):
 
 def _check_weight(b, b_scale, bias, out_dtype, device):
     """[N, K] int8 with [N] scales and bias: (n, k)."""
-    _block.check_tensor("b" if bias is None else "q_weight", b, (torch.int8,), device)
-    _block.check_tensor("weight scales", b_scale, (torch.float32,), device)
-    _block.require(out_dtype in _block.DTYPES, f"out_dtype must be one of {list(_block.DTYPES)}, got {out_dtype}")
-    _block.require(b.dim() == 2, f"the int8 weight must be [N, K], got {tuple(b.shape)}")
+    _block.check_tensor("the int8 weight", b, (torch.int8,), device)
+    _block.check_tensor("its scales", b_scale, (torch.float32,), device)
+    if out_dtype not in _block.DTYPES:
+        raise ValueError(f"out_dtype must be one of {list(_block.DTYPES)}, got {out_dtype}")
+    if b.dim() != 2:
+        raise ValueError(f"the int8 weight must be [N, K], got {tuple(b.shape)}")
     n, k = b.shape
-    _block.require(n > 0 and 0 < k <= _MAX_K, f"N must be positive and K in 1..{_MAX_K}, got N={n}, K={k}")
-    _block.require(b_scale.dim() == 1 and b_scale.shape[0] == n, f"weight scales must be [{n}]")
+    if n == 0 or not 0 < k <= _MAX_K:
+        raise ValueError(f"N must be positive and K in 1..{_MAX_K}, got N={n}, K={k}")
+    if b_scale.dim() != 1 or b_scale.shape[0] != n:
+        raise ValueError(f"the weight's scales must be [{n}], got {tuple(b_scale.shape)}")
     if bias is not None:
         _block.check_tensor("bias", bias, (out_dtype,), device)
-        _block.require(bias.dim() == 1 and bias.shape[0] == n, f"bias must be [{n}]")
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise ValueError(f"bias must be [{n}], got {tuple(bias.shape)}")
     return n, k
 
 
@@ -71,9 +77,11 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
     _block.check_tensor("a", a, (torch.int8,))
     _block.check_tensor("a_scale", a_scale, (torch.float32,), a.device)
     n, k = _check_weight(b, b_scale, bias, out_dtype, a.device)
-    _block.require(a.dim() == 2 and a.shape[1] == k, f"a is {tuple(a.shape)}, b {tuple(b.shape)}: expected [M, K] and [N, K]")
+    if a.dim() != 2 or a.shape[1] != k:
+        raise ValueError(f"a is {tuple(a.shape)}, b {tuple(b.shape)}: expected [M, K] and [N, K]")
     m = a.shape[0]
-    _block.require(tuple(a_scale.shape) == (m,), "a_scale must be [M]")
+    if tuple(a_scale.shape) != (m,):
+        raise ValueError(f"a_scale must be [{m}], got {tuple(a_scale.shape)}")
     a, b, a_scale, b_scale = _block.rows_of(a, k), _block.rows_of(b, k), a_scale.contiguous(), b_scale.contiguous()
     bias = None if bias is None else bias.contiguous()
     out = torch.empty(m, n, dtype=out_dtype, device=a.device)
@@ -97,8 +105,8 @@ def int8_linear(x, q_weight, weight_scale, bias=None, *, out_dtype=None):
         raise RuntimeError("int8_linear has no backward: call it under torch.no_grad() or on a detached input")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     n, k = _check_weight(q_weight, weight_scale, bias, out_dtype, x.device)
-    _block.require(x.dim() >= 1 and x.shape[-1] == k,
-                   f"x is {tuple(x.shape)}, q_weight {tuple(q_weight.shape)}: expected [..., K] and [N, K]")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x is {tuple(x.shape)}, q_weight {tuple(q_weight.shape)}: expected [..., K] and [N, K]")
     out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
     if out.numel() == 0:
         return out

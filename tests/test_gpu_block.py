@@ -523,3 +523,56 @@ def test_ff_few_tokens(size, tokens, dtype):
         t[n] = wide[:, :cols]
     ff_check(t, "gelu", p=0.25, seed=4, site=2)
     ff_check(t, "silu", wants=())
+
+
+def test_refusals_on_the_gpu():
+    t = ff_inputs(4, 8, 16, 8, BF16, True)
+    x, wi, wo, bi, bo = (t[n] for n in ("x", "w_in", "w_out", "b_in", "b_out"))
+    for args in ((x, wi[:-1], wo), (x, wi[:, 1:], wo), (x, wi, wo[:, :-1]), (x, wi, wo, bi[1:]), (x, wi, wo, bi, bo[1:]),
+                 (x, wi, wo[:0]), (x[:, :0], wi[:, :0], wo), (x, wi[0], wo)):
+        with pytest.raises(ValueError):
+            gated_feed_forward(*args)
+    for bad in (x.half(), x.float(), x.double()):
+        with pytest.raises(TypeError):
+            gated_feed_forward(bad, wi, wo)
+    with pytest.raises(TypeError):
+        gated_feed_forward(x, wi, wo, bi.float())
+    with pytest.raises(ValueError, match="activation"):
+        gated_feed_forward(x, wi, wo, activation="relu")
+    for kw in (dict(dropout_p=1.0), dict(dropout_p=-0.1), dict(dropout_p=0.1, site=-1)):
+        with pytest.raises(ValueError):
+            gated_feed_forward(x, wi, wo, **kw)
+        with pytest.raises(ValueError):
+            gated_feed_forward(x.detach().requires_grad_(), wi, wo, **kw)
+    with pytest.raises(TypeError):
+        gated_feed_forward(x, wi, wo, dropout_p=0.1, seed=torch.ones(1, device="cuda"))
+    with pytest.raises(ValueError):
+        gated_feed_forward(x, wi, wo, dropout_p=0.1, seed=torch.ones(2, dtype=torch.int64, device="cuda"))
+    with pytest.raises(RuntimeError):
+        gated_feed_forward(x, wi, wo, dropout_p=0.1, seed=torch.ones(1, dtype=torch.int64))
+    with pytest.raises(RuntimeError):
+        gated_feed_forward(x, wi.cpu(), wo)
+    with pytest.raises(ValueError):
+        dropout(x, 0.5, 1, residual=x[:2])
+    with pytest.raises(TypeError):
+        dropout(x, 0.5, 1, residual=x.float())
+    with pytest.raises(TypeError):
+        dropout(x.long(), 0.5, 1)
+    q, s = quantize_rows(wi)
+    for args in ((q[:, 1:], s, q, s), (q, s[1:], q, s), (q, s, q, s[1:]), (q, s, q[:0], s[:0]), (q[0], s, q, s)):
+        with pytest.raises(ValueError):
+            int8_matmul(*args)
+    with pytest.raises(ValueError):
+        int8_matmul(q, s, q, s, out_dtype=torch.float64)
+    with pytest.raises(TypeError):
+        int8_matmul(q, s, q, s, bias=torch.zeros(32, device="cuda"))
+    with pytest.raises(TypeError):
+        int8_matmul(q, s.double(), q, s)
+    with pytest.raises(TypeError):
+        quantize_rows(q)
+    with pytest.raises(ValueError):
+        quantize_rows(wi[:, :0])
+    with pytest.raises(ValueError):
+        int8_linear(x[:, 1:], q, s)
+    with pytest.raises(RuntimeError, match="no backward"):
+        int8_linear(x.detach().requires_grad_(), q, s)
