@@ -596,6 +596,8 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
   else __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&pipe->tmem);
+  tc::dependency_wait();  // everything up to here is the CTA's own
+  tc::let_dependents();
 
   if (warp == 0) {
     // Both CTAs of a pair load; the copies of both count on the first one's barrier.
@@ -760,6 +762,8 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
 
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmParams p) {
+  tc::dependency_wait();
+  tc::let_dependents();
   const int64_t groups = p.ld_partial / 4, total = (int64_t)p.M * groups;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t m = i / groups;
@@ -808,6 +812,8 @@ struct SumJobs {
 
 template <typename T>
 __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ SumJobs jobs) {
+  tc::dependency_wait();
+  tc::let_dependents();
   const SumJob& j = jobs.job[blockIdx.z];
   const int c = blockIdx.x * 32 + threadIdx.x % 32, w = threadIdx.x / 32;
   if ((int)blockIdx.x * 32 >= j.cols || (int)blockIdx.y >= j.parts) return;
@@ -827,6 +833,8 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant_
 }
 template <typename T>
 __global__ void __launch_bounds__(256) column_join_kernel(const __grid_constant__ SumJobs jobs) {
+  tc::dependency_wait();
+  tc::let_dependents();
   const SumJob& j = jobs.job[blockIdx.z];
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (j.seg_pad ? 2 * j.seg : j.cols)) return;
@@ -854,6 +862,8 @@ struct AlignJobs {
 
 template <typename E>
 __global__ void __launch_bounds__(256) align_kernel(const __grid_constant__ AlignJobs jobs) {
+  tc::dependency_wait();
+  tc::let_dependents();
   const AlignJob& j = jobs.job[blockIdx.y];
   // a warp copies whole rows
   const int lane = threadIdx.x & 31;
@@ -896,6 +906,8 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
   constexpr int kChunk = 2048;                      // columns of x in shared memory at a time
   __shared__ __align__(16) T xs[TOKENS][kChunk];
   __shared__ float part[kSkinnyWarps][TOKENS];
+  tc::dependency_wait();
+  tc::let_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = blockIdx.x * (kSkinnyWarps / kShare) + warp / kShare;
   const bool live = n < p.n;
@@ -1027,6 +1039,8 @@ struct DropoutParams {
 template <typename T, bool VEC, bool ROWS, bool RES, typename I>
 __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
   constexpr int V = VEC ? 16 / sizeof(T) : 4, U = 2;
+  tc::dependency_wait();
+  tc::let_dependents();
   const Philox rng(p.drop);
   const I inner = (I)(ROWS ? p.rows : p.groups), outer = (I)(ROWS ? p.groups : p.rows);
   const I step = (I)gridDim.x * blockDim.x;
@@ -1110,6 +1124,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
   constexpr int64_t per_block = 256 / TPR;
   constexpr int kHeld = VPL > 0 ? VPL : 1;
   __shared__ uint32_t warp_max[8];
+  tc::dependency_wait();
+  tc::let_dependents();
   for (int64_t base = blockIdx.x * per_block; base < rows; base += gridDim.x * per_block) {
     const int64_t r = base + threadIdx.x / TPR;
     const bool live = r < rows;
@@ -1182,6 +1198,22 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
     const cudaError_t e_ = (call);                                                                \
     if (e_ != cudaSuccess) return gf::fail(GF_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));     \
   } while (0)
+
+// Launches with the dependent-launch attribute (see tc::dependency_wait).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return cudaGetLastError();
+}
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -1337,14 +1369,14 @@ gf_status launch_gemm(GemmParams p, int sms, cudaStream_t st) {
   cfg.blockDim = dim3(C::threads);
   cfg.dynamicSmemBytes = smem_bytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  if (PAIR) {
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-  }
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1509,8 +1541,7 @@ gf_status run_align(const AlignJobs& jobs, int sms, cudaStream_t st) {
   if (jobs.n == 0) return GF_OK;
   int64_t rows = 0;
   for (int i = 0; i < jobs.n; ++i) rows = jobs.job[i].dst_rows > rows ? jobs.job[i].dst_rows : rows;
-  align_kernel<E><<<dim3(grid_for(rows, 8, sms), jobs.n), 256, 0, st>>>(jobs);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch(align_kernel<E>, dim3(grid_for(rows, 8, sms), jobs.n), 256, st, jobs);
   if (e != cudaSuccess) return fail(GF_ERR_CUDA, "align_kernel: %s", cudaGetErrorString(e));
   return GF_OK;
 }
@@ -1586,8 +1617,7 @@ gf_status product(const Shape& s, const Operand& a, bool a_mn, const Operand& b,
     GFB_TRY(make_out_map(&p.mo, Operand{out, M, N, ld_out}, map_type<T>(), 2));
   GFB_TRY((launch_gemm<EPI_STORE, T, 0, false>(p, s, sms, st)));
   if (s.splits > 1) {
-    join_kernel<T><<<grid_for(M * (p.ld_partial / 4), 256, sms), 256, 0, st>>>(p);
-    GFB_CUDA(cudaGetLastError());
+    GFB_CUDA(launch(join_kernel<T>, dim3(grid_for(M * (p.ld_partial / 4), 256, sms)), 256, st, p));
   }
   return GF_OK;
 }
@@ -1606,10 +1636,10 @@ gf_status skinny(const SkinnyParams& p, cudaStream_t st) {
   // (gated: a warp per column of h, padding included; else four per column of y)
   const int cols = GATED ? p.hp : p.n, per = GATED ? kSkinnyWarps : kSkinnyWarps / 4;
   const int grid = (int)ceil_div(cols, per);
-  if (p.tokens == 1) skinny_kernel<T, 1, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
-  else if (p.tokens <= 4) skinny_kernel<T, 4, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
-  else skinny_kernel<T, kSkinnyTokens, GATED><<<grid, 32 * kSkinnyWarps, 0, st>>>(p);
-  GFB_CUDA(cudaGetLastError());
+  const auto kernel = p.tokens == 1   ? skinny_kernel<T, 1, GATED>
+                      : p.tokens <= 4 ? skinny_kernel<T, 4, GATED>
+                                      : skinny_kernel<T, kSkinnyTokens, GATED>;
+  GFB_CUDA(launch(kernel, dim3(grid), 32 * kSkinnyWarps, st, p));
   return GF_OK;
 }
 
@@ -1661,10 +1691,8 @@ gf_status column_sums(const SumJobs& jobs, int n, cudaStream_t st) {
     cols = jobs.job[i].cols > cols ? jobs.job[i].cols : cols;
     parts = jobs.job[i].parts > parts ? jobs.job[i].parts : parts;
   }
-  column_sums_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), parts, n), 256, 0, st>>>(jobs);
-  GFB_CUDA(cudaGetLastError());
-  column_join_kernel<T><<<dim3((unsigned)ceil_div(cols, 256), 1, n), 256, 0, st>>>(jobs);
-  GFB_CUDA(cudaGetLastError());
+  GFB_CUDA(launch(column_sums_kernel<T>, dim3((unsigned)ceil_div(cols, 32), parts, n), 256, st, jobs));
+  GFB_CUDA(launch(column_join_kernel<T>, dim3((unsigned)ceil_div(cols, 256), 1, n), 256, st, jobs));
   return GF_OK;
 }
 
@@ -1716,45 +1744,44 @@ gf_status ff_backward(const gf_gated_ff& f, const FfPlan& pl, cudaStream_t st) {
 // ---- dropout and the 8-bit product
 
 template <typename T, bool RES, typename I>
-void launch_dropout(const DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
+cudaError_t launch_dropout(const DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
   const int grid = grid_for(ceil_div(p.rows * p.groups, 2), 256, sms);
-  if (vec) dropout_kernel<T, true, false, RES, I><<<grid, 256, 0, st>>>(p);
-  else if (by_rows) dropout_kernel<T, false, true, RES, I><<<grid, 256, 0, st>>>(p);
-  else dropout_kernel<T, false, false, RES, I><<<grid, 256, 0, st>>>(p);
+  const auto kernel = vec       ? dropout_kernel<T, true, false, RES, I>
+                      : by_rows ? dropout_kernel<T, false, true, RES, I>
+                                : dropout_kernel<T, false, false, RES, I>;
+  return launch(kernel, dim3(grid), 256, st, p);
 }
 template <typename T>
-void launch_dropout(DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
+cudaError_t launch_dropout(DropoutParams& p, bool vec, bool by_rows, int sms, cudaStream_t st) {
   p.groups = ceil_div(p.cols, vec ? 16 / (int64_t)sizeof(T) : 4);
   // positions pass their end by up to two strides of the grid
   const bool narrow = p.rows * p.groups < (int64_t(1) << 31);
-  if (p.res) {
-    if (narrow) launch_dropout<T, true, uint32_t>(p, vec, by_rows, sms, st);
-    else launch_dropout<T, true, uint64_t>(p, vec, by_rows, sms, st);
-  } else {
-    if (narrow) launch_dropout<T, false, uint32_t>(p, vec, by_rows, sms, st);
-    else launch_dropout<T, false, uint64_t>(p, vec, by_rows, sms, st);
-  }
+  if (p.res)
+    return narrow ? launch_dropout<T, true, uint32_t>(p, vec, by_rows, sms, st)
+                  : launch_dropout<T, true, uint64_t>(p, vec, by_rows, sms, st);
+  return narrow ? launch_dropout<T, false, uint32_t>(p, vec, by_rows, sms, st)
+                : launch_dropout<T, false, uint64_t>(p, vec, by_rows, sms, st);
 }
 
 template <typename T, int TPR, int VPL>
-void launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
+cudaError_t launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
                      cudaStream_t st) {
-  quantize_rows_kernel<T, TPR, VPL><<<grid_for(rows, 256 / TPR, sms), 256, 0, st>>>(rows, (int)cols, static_cast<const T*>(x),
-                                                                                  ld_x, q, ld_q, scale);
+  return launch(quantize_rows_kernel<T, TPR, VPL>, dim3(grid_for(rows, 256 / TPR, sms)), 256, st, rows, (int)cols,
+         static_cast<const T*>(x), ld_x, q, ld_q, scale);
 }
 template <typename T>
-void launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
+cudaError_t launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int sms,
                      cudaStream_t st) {
   const bool vec = aligned_rows(x, rows, ld_x, sizeof(T)) && cols % 8 == 0 && ld_q % 8 == 0 &&
                    (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
   // a warp for a row of up to 2048 values, a CTA for a longer one; aligned rows
   // of up to 16384 stay in registers
-  if (vec && cols <= 512) launch_quantize<T, 32, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (vec && cols <= 1280) launch_quantize<T, 32, 5>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (vec && cols <= 4096) launch_quantize<T, 256, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (vec && cols <= 16384) launch_quantize<T, 256, 8>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (cols <= 2048) launch_quantize<T, 32, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else launch_quantize<T, 256, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (vec && cols <= 512) return launch_quantize<T, 32, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (vec && cols <= 1280) return launch_quantize<T, 32, 5>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (vec && cols <= 4096) return launch_quantize<T, 256, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (vec && cols <= 16384) return launch_quantize<T, 256, 8>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (cols <= 2048) return launch_quantize<T, 32, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  return launch_quantize<T, 256, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
 }
 
 bool known_dtype(int d) { return d == GF_F32 || d == GF_BF16 || d == GF_F16; }
@@ -1846,10 +1873,9 @@ gf_status int8_product(const gf_int8_product& d, const Int8Plan& pl, cudaStream_
 gf_status quantise(int64_t rows, int64_t cols, int32_t dtype, const void* x, int64_t ld_x, int8_t* q, int64_t ld_q,
                    float* scale, cudaStream_t st) {
   const int sms = sm_count();
-  if (dtype == GF_F32) launch_quantize<float>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else if (dtype == GF_BF16) launch_quantize<__nv_bfloat16>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  else launch_quantize<__half>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  GFB_CUDA(cudaGetLastError());
+  GFB_CUDA(dtype == GF_F32    ? launch_quantize<float>(rows, cols, x, ld_x, q, ld_q, scale, sms, st)
+           : dtype == GF_BF16 ? launch_quantize<__nv_bfloat16>(rows, cols, x, ld_x, q, ld_q, scale, sms, st)
+                              : launch_quantize<__half>(rows, cols, x, ld_x, q, ld_q, scale, sms, st));
   return GF_OK;
 }
 
@@ -1931,10 +1957,9 @@ gf_status gf_dropout(int64_t rows, int64_t cols, int32_t dtype, const gf_dropout
   const bool by_rows = x_col_stride > x_row_stride && x_row_stride > 0;
   const int sms = gfb::sm_count();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GF_F32) gfb::launch_dropout<float>(p, vec, by_rows, sms, st);
-  else if (dtype == GF_BF16) gfb::launch_dropout<__nv_bfloat16>(p, vec, by_rows, sms, st);
-  else gfb::launch_dropout<__half>(p, vec, by_rows, sms, st);
-  GFB_CUDA(cudaGetLastError());
+  GFB_CUDA(dtype == GF_F32    ? gfb::launch_dropout<float>(p, vec, by_rows, sms, st)
+           : dtype == GF_BF16 ? gfb::launch_dropout<__nv_bfloat16>(p, vec, by_rows, sms, st)
+                              : gfb::launch_dropout<__half>(p, vec, by_rows, sms, st));
   return GF_OK;
 }
 

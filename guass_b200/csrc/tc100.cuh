@@ -73,6 +73,14 @@ __device__ __forceinline__ void fence_barrier_init() {
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// ---- programmatic dependent launch.  A kernel launched with the attribute may
+// start while the kernel before it in the stream ends; dependency_wait()
+// returns once that one is complete and its memory visible, and comes before
+// every access to global memory.  let_dependents() allows the kernel after
+// this one the same, from when every CTA has said so.
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Loads the tile at (x = element along the contiguous dimension, y = row).
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
