@@ -22,7 +22,7 @@ def quantize_rows(x):
     bits, ``scale = max|x| / 127`` and ``q = round(x * (127 / max|x|))`` (to
     even), both in fp32.  A row whose maximum is below 2^-100 gives zeros and
     scale 0; a row that holds an infinity or a NaN gives zeros and scale NaN,
-    so that products with it are NaN.  ``q`` [..., K] is a view of rows that
+    so that products with it are NaN.  Not differentiable.  ``q`` [..., K] is a view of rows that
     start on 16-byte boundaries, the layout the product reads in place."""
     _block.check_tensor("x", x, tuple(_block.DTYPES))
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -35,6 +35,11 @@ def quantize_rows(x):
     _block.call(x.device, _block.lib().gf_quantize_rows, v.shape[0], k, _block.DTYPES[x.dtype], v.data_ptr(),
                 _block.ld(v), q.data_ptr(), kp, scale.data_ptr())
     return q.view(*x.shape[:-1], kp)[..., :k], scale.view(x.shape[:-1])
+
+
+def _forward_only(who, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who} has no backward: call it under torch.no_grad() or on detached inputs")
 
 
 def _check_weight(b, b_scale, bias, out_dtype, device):
@@ -73,9 +78,10 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, *, out_dtype=torch.bfloat16):
     ``a`` [M, K] and ``b`` [N, K] int8 (K at most 131071, so that the integer
     sums are exact), ``a_scale`` [M] and ``b_scale`` [N] fp32, ``bias`` [N] of
     ``out_dtype`` or None.  Any row strides; rows that do not start on 16-byte
-    boundaries cost a copy."""
+    boundaries cost a copy.  Forward only."""
     _block.check_tensor("a", a, (torch.int8,))
     _block.check_tensor("a_scale", a_scale, (torch.float32,), a.device)
+    _forward_only("int8_matmul", a_scale, b_scale, bias)
     n, k = _check_weight(b, b_scale, bias, out_dtype, a.device)
     if a.dim() != 2 or a.shape[1] != k:
         raise ValueError(f"a is {tuple(a.shape)}, b {tuple(b.shape)}: expected [M, K] and [N, K]")
@@ -98,11 +104,10 @@ def int8_linear(x, q_weight, weight_scale, bias=None, *, out_dtype=None):
     """``linear(x, q_weight * weight_scale[:, None], bias)`` with ``x`` [..., K]
     (fp32, bf16 or fp16) quantised row by row as :func:`quantize_rows` does;
     ``q_weight`` [N, K] int8, ``weight_scale`` [N] fp32, ``bias`` [N] of
-    ``out_dtype``, which defaults to ``x``'s.  Forward only: refuses an ``x``
-    that needs a gradient."""
+    ``out_dtype``, which defaults to ``x``'s.  Forward only: refuses inputs
+    that need a gradient."""
     _block.check_tensor("x", x, tuple(_block.DTYPES))
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("int8_linear has no backward: call it under torch.no_grad() or on a detached input")
+    _forward_only("int8_linear", x, weight_scale, bias)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     n, k = _check_weight(q_weight, weight_scale, bias, out_dtype, x.device)
     if x.dim() < 1 or x.shape[-1] != k:

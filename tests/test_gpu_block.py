@@ -576,3 +576,71 @@ def test_refusals_on_the_gpu():
         int8_linear(x[:, 1:], q, s)
     with pytest.raises(RuntimeError, match="no backward"):
         int8_linear(x.detach().requires_grad_(), q, s)
+    with pytest.raises(RuntimeError, match="no backward"):
+        int8_linear(x, q, s, bias=torch.zeros(32, dtype=BF16, device="cuda", requires_grad=True))
+    with pytest.raises(RuntimeError, match="no backward"):
+        int8_matmul(q, s.clone().requires_grad_(), q, s)
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    t = ff_inputs(300, 64, 200, 48, BF16, True)
+    args = [t[n] for n in ("x", "w_in", "w_out", "b_in", "b_out")]
+    layer = Int8Linear.from_weight(t["w_in"])
+    want = gated_feed_forward(*args), layer(t["x"]), dropout(t["x"], 0.3, 1)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = gated_feed_forward(*args), layer(t["x"]), dropout(t["x"], 0.3, 1)
+                s.synchronize()
+                wrong.extend(i for i in range(3) if not torch.equal(got[i], want[i]))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from guass_b200.dropout import dropout
+from guass_b200.feedforward import gated_feed_forward
+from guass_b200.int8 import Int8Linear, int8_linear
+x = torch.randn(40, 64, device="cuda").bfloat16().requires_grad_()
+w = torch.randn(256, 64, device="cuda").bfloat16() * 0.1
+v = torch.randn(64, 128, device="cuda").bfloat16() * 0.1
+dy = torch.randn(40, 64, device="cuda").bfloat16()
+q = torch.randint(-127, 128, (48, 64), dtype=torch.int8, device="cuda")
+s = torch.rand(48, device="cuda")
+
+def step():
+    y = dropout(gated_feed_forward(x, w, v, dropout_p=0.1, seed=3), 0.2, 4, residual=x)
+    g, = torch.autograd.grad(y, [x], dy)
+    return y.detach(), g, int8_linear(x.detach(), q, s)
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+print("ok")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stderr[-2000:]

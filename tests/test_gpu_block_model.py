@@ -155,3 +155,21 @@ def test_8_bits_refuse_training():
         m(x)
     with torch.no_grad():
         assert m(x).shape == (3, m.out_features)
+
+
+def test_8_bits_after_merging_count_the_delta_once():
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = sd15.SD15UNet(sd15.tiny_config(), dtype=torch.bfloat16)
+    model.cuda()
+    bank = BatchedAdapters(model.adapters(), out_dtype=torch.bfloat16)
+    bank.install()
+    m = bank.modules[0]
+    bank.merge_into_weights()
+    merged = m.weight.detach().float()
+    bank.quantize_merged()
+    q, scale = ref.quantise(merged)
+    layer = bank._int8[0][2]
+    assert torch.equal(layer.q_weight.cpu(), q) and torch.equal(layer.weight_scale.cpu(), scale)
+    bank.unquantize()
+    bank.unmerge_weights()
