@@ -431,13 +431,12 @@ struct EpilogueWarp {
       if (half == 1) release();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        uint64_t keep[2];
+        uint32_t keep[2];  // of two 16-bit results: ones where they are kept (a dropped one is 0 whatever it holds)
         if constexpr (DROP) {
           const uint4 w = rng((uint32_t)(n + 16 * half + 4 * q) >> 2, (uint32_t)(m + lane));
           const uint32_t th = p.drop.threshold;
-          const float s = p.drop.scale;
-          keep[0] = tc::pack_f2(w.x >= th ? s : 0.0f, w.y >= th ? s : 0.0f);
-          keep[1] = tc::pack_f2(w.z >= th ? s : 0.0f, w.w >= th ? s : 0.0f);
+          keep[0] = (w.x >= th ? 0xFFFFu : 0u) | (w.y >= th ? 0xFFFF0000u : 0u);
+          keep[1] = (w.z >= th ? 0xFFFFu : 0u) | (w.w >= th ? 0xFFFF0000u : 0u);
         }
         const float4 b0 = *reinterpret_cast<const float4*>(vec0 + 16 * half + 4 * q);
         const float4 b1 = *reinterpret_cast<const float4*>(vec1 + 16 * half + 4 * q);
@@ -452,15 +451,19 @@ struct EpilogueWarp {
           float2 r;
           if constexpr (kBack) {
             uint64_t d = tc::pack_f2(f(dh[c]), f(dh[c + 1]));
-            if constexpr (DROP) d = tc::mul_f2(d, keep[i]);
+            if constexpr (DROP) d = tc::mul_f2(d, tc::pack_f2(p.drop.scale, p.drop.scale));
             r = tc::unpack_f2(tc::mul_f2(d, value));
             o0[o] = pack2<T>(r.x, r.y);
             r = tc::unpack_f2(tc::mul_f2(tc::mul_f2(d, x), slope));
             o1[o] = pack2<T>(r.x, r.y);
           } else {
-            if constexpr (DROP) value = tc::mul_f2(value, keep[i]);
+            if constexpr (DROP) value = tc::mul_f2(value, tc::pack_f2(p.drop.scale, p.drop.scale));
             r = tc::unpack_f2(tc::mul_f2(x, value));
             o0[o] = pack2<T>(r.x, r.y);
+          }
+          if constexpr (DROP) {
+            o0[o] &= keep[i];
+            if constexpr (kBack) o1[o] &= keep[i];
           }
         }
       }
@@ -990,14 +993,13 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
       uint64_t value, slope;
       if (p.act == GF_ACT_GELU) activate<GF_ACT_GELU, false>(g, g, value, slope);
       else activate<GF_ACT_SILU, false>(g, g, value, slope);
-      float v = tc::unpack_f2(value).x;
+      float h = a * tc::unpack_f2(value).x;
       if (p.drop.on) {
         const uint4 w = Philox(p.drop)((uint32_t)n >> 2, (uint32_t)lane);
         const uint32_t word = (n & 3) == 0 ? w.x : (n & 3) == 1 ? w.y : (n & 3) == 2 ? w.z : w.w;
-        const float keep = word >= p.drop.threshold ? p.drop.scale : 0.0f;
-        v = keep * v;
+        h = word >= p.drop.threshold ? h * p.drop.scale : 0.0f;
       }
-      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(a * v);
+      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(h);
     } else if (!live && n < p.hp && lane < p.tokens) {
       static_cast<T*>(p.out)[lane * p.ld_out + n] = T(0.0f);
     }

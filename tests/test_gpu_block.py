@@ -282,6 +282,24 @@ def test_ff_and_dropout_share_the_rule():
     assert torch.equal(d, dropout(h, 0.5, 21, site=4))  # 1 / (1 - p) = 2: no rounding
 
 
+@pytest.mark.parametrize("tokens", [6, 200])
+def test_ff_drops_whatever_was_there(tokens):
+    """One hidden unit that is infinite for every row reaches only the rows that keep it, forward and backward."""
+    t = ff_inputs(tokens, 32, 64, 40, BF16, True)
+    clean = {n: t[n].detach().clone() for n in t}
+    t["b_in"][5] = float("inf")
+    kept = ref.keep_mask(tokens, 64, 0.5, 9, 0)[:, 5].cuda()
+    assert kept.any() and not kept.all()
+    out = []
+    for v in (clean, t):
+        x = v["x"].detach().requires_grad_()
+        y = gated_feed_forward(x, v["w_in"], v["w_out"], v["b_in"], v["b_out"], dropout_p=0.5, seed=9)
+        out.append((y.detach(), torch.autograd.grad(y, [x], torch.ones_like(y))[0]))
+    for a, b in zip(*out):
+        assert torch.equal(a[~kept], b[~kept])
+    assert not torch.isfinite(out[1][0][kept]).any()
+
+
 # ---------------------------------------------------------------------------
 # 8-bit product
 
