@@ -9,7 +9,9 @@ namespace tc {
 
 // A wait that finds nothing after this many tries gives up (each try suspends
 // for up to a microsecond, so between about 0.1 s and 5 s): far beyond any
-// legitimate wait, and short enough that a kernel always ends.
+// legitimate wait, and short enough that a kernel always ends.  Suspended, the
+// waiting warps leave the issue slots to the others: polling without it made
+// the feed-forward's passes 3 to 5 % slower, a longer suspension changed nothing.
 constexpr uint32_t kWaitTries = 1u << 22;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

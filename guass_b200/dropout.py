@@ -69,4 +69,6 @@ def dropout(x, p: float, seed, *, site: int = 0, residual=None):
     if x.numel() == 0:
         _block.make_rule(p, seed, site, x.device)
         return x.clone() if residual is None else residual + x
-    return _Dropout.apply(x, residual, p, seed, site)
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
+        return _Dropout.apply(x, residual, p, seed, site)
+    return _run(x, _block.make_rule(p, seed, site, x.device), residual)
