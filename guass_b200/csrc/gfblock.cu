@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       tc::mbar_init(acc_full + 8 * i, 1);
       tc::mbar_init(acc_empty + 8 * i, C::epi_warps * (PAIR ? 2 : 1));
     }
+    tc::mbar_init(tc::smem_addr(&pipe->spare), 1);
     pipe->abort = 0;
     tc::fence_barrier_init();
     tc::fence_proxy_async();
@@ -745,12 +746,14 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
   if (threadIdx.x == 0 && *abort) atomicOr(&g_status, GF_FLAG_TIMEOUT);
   if (warp == 1) {
     tc::fence_after();
-    if (*abort && rank == 0) {  // products may still be running: their end is a commit away
+    if (*abort && rank == 0) {
+      // Products may still be running: their end is a commit away, by the lane
+      // that issued them and, as every tcgen05 instruction of a kernel, with its
+      // cta_group (a pair's commit arrives on both CTAs' barriers).
       if (tc::elect_one()) {
         volatile uint32_t ignore = 0;
         const uint32_t spare = tc::smem_addr(&pipe->spare);
-        tc::mbar_init(spare, 1);
-        tc::mma_commit<false>(spare);
+        tc::mma_commit<PAIR>(spare);
         tc::mbar_wait(spare, 0, &ignore);
       }
       __syncwarp();

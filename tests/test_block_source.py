@@ -1,0 +1,36 @@
+"""Rules of the block operators' kernels that no run can show without a fault:
+read from the source."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parent.parent / "guass_b200" / "csrc"
+SOURCE = (CSRC / "gfblock.cu").read_text()
+
+
+def body(name: str) -> str:
+    """The text of the function ``name``, from its name to its closing brace."""
+    at = re.search(r"\b" + name + r"\s*\(", SOURCE).start()
+    depth = 0
+    for i in range(SOURCE.index("{", at), len(SOURCE)):
+        depth += {"{": 1, "}": -1}.get(SOURCE[i], 0)
+        if depth == 0:
+            return SOURCE[at:i + 1]
+    raise AssertionError(name)
+
+
+def test_one_cta_group_in_a_kernel():
+    """Every tcgen05 instruction of a kernel has the same cta_group, the ones behind a wait that gave up too."""
+    used = re.findall(r"tc::(tmem_alloc|tmem_free|mma_commit|mma)<([^>;]*?)[,>]", body("gemm_kernel"))
+    assert len(used) >= 6
+    assert {group for _, group in used} == {"PAIR"}
+
+
+def test_barriers_are_initialised_before_the_fence():
+    text = body("gemm_kernel")
+    fence = text.index("fence_barrier_init")
+    inits = [m.start() for m in re.finditer("mbar_init", text)]
+    assert inits and max(inits) < fence
+    for bar in ("full", "empty", "acc_full", "acc_empty", "spare"):
+        assert re.search(r"mbar_init\([^;]*\b" + bar + r"\b", text[:fence]), bar
