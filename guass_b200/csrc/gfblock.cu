@@ -655,10 +655,16 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       }
       // The copies in flight must land before the CTA ends.  Every product
       // waits for its copies, so this matters after a wait that gave up only.
+      // The second CTA's count on the first one's barriers, where the first
+      // waits for those of the stages it has filled too; of one that the
+      // second was ahead with nobody knows, so it stays for far longer than a
+      // copy takes.
       if (!ok && rank == 0) {
         volatile uint32_t ignore = 0;
         const uint32_t from = n > (uint32_t)p.stages ? n - p.stages : 0;
         for (uint32_t i = from; i < n; ++i) tc::mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1, &ignore);
+      } else if (!ok) {
+        for (int i = 0; i < 20; ++i) __nanosleep(1000000);  // at most a millisecond each
       }
     }
   } else if (warp == 1) {

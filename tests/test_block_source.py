@@ -34,3 +34,13 @@ def test_barriers_are_initialised_before_the_fence():
     assert inits and max(inits) < fence
     for bar in ("full", "empty", "acc_full", "acc_empty", "spare"):
         assert re.search(r"mbar_init\([^;]*\b" + bar + r"\b", text[:fence]), bar
+
+
+def test_both_ctas_of_a_pair_stay_for_their_copies():
+    """A producer that gave up outlasts its copies in flight: the first CTA waits for the stages it filled, the second,
+    whose copies count on the first one's barriers, for a fixed time."""
+    text = body("gemm_kernel")
+    first = text.index("if (!ok && rank == 0) {")
+    after = text[first:text.index("warp == 1", first)]
+    assert "mbar_wait(full" in after.split("else if (!ok)")[0]
+    assert "__nanosleep" in after.split("else if (!ok)")[1]
