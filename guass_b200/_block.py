@@ -175,6 +175,22 @@ def ld(v: torch.Tensor) -> int:
     return v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
 
+class KeptSeed:
+    """A forward's seed for its backward.  A seed tensor is kept itself, not
+    through save_for_backward: under saved-tensor hooks (checkpointing,
+    offloading) that would neither keep its memory nor see that it changed."""
+
+    def __init__(self, seed):
+        self.seed = seed
+        self.version = seed._version if isinstance(seed, torch.Tensor) else None
+
+    def get(self):
+        if self.version is not None and self.seed._version != self.version:
+            raise RuntimeError("the dropout seed has been modified by an inplace operation between the forward and its "
+                               "backward")
+        return self.seed
+
+
 def make_rule(p: float, seed, site: int, device) -> GfDropoutRule:
     """``seed``: an int, or a one-element int64 CUDA tensor that the kernel reads."""
     p, site = float(p), int(site)

@@ -34,16 +34,14 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site):
         rule = _block.make_rule(p, seed, site, x.device)
-        if isinstance(seed, torch.Tensor):
-            ctx.save_for_backward(seed)  # autograd then refuses one that has changed
-        ctx.rule = rule
+        ctx.kept, ctx.p, ctx.site = _block.KeptSeed(seed), p, site
         return _run(x, rule, residual)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        ctx.saved_tensors
-        dx = _run(dy, ctx.rule, None) if ctx.needs_input_grad[0] else None
+        rule = _block.make_rule(ctx.p, ctx.kept.get(), ctx.site, dy.device)
+        dx = _run(dy, rule, None) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 

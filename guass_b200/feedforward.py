@@ -69,21 +69,21 @@ class _GatedFeedForward(torch.autograd.Function):
         need = ctx.needs_input_grad
         rule = _block.make_rule(p, seed, site, x.device)
         y, h = _forward(x, w_in, w_out, b_in, b_out, activation, rule, need[2])
-        # (a saved seed tensor: autograd refuses one that has changed)
-        ctx.save_for_backward(x, w_in, w_out, b_in, h, seed if isinstance(seed, torch.Tensor) else None)
-        ctx.activation, ctx.rule = activation, rule
+        ctx.save_for_backward(x, w_in, w_out, b_in, h)
+        ctx.activation, ctx.kept, ctx.p, ctx.site = activation, _block.KeptSeed(seed), p, site
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w_in, w_out, b_in, h, _ = ctx.saved_tensors
+        x, w_in, w_out, b_in, h = ctx.saved_tensors
         need, (out, hidden), d, shape = ctx.needs_input_grad, w_out.shape, w_in.shape[1], x.shape
         dy, x = _block.rows_of(dy, out), _block.rows_of(x, d)
         w_in, w_out = _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
         b_in = None if b_in is None else b_in.contiguous()
         L = _block.lib()
-        f = _describe(x, w_in, w_out, b_in, None, ctx.activation, ctx.rule)
+        rule = _block.make_rule(ctx.p, ctx.kept.get(), ctx.site, dy.device)
+        f = _describe(x, w_in, w_out, b_in, None, ctx.activation, rule)
         f.dy, f.ld_dy = dy.data_ptr(), _block.ld(dy)
         if h is not None:
             f.h = h.data_ptr()

@@ -1,0 +1,95 @@
+"""The block operators' autograd functions on the CPU, their launches replaced
+by recorders: what they keep for the backward and what they refuse."""
+from __future__ import annotations
+
+import ctypes
+import gc
+import weakref
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from guass_b200 import _block
+from guass_b200 import dropout as dropout_module
+from guass_b200 import feedforward as ff_module
+
+
+def seed_behind(rule) -> int:
+    return ctypes.c_int64.from_address(rule.seed_ptr).value if rule.seed_ptr else rule.seed
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Lets CPU tensors through; every launch appends (kind, seed it would read)."""
+    seen, alive = [], []
+
+    def drop(x, rule, residual):
+        assert all(ref() is not None for ref in alive), "the seed's memory is gone"
+        seen.append(("dropout", seed_behind(rule)))
+        return x * 2 if residual is None else x * 2 + residual
+
+    def forward(x, w_in, w_out, b_in, b_out, activation, rule, keep):
+        seen.append(("forward", seed_behind(rule)))
+        return x * 2, (x.clone() if keep else None)
+
+    def run(device, size_fn, fn, desc, *args, **kw):
+        assert all(ref() is not None for ref in alive), "the seed's memory is gone"
+        seen.append(("backward", seed_behind(desc.dropout)))
+
+    monkeypatch.setattr(_block, "check_tensor", lambda *a: None)
+    monkeypatch.setattr(dropout_module, "_run", drop)
+    monkeypatch.setattr(ff_module, "_forward", forward)
+    monkeypatch.setattr(_block, "run", run)
+    return seen, alive
+
+
+def operators():
+    w_in, w_out = torch.ones(16, 4), torch.ones(4, 8)
+    return {"dropout": lambda x, seed: dropout_module.dropout(x, 0.5, seed),
+            "feed_forward": lambda x, seed: ff_module.gated_feed_forward(x, w_in, w_out, dropout_p=0.5, seed=seed)}
+
+
+@pytest.mark.parametrize("op", ["dropout", "feed_forward"])
+@pytest.mark.parametrize("hooks", ["none", "checkpoint", "save_on_cpu", "clone"])
+def test_a_seed_made_on_the_way_lives_until_the_backward(launches, op, hooks):
+    seen, alive = launches
+    fn, base = operators()[op], torch.tensor([5])
+    x = torch.ones(3, 4, requires_grad=True)
+
+    def part(x):
+        seed = base + 7
+        if not alive:
+            alive.append(weakref.ref(seed))
+        return fn(x, seed)
+
+    if hooks == "checkpoint":
+        y = checkpoint(part, x, use_reentrant=False)
+    elif hooks == "save_on_cpu":
+        with torch.autograd.graph.save_on_cpu():
+            y = part(x)
+    elif hooks == "clone":  # what is packed is not the tensor itself, as when it is offloaded
+        with torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t):
+            y = part(x)
+    else:
+        y = part(x)
+    gc.collect()
+    y.sum().backward()
+    assert {seed for _, seed in seen} == {12} and len(seen) >= 2
+
+
+@pytest.mark.parametrize("op", ["dropout", "feed_forward"])
+@pytest.mark.parametrize("hooks", ["none", "checkpoint", "clone"])
+def test_a_seed_that_changed_is_refused(launches, op, hooks):
+    fn, seed = operators()[op], torch.tensor([5])
+    x = torch.ones(3, 4, requires_grad=True)
+    if hooks == "checkpoint":
+        y = checkpoint(lambda x: fn(x, seed), x, use_reentrant=False)
+    elif hooks == "clone":
+        with torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t):
+            y = fn(x, seed)
+    else:
+        y = fn(x, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
