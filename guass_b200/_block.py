@@ -5,6 +5,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from guass_b200 import _lib
 
@@ -127,6 +128,13 @@ def check_tensor(name: str, t, dtypes, device=None) -> None:
         raise RuntimeError(f"{name} is on {t.device}, the input on {device}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def refuse_tangents(who: str, *tensors) -> None:
+    """Forward-mode derivatives would be lost without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{who} has no forward-mode derivative: call it on primals")
 
 
 def call(device, fn, *args) -> None:

@@ -58,7 +58,7 @@ def dropout(x, p: float, seed, *, site: int = 0, residual=None):
     on any device, stream and layout.
 
     fp32, bf16 or fp16 with any strides; the result is contiguous.
-    Differentiable once in ``x`` and ``residual``."""
+    Differentiable once in ``x`` and ``residual``, in reverse mode."""
     _block.check_tensor("x", x, tuple(_block.DTYPES))
     if residual is not None:
         _block.check_tensor("residual", residual, (x.dtype,), x.device)
@@ -67,6 +67,7 @@ def dropout(x, p: float, seed, *, site: int = 0, residual=None):
     if x.numel() == 0:
         _block.make_rule(p, seed, site, x.device)
         return x.clone() if residual is None else residual + x
+    _block.refuse_tangents("dropout", x, residual)
     if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad):
         return _Dropout.apply(x, residual, p, seed, site)
     return _run(x, _block.make_rule(p, seed, site, x.device), residual)

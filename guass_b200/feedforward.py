@@ -136,9 +136,10 @@ def gated_feed_forward(x, w_in, w_out, b_in=None, b_out=None, *, activation: str
     on the hidden ``[rows, hidden]``; a seed tensor must not change between
     the forward and its backward.  Returns [..., out].
 
-    Differentiable once in every tensor.  Work goes to the current stream of
+    Differentiable once in every tensor, in reverse mode.  Work goes to the current stream of
     ``x``'s device; nothing synchronises, and both passes can be captured."""
     _check(x, w_in, w_out, b_in, b_out, activation)
+    _block.refuse_tangents("gated_feed_forward", x, w_in, w_out, b_in, b_out)
     if torch.is_grad_enabled() and (x.requires_grad or w_in.requires_grad or w_out.requires_grad
                                     or b_in is not None and b_in.requires_grad
                                     or b_out is not None and b_out.requires_grad):

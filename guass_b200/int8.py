@@ -40,6 +40,7 @@ def quantize_rows(x):
 def _forward_only(who, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who} has no backward: call it under torch.no_grad() or on detached inputs")
+    _block.refuse_tangents(who, *tensors)
 
 
 def _check_weight(b, b_scale, bias, out_dtype, device):

@@ -8,11 +8,13 @@ import weakref
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from guass_b200 import _block
 from guass_b200 import dropout as dropout_module
 from guass_b200 import feedforward as ff_module
+from guass_b200 import int8 as int8_module
 
 
 def seed_behind(rule) -> int:
@@ -93,3 +95,28 @@ def test_a_seed_that_changed_is_refused(launches, op, hooks):
     seed.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(launches, grad):
+    """A tangent is refused, not dropped, wherever it comes in; primals work in a dual level as outside."""
+    drop, ff = dropout_module.dropout, ff_module.gated_feed_forward
+    x, w_in, w_out, b_in, b_out = (torch.ones(*s) for s in ((3, 4), (16, 4), (4, 8), (16,), (4,)))
+    q, s = torch.ones(4, 4, dtype=torch.int8), torch.ones(4)
+    seen, _ = launches
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: drop(dual(x), 0.5, 1), lambda: drop(x, 0.5, 1, residual=dual(x)),
+                 lambda: int8_module.int8_linear(dual(x), q, s), lambda: int8_module.int8_linear(x, q, dual(s)),
+                 lambda: int8_module.int8_matmul(q, dual(s), q, s),
+                 lambda: int8_module.int8_matmul(q, s, q, s, bias=dual(b_out.bfloat16()))]
+        args = [x, w_in, w_out, b_in, b_out]
+        calls += [lambda i=i: ff(*args[:i], dual(args[i]), *args[i + 1:]) for i in range(5)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not seen
+        drop(x, 0.5, 1), ff(*args)
+    assert len(seen) == 2
