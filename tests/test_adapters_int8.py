@@ -1,0 +1,72 @@
+"""8-bit serving of merged adapters (guass_b200.adapters) on the CPU: which
+weight is quantised and whose forward serves when.  The layer is a test double
+that keeps its weight; the GPU tests cover the product."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from guass_b200 import int8
+from guass_b200.adapters import BatchedAdapters, ModelRenderer
+from oracle_batch import OracleBatch
+from test_adapters import FakeLinear
+
+
+class KeptLinear(nn.Module):
+    def __init__(self, weight, bias):
+        super().__init__()
+        self.weight, self.bias = weight.detach().clone(), bias
+
+    @classmethod
+    def from_weight(cls, weight, bias=None):
+        return cls(weight, bias)
+
+    def forward(self, x):
+        return F.linear(x, self.weight, self.bias)
+
+
+class Layer(FakeLinear):
+    def forward(self, x):
+        return F.linear(x, self.weight + self.compute_delta_weight(), self.bias)
+
+    def compute_delta_weight(self):  # without a binding: no adapter
+        return torch.zeros_like(self.weight)
+
+
+@pytest.fixture(autouse=True)
+def kept_layers(monkeypatch):
+    monkeypatch.setattr(int8, "Int8Linear", KeptLinear)
+
+
+def modules():
+    return {"a": Layer(40, 70, 6, 1, scale=0.5), "b": Layer(33, 40, 4, 3, scale=0.5)}
+
+
+def make(fused=False):
+    mods = modules()
+    bank = BatchedAdapters(mods, batch_factory=OracleBatch, out_dtype=torch.float32, fused_weight=fused)
+    base = [m.weight.detach().clone() for m in bank.modules]
+    with torch.no_grad():
+        full = [d.clone() if fused else w + d for w, d in zip(base, bank.render())]
+    bank._current = None
+    return bank, full
+
+
+def served(bank):
+    return [layer.weight for _, _, layer in bank._int8]
+
+
+@pytest.mark.parametrize("between", ["nothing", "render", "unfreeze"])
+def test_quantising_after_merging_counts_the_delta_once(between):
+    bank, full = make()
+    bank.install()
+    bank.merge_into_weights()
+    if between == "render":
+        bank.render()
+    elif between == "unfreeze":
+        bank.unfreeze()
+    bank.quantize_merged()
+    for got, m, want in zip(served(bank), bank.modules, full):
+        assert torch.equal(got, m.weight) and torch.allclose(got, want, rtol=0, atol=1e-6)
