@@ -339,7 +339,12 @@ class BatchedAdapters:
     def render(self):
         """Render every adapter's delta (autograd-connected) and return the
         list of ``[out, in]`` deltas, already multiplied by adapter_scale
-        (fused mode: the effective weights W0 + adapter_scale * delta)."""
+        (fused mode: the effective weights W0 + adapter_scale * delta).
+        Zeros after :meth:`merge_into_weights`."""
+        if getattr(self, "_merged", None):  # the base weights carry the deltas
+            if self._current is None:
+                self._current = [torch.zeros_like(dw) for dw in self._merged]
+            return self._current
         if getattr(self, "_frozen", None):
             return self._frozen
         if self._measure:

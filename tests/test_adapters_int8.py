@@ -70,3 +70,28 @@ def test_quantising_after_merging_counts_the_delta_once(between):
     bank.quantize_merged()
     for got, m, want in zip(served(bank), bank.modules, full):
         assert torch.equal(got, m.weight) and torch.allclose(got, want, rtol=0, atol=1e-6)
+
+
+@pytest.mark.parametrize("again", ["render", "hook", "unfreeze"])
+def test_merged_weights_serve_the_delta_once(again):
+    """A render after merge_into_weights (ModelRenderer renders before every forward) adds nothing."""
+    bank, full = make()
+    model = nn.ModuleDict(zip("ab", bank.modules))
+    bank.install()
+    bank.merge_into_weights()
+    if again == "hook":
+        r = ModelRenderer.__new__(ModelRenderer)
+        r.bank = bank
+        r._before_forward(model, ())
+    elif again == "unfreeze":
+        bank.unfreeze()
+        bank.render()
+    else:
+        bank.render()
+    for m, want in zip(bank.modules, full):
+        x = torch.ones(2, m.in_features)
+        assert torch.allclose(m(x), F.linear(x, want), rtol=0, atol=1e-4)
+    bank.unmerge_weights()
+    with torch.no_grad():
+        for m, d, want in zip(bank.modules, bank.render(), full):
+            assert torch.allclose(m.weight + d, want, rtol=0, atol=1e-6)
