@@ -274,6 +274,8 @@ class BatchedAdapters:
         """Inference: render once and serve the cached deltas until
         :meth:`unfreeze` (the reference re-renders every layer at every
         denoising step, scripts/sample_eval_10751.py:202-259)."""
+        if getattr(self, "_merged", None):
+            raise RuntimeError("freeze: the merged weights serve without a render; unmerge_weights() first")
         self._frozen = False
         self._frozen = [d.clone() for d in self.render()]
         self._current = self._frozen
@@ -292,6 +294,8 @@ class BatchedAdapters:
         :meth:`unmerge_weights`."""
         if self.fused:
             raise RuntimeError("merge_into_weights: the fused mode already applies W0 + delta")
+        if getattr(self, "_merged", None):
+            raise RuntimeError("merge_into_weights: the deltas are merged already")
         deltas = self.render()
         self._merged = []
         for m, d in zip(self.modules, deltas):
@@ -346,6 +350,7 @@ class BatchedAdapters:
                 self._current = [torch.zeros_like(dw) for dw in self._merged]
             return self._current
         if getattr(self, "_frozen", None):
+            self._current = self._frozen
             return self._frozen
         if self._measure:
             self.ensure_capacity()

@@ -95,3 +95,17 @@ def test_merged_weights_serve_the_delta_once(again):
     with torch.no_grad():
         for m, d, want in zip(bank.modules, bank.render(), full):
             assert torch.allclose(m.weight + d, want, rtol=0, atol=1e-6)
+
+
+def test_merging_twice_and_freezing_merged_weights_are_refused():
+    bank, full = make()
+    bank.freeze()
+    bank.merge_into_weights()
+    with pytest.raises(RuntimeError, match="already"):
+        bank.merge_into_weights()
+    with pytest.raises(RuntimeError, match="unmerge_weights"):
+        bank.freeze()
+    bank.unmerge_weights()
+    for m, d, want in zip(bank.modules, bank.render(), full):  # frozen before the merge, so frozen still
+        assert torch.equal(m.compute_delta_weight(), d) and torch.allclose(m.weight + d, want, rtol=0, atol=1e-6)
+    bank.unfreeze()
