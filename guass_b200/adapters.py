@@ -406,7 +406,9 @@ class BatchedAdapters:
         for f, m in enumerate(self.modules):
             if id(m) in self._orig:
                 continue
-            self._orig[id(m)] = (m.compute_delta_weight, m.__dict__.get("forward"))
+            # (a layer served in 8 bits keeps that forward; what is below it is what changes)
+            below = None if not self._int8 else self._int8[f]
+            self._orig[id(m)] = (m.compute_delta_weight, below[1] if below else m.__dict__.get("forward"))
             if self.fused:
                 n0, n1 = self.n_off[f], self.n_off[f + 1]
 
@@ -417,7 +419,10 @@ class BatchedAdapters:
                 def fwd(x, f=f, m=m):
                     return F.linear(x, self._slot(f), m.bias)
 
-                m.forward = fwd
+                if below:
+                    self._int8[f] = (m, fwd, below[2])
+                else:
+                    m.forward = fwd
             else:
                 def cdw(f=f):
                     return self._slot(f)

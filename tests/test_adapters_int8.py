@@ -109,3 +109,41 @@ def test_merging_twice_and_freezing_merged_weights_are_refused():
     for m, d, want in zip(bank.modules, bank.render(), full):  # frozen before the merge, so frozen still
         assert torch.equal(m.compute_delta_weight(), d) and torch.allclose(m.weight + d, want, rtol=0, atol=1e-6)
     bank.unfreeze()
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("own_forward", [False, True])
+@pytest.mark.parametrize("order", ["install first", "quantise first"])
+def test_installing_and_quantising_in_any_order(order, fused, own_forward):
+    """8 bits serve from quantize_merged until unquantize or uninstall, which leave the modules as they were."""
+    bank, full = make(fused)
+    plain = [m.forward for m in bank.modules]
+    if own_forward:  # a forward that someone else put on the module
+        for m, f in zip(bank.modules, plain):
+            m.forward = lambda x, f=f: f(x) + 1
+    before = [m.__dict__.get("forward") for m in bank.modules]
+    x = [torch.ones(2, m.in_features) for m in bank.modules]
+
+    def eight_bits():
+        return all(torch.equal(m(v), F.linear(v, w)) for m, v, w in zip(bank.modules, x, full))
+
+    if order == "install first":
+        bank.install()
+        bank.quantize_merged()
+    else:
+        bank.quantize_merged()
+        bank.install()
+    assert eight_bits()
+    bank.install()  # again: nothing changes
+    assert eight_bits()
+    bank.unquantize()
+    with torch.no_grad():
+        bank.render()
+        for m, v, w in zip(bank.modules, x, full):
+            want = F.linear(v, w) + (1 if own_forward and not fused else 0)
+            assert torch.allclose(m(v), want, rtol=0, atol=1e-4)
+    bank.quantize_merged()
+    assert eight_bits()
+    bank.uninstall()
+    assert [m.__dict__.get("forward") for m in bank.modules] == before and not bank._int8
+    assert all("compute_delta_weight" not in m.__dict__ or m.compute_delta_weight().eq(0).all() for m in bank.modules)
