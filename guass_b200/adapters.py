@@ -323,12 +323,13 @@ class BatchedAdapters:
 
         if self._int8:
             raise RuntimeError("quantize_merged: the layers are already served in 8 bits")
-        self._int8 = []
+        layers = []  # published once all are made
         # after merge_into_weights() the base weights carry the deltas already
         deltas = [None] * len(self.modules) if getattr(self, "_merged", None) else self.render()
         for m, d in zip(self.modules, deltas):
             w = m.weight.float() if d is None else d.float() if self.fused else m.weight.float() + d.float()
-            self._int8.append((m, m.__dict__.get("forward"), Int8Linear.from_weight(w, m.bias)))
+            layers.append((m, m.__dict__.get("forward"), Int8Linear.from_weight(w, m.bias)))
+        self._int8 = layers
         for m, _, layer in self._int8:
             m.forward = layer.forward
 

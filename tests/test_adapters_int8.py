@@ -147,3 +147,23 @@ def test_installing_and_quantising_in_any_order(order, fused, own_forward):
     bank.uninstall()
     assert [m.__dict__.get("forward") for m in bank.modules] == before and not bank._int8
     assert all("compute_delta_weight" not in m.__dict__ or m.compute_delta_weight().eq(0).all() for m in bank.modules)
+
+
+def test_a_layer_that_cannot_be_quantised_changes_nothing(monkeypatch):
+    bank, full = make()
+    bank.install()
+    calls = []
+
+    def from_weight(weight, bias=None):
+        calls.append(weight)
+        if len(calls) == 2:
+            raise MemoryError
+        return KeptLinear(weight, bias)
+
+    with monkeypatch.context() as m:
+        m.setattr(KeptLinear, "from_weight", from_weight)
+        with pytest.raises(MemoryError):
+            bank.quantize_merged()
+    assert not bank._int8 and not any("forward" in m.__dict__ for m in bank.modules)
+    bank.quantize_merged()
+    assert all(torch.equal(a, b) for a, b in zip(served(bank), full))
