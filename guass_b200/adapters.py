@@ -260,10 +260,12 @@ class BatchedAdapters:
         return any(int(m.mu_raw.shape[0]) != k for m, (_, _, k) in zip(self.modules, self.shapes))
 
     def rebuilt(self) -> "BatchedAdapters":
-        """A new binding for the modules' current K (keeps install state)."""
+        """A new binding for the modules' current K (keeps install state; a
+        binding that served in 8 bits has to quantise the new deltas again)."""
         fresh = BatchedAdapters(dict(zip(self.names, self.modules)), batch_factory=self._factory,
                                 out_dtype=self._out_dtype, fused_weight=self.fused,
                                 track_metadata=self.track_metadata, fast_exp=self.fast_exp)
+        self.unquantize()  # of the former K
         if self._orig:
             self.uninstall()
             fresh.install()

@@ -167,3 +167,22 @@ def test_a_layer_that_cannot_be_quantised_changes_nothing(monkeypatch):
     assert not bank._int8 and not any("forward" in m.__dict__ for m in bank.modules)
     bank.quantize_merged()
     assert all(torch.equal(a, b) for a, b in zip(served(bank), full))
+
+
+@pytest.mark.parametrize("installed", [False, True])
+def test_a_new_k_ends_serving_the_old_one(installed):
+    bank, _ = make()
+    if installed:
+        bank.install()
+    bank.quantize_merged()
+    m = bank.modules[0]
+    for name in ("mu_raw", "chol_raw", "amp"):
+        setattr(m, name, nn.Parameter(getattr(m, name).detach()[:-1]))
+    assert bank.shapes_changed()
+    fresh = bank.rebuilt()
+    assert not bank._int8 and not fresh._int8 and not any("forward" in q.__dict__ for q in bank.modules)
+    fresh.quantize_merged()
+    with torch.no_grad():
+        assert all(torch.equal(w, q.weight + d) for w, q, d in zip(served(fresh), fresh.modules, fresh.render()))
+    fresh.uninstall()
+    assert not any("forward" in q.__dict__ for q in bank.modules)
