@@ -142,6 +142,14 @@ class Int8Linear(nn.Module):
         q, scale = quantize_rows(weight)
         return cls(q, scale, None if bias is None else bias.detach().clone())
 
+    def _apply(self, fn, recurse=True):
+        """Casts (``.half()``, ``.to(torch.bfloat16)``) reach the bias alone: scales stay fp32."""
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != scale.dtype:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def forward(self, x):
         bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
         return int8_linear(x, self.q_weight, self.weight_scale, bias)

@@ -120,3 +120,14 @@ def test_forward_mode_is_refused(launches, grad):
         assert not seen
         drop(x, 0.5, 1), ff(*args)
     assert len(seen) == 2
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(),
+                                  lambda m: m.to("cpu", torch.float16)])
+def test_casting_a_model_keeps_8_bit_scales(launches, cast):
+    scale = torch.tensor([1.0 + 2.0 ** -20, 0.3])
+    layer = int8_module.Int8Linear(torch.ones(2, 16, dtype=torch.int8), scale, torch.zeros(2))
+    model = cast(torch.nn.Sequential(layer))
+    assert model[0] is layer and layer.weight_scale.dtype == torch.float32
+    assert torch.equal(layer.weight_scale, scale) and layer.q_weight.dtype == torch.int8
+    assert torch.equal(layer.state_dict()["weight_scale"], scale) and layer.bias.dtype != torch.float32
