@@ -395,9 +395,10 @@ class DataParallelTrainer:
         self.alphas_cumprod = noise_schedule(self.params[0].device)
         # optional list of (start, end) CUDA events around each step's all-reduce
         self.allreduce_events = None
-        if model.dropout_seed is not None:
+        drop = getattr(model, "dropout_seed", None)  # (not every model has dropout)
+        if drop is not None:
             rank = torch.distributed.get_rank(group) if world > 1 else 0
-            model.dropout_seed.fill_(seed + (rank << 40))
+            drop.fill_(seed + (rank << 40))
 
     def backward(self, inputs: StepInputs) -> torch.Tensor:
         """Render, forward, backward and gradient all-reduce (no optimizer step)."""
@@ -421,6 +422,7 @@ class DataParallelTrainer:
         loss = self.backward(inputs)
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
-        if self.model.dropout_seed is not None:
-            self.model.dropout_seed.add_(1)
+        drop = getattr(self.model, "dropout_seed", None)
+        if drop is not None:
+            drop.add_(1)
         return loss

@@ -1,0 +1,37 @@
+"""DataParallelTrainer and the seed of a model's dropout, on the CPU."""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from guass_b200 import sd15
+from guass_b200.adapters import BatchedAdapters
+from oracle_batch import OracleBatch
+
+
+class OtherModel(nn.Module):
+    """A model of someone else: adapters, no dropout and no seed of one."""
+
+    def __init__(self):
+        super().__init__()
+        torch.manual_seed(0)
+        self.unet = sd15.SD15UNet(sd15.tiny_config(), dtype=torch.float32)
+
+    def adapters(self):
+        return self.unet.adapters()
+
+    def forward(self, x, t, ctx):
+        return self.unet(x, t, ctx)
+
+
+def trainer(model, **kw):
+    bank = BatchedAdapters(model.adapters(), batch_factory=OracleBatch, out_dtype=torch.float32)
+    bank.install()
+    return sd15.DataParallelTrainer(model, bank, **kw)
+
+
+def test_any_model_with_adapters_trains():
+    tr = trainer(OtherModel())
+    before = tr.params[0].detach().clone()
+    loss = tr.step(sd15.synthetic_inputs(sd15.tiny_config(), 1, 3, dtype=torch.float32))
+    assert torch.isfinite(loss) and not torch.equal(tr.params[0], before)
