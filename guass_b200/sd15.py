@@ -383,7 +383,9 @@ class DataParallelTrainer:
 
     A model with dropout draws new masks each step: its seed starts at
     ``seed`` (offset by the rank, so that ranks drop independently) and is
-    advanced on the device after every :meth:`step`."""
+    advanced on the device after every :meth:`step`.  It is no part of any
+    state dict: a run that resumes after n steps passes ``seed + n``, or its
+    masks repeat."""
 
     def __init__(self, model: SD15UNet, bank, lr: float = 1e-4, world: int = 1, group=None, seed: int = 0):
         from guass_b200.adapters import adapter_parameters

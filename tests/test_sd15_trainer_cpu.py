@@ -35,3 +35,28 @@ def test_any_model_with_adapters_trains():
     before = tr.params[0].detach().clone()
     loss = tr.step(sd15.synthetic_inputs(sd15.tiny_config(), 1, 3, dtype=torch.float32))
     assert torch.isfinite(loss) and not torch.equal(tr.params[0], before)
+
+
+def test_a_resumed_run_goes_on_with_its_masks(monkeypatch):
+    """seed + n draws after a resume what the run would have drawn from step n on."""
+    seeds = []
+
+    def dropout(x, p, seed, *, site=0, residual=None):
+        seeds.append((int(seed), site))
+        return x if residual is None else residual + x
+
+    monkeypatch.setattr(sd15, "dropout", dropout)
+
+    def run(start, steps):
+        cfg = sd15.tiny_config()
+        cfg.dropout = 0.1
+        torch.manual_seed(0)
+        tr = trainer(sd15.SD15UNet(cfg, dtype=torch.float32), seed=start)
+        seeds.clear()
+        for _ in range(steps):
+            tr.step(sd15.synthetic_inputs(cfg, 1, 3, dtype=torch.float32))
+        return list(seeds)
+
+    whole = run(7, 3)
+    assert len(set(whole)) == len(whole)  # no mask twice
+    assert whole[2 * len(whole) // 3:] == run(7 + 2, 1)
