@@ -762,7 +762,7 @@ def train_arm(a, rank: int, world: int, local: int) -> None:
     """cfg4: one step = render every delta (batched), UNet forward + epsilon
     MSE, backward (batched render backward), one flat NCCL all-reduce of the
     Gaussian-parameter gradients, AdamW.  Weak scaling: a fixed batch per GPU."""
-    from guass_b200 import _lib, sd15
+    from guass_b200 import _block, _lib, sd15
     from guass_b200.adapters import BatchedAdapters
     from guass_b200.partition import field_costs
 
@@ -854,6 +854,7 @@ def train_arm(a, rank: int, world: int, local: int) -> None:
     tr.allreduce_events = None
     clocks = sampler.stop() if sampler else None
     assert torch.isfinite(loss).item()
+    assert _block.device_flags() == 0
 
     # end to end: this step's inputs copied from pinned host memory, the loss read back, every step
     d_in = inp.tensors()

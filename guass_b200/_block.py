@@ -17,7 +17,7 @@ DTYPES = {torch.float32: _lib.GF_F32, torch.bfloat16: _lib.GF_BF16, torch.float1
 # Every symbol include/gfblock.h declares.
 EXPORTED = ("gf_gated_ff_workspace_bytes", "gf_gated_ff_forward", "gf_gated_ff_backward", "gf_dropout",
             "gf_quantize_rows", "gf_int8_product_workspace_bytes", "gf_int8_matmul",
-            "gf_int8_linear_workspace_bytes", "gf_int8_linear", "gf_block_status")
+            "gf_int8_linear_workspace_bytes", "gf_int8_linear", "gf_block_status", "gf_block_status_async")
 
 
 class GfDropoutRule(ctypes.Structure):
@@ -102,6 +102,8 @@ def lib() -> ctypes.CDLL:
     L.gf_int8_linear.restype = ctypes.c_int
     L.gf_block_status.argtypes = [ptr, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
     L.gf_block_status.restype = ctypes.c_int
+    L.gf_block_status_async.argtypes = [ptr, ptr]
+    L.gf_block_status_async.restype = ctypes.c_int
     _ready = L
     return L
 
@@ -114,6 +116,25 @@ def device_flags(device="cuda", reset: bool = False) -> int:
     with torch.cuda.device(device):
         _lib.check(lib().gf_block_status(torch.cuda.current_stream().cuda_stream, int(reset), ctypes.byref(flags)))
     return flags.value
+
+
+class FlagWatch:
+    """The condition bits of a device for a loop that does not synchronise:
+    :meth:`look` enqueues a copy of them behind the work so far, :meth:`check`
+    raises once a copy that has arrived shows one.  (The bits stay set until
+    they are reset, so whichever copy arrived last shows them.)"""
+
+    def __init__(self, device: torch.device):
+        self.device = device
+        self.flags = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+
+    def look(self) -> None:
+        call(self.device, lib().gf_block_status_async, self.flags.data_ptr())
+
+    def check(self) -> None:
+        if self.flags[0] != 0:
+            raise RuntimeError(f"a block operator gave up waiting for its own copies or products (condition bits "
+                               f"{int(self.flags[0]):#x}): what it computed is not valid")
 
 
 def check_tensor(name: str, t, dtypes, device=None) -> None:

@@ -33,7 +33,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from guass_b200 import synthetic
+from guass_b200 import _block, synthetic
 from guass_b200.dropout import dropout
 from guass_b200.feedforward import gated_feed_forward
 
@@ -379,7 +379,8 @@ class DataParallelTrainer:
     forward + epsilon MSE, backward (the renderer's batched backward gives the
     Gaussian-parameter gradients), one flat all-reduce of those gradients
     averaged over the ranks (:func:`guass_b200.adapters.allreduce_adapter_grads`),
-    AdamW step.  Returns the detached loss.
+    AdamW step.  Returns the detached loss.  Raises when a kernel of an
+    earlier step reported that its results are not valid.
 
     A model with dropout draws new masks each step: its seed starts at
     ``seed`` (offset by the rank, so that ranks drop independently) and is
@@ -397,6 +398,9 @@ class DataParallelTrainer:
         self.alphas_cumprod = noise_schedule(self.params[0].device)
         # optional list of (start, end) CUDA events around each step's all-reduce
         self.allreduce_events = None
+        # the fused feed-forward's condition bits, looked at without waiting for the device
+        fused = any(getattr(m, "fused_ff", False) for m in model.modules())
+        self._flags = _block.FlagWatch(self.params[0].device) if fused and self.params[0].is_cuda else None
         drop = getattr(model, "dropout_seed", None)  # (not every model has dropout)
         if drop is not None:
             rank = torch.distributed.get_rank(group) if world > 1 else 0
@@ -421,7 +425,11 @@ class DataParallelTrainer:
         return loss.detach()
 
     def step(self, inputs: StepInputs) -> torch.Tensor:
+        if self._flags is not None:
+            self._flags.check()
         loss = self.backward(inputs)
+        if self._flags is not None:
+            self._flags.look()
         self.opt.step()
         self.opt.zero_grad(set_to_none=True)
         drop = getattr(self.model, "dropout_seed", None)

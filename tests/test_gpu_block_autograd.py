@@ -72,3 +72,30 @@ def test_a_changed_seed_is_refused_under_hooks(hooks):
         seed.add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+def test_flag_watch_and_trainer_on_the_gpu():
+    """A training step with the fused feed-forward looks at the flags without finding one; the copy is asynchronous."""
+    from guass_b200 import sd15
+    from guass_b200.adapters import BatchedAdapters
+
+    cfg = sd15.tiny_config()
+    cfg.feed_forward = "kernel"
+    torch.manual_seed(0)
+    with torch.device("cuda"):
+        model = sd15.SD15UNet(cfg, dtype=torch.bfloat16)
+    model.cuda()
+    bank = BatchedAdapters(model.adapters(), out_dtype=torch.bfloat16)
+    bank.install()
+    tr = sd15.DataParallelTrainer(model, bank)
+    inp = sd15.synthetic_inputs(cfg, 2, 1, device="cuda")
+    tr._flags.flags.fill_(-1)  # overwritten by a copy of the device's zero
+    tr._flags.look()
+    torch.cuda.synchronize()
+    assert tr._flags.flags.item() == 0
+    for _ in range(3):
+        assert torch.isfinite(tr.step(inp)).item()
+    assert _block.device_flags() == 0
+    tr._flags.flags.fill_(_block.GF_FLAG_TIMEOUT)
+    with pytest.raises(RuntimeError, match="not valid"):
+        tr.step(inp)

@@ -1,6 +1,9 @@
 """DataParallelTrainer and the seed of a model's dropout, on the CPU."""
 from __future__ import annotations
 
+import ctypes
+
+import pytest
 import torch
 from torch import nn
 
@@ -60,3 +63,31 @@ def test_a_resumed_run_goes_on_with_its_masks(monkeypatch):
     whole = run(7, 3)
     assert len(set(whole)) == len(whole)  # no mask twice
     assert whole[2 * len(whole) // 3:] == run(7 + 2, 1)
+
+
+def test_a_wait_that_ran_out_stops_the_training(monkeypatch):
+    """The fused feed-forward's condition bits, copied behind a step, end the next one."""
+    from guass_b200 import _block
+
+    class Library:  # sets what the device would have set during the second step
+        calls = 0
+
+        def gf_block_status_async(self, pointer, stream):
+            Library.calls += 1
+            ctypes.c_uint32.from_address(pointer).value = _block.GF_FLAG_TIMEOUT if Library.calls == 2 else 0
+            return 0
+
+    plain = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, pin_memory=False, **kw: plain(*a, **kw))
+    monkeypatch.setattr(_block, "lib", Library)
+    monkeypatch.setattr(_block, "call", lambda device, fn, *args: fn(*args, None))
+    model = OtherModel()
+    tr = trainer(model)
+    assert tr._flags is None  # composed feed-forwards, and no GPU
+    tr._flags = _block.FlagWatch(torch.device("cpu"))
+    inputs = sd15.synthetic_inputs(sd15.tiny_config(), 1, 3, dtype=torch.float32)
+    tr.step(inputs)
+    tr.step(inputs)
+    with pytest.raises(RuntimeError, match="0x10"):
+        tr.step(inputs)
+    assert Library.calls == 2
