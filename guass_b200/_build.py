@@ -28,8 +28,6 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
     "-Xptxas", "-warn-spills",
 ]
-# sources whose debug build differs (GF_CHECK); the others share one object
-CHECKED = {"gfield.cu"}
 OBJECTS = PKG / "build"
 
 
@@ -49,7 +47,7 @@ def needs_build(lib: Path = LIB) -> bool:
 
 
 def _object(src: Path, check: bool) -> Path:
-    return OBJECTS / (src.stem + ("_check.o" if check and src.name in CHECKED else ".o"))
+    return OBJECTS / (src.stem + ("_check.o" if check else ".o"))
 
 
 def build(force: bool = False, verbose: bool = False, check: bool = False) -> Path:
@@ -64,7 +62,7 @@ def build(force: bool = False, verbose: bool = False, check: bool = False) -> Pa
         obj = _object(src, check)
         if force or _newer(obj, [src, *HEADERS]):
             tmp = obj.with_suffix(".tmp.o")
-            cmd = [nvcc(), *NVCC_FLAGS, *(["-DGF_CHECK"] if check and src.name in CHECKED else []),
+            cmd = [nvcc(), *NVCC_FLAGS, *(["-DGF_CHECK"] if check else []),
                    f"-I{ROOT / 'include'}", "-c", str(src), "-o", str(tmp)]
             if verbose:
                 print(" ".join(cmd), file=sys.stderr)

@@ -35,7 +35,24 @@ constexpr I round_up(I v, I m) {
 }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-__device__ uint32_t g_status;  // GF_FLAG_TIMEOUT, sticky (gf_block_status)
+__device__ uint32_t g_status;  // GF_FLAG_*, sticky (gf_block_status)
+
+// Bounds checks of the debug build (-DGF_CHECK, libgfield_check.so): every
+// access to global memory by an address of its own (TMA copies are clipped by
+// their tensor maps) is tested against its extent; a failure sets
+// GF_FLAG_BOUNDS and the access is skipped (never a trap).  In the release
+// build the check is the constant true and compiles away.
+#ifdef GF_CHECK
+__device__ __forceinline__ bool bounds_ok(bool ok) {
+  if (!ok) atomicOr(&g_status, GF_FLAG_BOUNDS);
+  return ok;
+}
+#define GFB_IN_BOUNDS(cond) gfb::bounds_ok(cond)
+#else
+#define GFB_IN_BOUNDS(cond) ((void)sizeof(cond), true)  // unevaluated: names its operands, costs nothing
+#endif
+// v in [0, n), and the `count` elements from v within n
+__device__ __forceinline__ bool within(int64_t v, int64_t n, int64_t count = 1) { return v >= 0 && v + count <= n; }
 
 // ---------------------------------------------------------------------------
 // element types
@@ -320,6 +337,7 @@ struct EpilogueWarp {
     x.a = x.b = 0.0f;
     if (lane < p.N - n) {
       const T* bias = static_cast<const T*>(p.bias);
+      if (!GFB_IN_BOUNDS(within(n + lane, p.N))) return;
       if (bias) x.a = to_float(bias[n + lane]);
       if ((EPI == EPI_GATED || EPI == EPI_GATED_BWD) && bias) x.b = to_float(bias[p.N + n + lane]);
       if (EPI == EPI_INT8) x.b = p.b_scale[n + lane];
@@ -543,7 +561,7 @@ struct EpilogueWarp {
       char* dst = static_cast<char*>(p.out) + ES * (row * p.ld_out + at);
       for (int i = lane; i < 32 * per_row; i += 32) {
         const int r = i / per_row, c = i % per_row, b = c * ES;
-        if (r < rows && c < cols) {
+        if (r < rows && c < cols && GFB_IN_BOUNDS(within(row + r, p.seg_pad ? 2 * (int64_t)p.seg : p.M) && within(at + c, p.N))) {
           const char* src = stage + k * kRowsBytes + r * 64 + (((b >> 4) ^ ((r >> 1) & 3)) << 4) + (b & 15);
           if constexpr (ES == 2)
             *reinterpret_cast<uint16_t*>(dst + ES * (r * p.ld_out + c)) = *reinterpret_cast<const uint16_t*>(src);
@@ -723,7 +741,10 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
       const uint32_t acc = lanes + (EPI == EPI_GATED_BWD ? 0 : buf * kMaxN), acc2 = lanes + kMaxN + buf * (kMaxN / 2);
       int c = 32 * set;
-      if (EPI == EPI_INT8) epi.row_scale = m + (int)(threadIdx.x & 31) < p.M ? p.a_scale[m + (threadIdx.x & 31)] : 0.0f;
+      if (EPI == EPI_INT8) {
+        const int row = m + (int)(threadIdx.x & 31);
+        epi.row_scale = row < p.M && GFB_IN_BOUNDS(within(row, p.M)) ? p.a_scale[row] : 0.0f;
+      }
       typename decltype(epi)::Ahead ahead;
       if (c < c_end) epi.fetch(ahead, t.n0 + c);
       if (!__all_sync(0xFFFFFFFFu, tc::mbar_wait(acc_full + 8 * buf, (it >> 1) & 1, abort))) break;
@@ -789,9 +810,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
     }
     float4 s = make_float4(0, 0, 0, 0);
     for (int k = 0; k < p.splits; ++k) {
+      if (!GFB_IN_BOUNDS(within(m, p.rows_m) && within(n, p.ld_partial, 4))) continue;
       const float4 v = *reinterpret_cast<const float4*>(p.partial + ((int64_t)k * p.rows_m + m) * p.ld_partial + n);
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
+    if (!GFB_IN_BOUNDS(within(row, p.seg_pad ? 2 * (int64_t)p.seg : p.M) && within(n, p.N))) continue;
     const float f[4] = {s.x, s.y, s.z, s.w};
     T* out = static_cast<T*>(p.out) + row * p.ld_out + n;
     const T* bias = static_cast<const T*>(p.bias);
@@ -833,14 +856,15 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant_
   const int64_t r0 = (int64_t)blockIdx.y * j.run, r1 = min((int64_t)j.rows, r0 + j.run);
   float s = 0.0f;
   if (c < j.cols)
-    for (int64_t r = r0 + w; r < r1; r += 8) s += to_float(src[r * j.ld + c]);
+    for (int64_t r = r0 + w; r < r1; r += 8)
+      if (GFB_IN_BOUNDS(within(r, j.rows) && within(c, j.cols))) s += to_float(src[r * j.ld + c]);
   __shared__ float sums[8][32];
   sums[w][threadIdx.x % 32] = s;
   __syncthreads();
   if (w == 0 && c < j.cols) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) s += sums[i][threadIdx.x];
-    j.partial[(int64_t)blockIdx.y * j.cols + c] = s;
+    if (GFB_IN_BOUNDS(within(blockIdx.y, j.parts) && within(c, j.cols))) j.partial[(int64_t)blockIdx.y * j.cols + c] = s;
   }
 }
 template <typename T>
@@ -852,6 +876,7 @@ __global__ void __launch_bounds__(256) column_join_kernel(const __grid_constant_
   if (i >= (j.seg_pad ? 2 * j.seg : j.cols)) return;
   const int c = j.seg_pad && i >= j.seg ? j.seg_pad + i - j.seg : i;
   float s = 0.0f;
+  if (!GFB_IN_BOUNDS(within(c, j.cols))) return;
   for (int k = 0; k < j.parts; ++k) s += j.partial[(int64_t)k * j.cols + c];
   static_cast<T*>(j.out)[i] = from_float<T>(s);
 }
@@ -888,6 +913,7 @@ __global__ void __launch_bounds__(256) align_kernel(const __grid_constant__ Alig
     const E* src = static_cast<const E*>(j.src) + from * j.ld;
     E* dst = static_cast<E*>(j.dst) + r * j.ld_dst;
     const int cols = from < j.src_rows ? j.cols : 0;
+    if (!GFB_IN_BOUNDS(within(r, j.dst_rows) && (cols == 0 || (within(from, j.src_rows) && cols <= j.ld)))) continue;
     for (int c = lane; c < j.ld_dst; c += 32) dst[c] = c < cols ? src[c] : E(0);
   }
 }
@@ -932,13 +958,16 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
       if (c >= len) continue;
       uint4 v = make_uint4(0, 0, 0, 0);
       const T* src = static_cast<const T*>(p.x) + m * p.ld_x + k0 + c;
-      if (m < p.tokens && c + 8 <= len) v = *reinterpret_cast<const uint4*>(src);
+      if (m < p.tokens && c + 8 <= len && GFB_IN_BOUNDS(within(m, p.tokens) && within(k0 + c, p.k, 8)))
+        v = *reinterpret_cast<const uint4*>(src);
       *reinterpret_cast<uint4*>(&xs[m][c]) = v;
       if (m < p.tokens && c + 8 > len)
-        for (int j = 0; c + j < len; ++j) xs[m][c + j] = src[j];
+        for (int j = 0; c + j < len; ++j)
+          if (GFB_IN_BOUNDS(within(k0 + c + j, p.k))) xs[m][c + j] = src[j];
     }
     __syncthreads();
     if (!live) continue;
+    if (!GFB_IN_BOUNDS(within(n, p.n) && (kRows == 1 || p.gate_row == p.n))) continue;
     const T* w = static_cast<const T*>(p.w) + n * p.ld_w + k0;
     auto add = [&](const uint4 (&v)[kRows], int c) {
 #pragma unroll
@@ -964,7 +993,10 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) v[i][r] = *reinterpret_cast<const uint4*>(w + r * p.gate_row * p.ld_w + c + i * kStep);
+        for (int r = 0; r < kRows; ++r)
+          v[i][r] = GFB_IN_BOUNDS(within(k0 + c + i * kStep, p.k, 8))
+                        ? *reinterpret_cast<const uint4*>(w + r * p.gate_row * p.ld_w + c + i * kStep)
+                        : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) add(v[i], c + i * kStep);
     }
@@ -974,10 +1006,10 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
       for (int r = 0; r < kRows; ++r) {
         const T* at = w + r * p.gate_row * p.ld_w + c;
         if (c < whole) {
-          v[r] = *reinterpret_cast<const uint4*>(at);
+          v[r] = GFB_IN_BOUNDS(within(k0 + c, p.k, 8)) ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
         } else {  // the row's last few: what follows is not its own
           T tail[8];
-          for (int j = 0; j < 8; ++j) tail[j] = c + j < len ? at[j] : T(0.0f);
+          for (int j = 0; j < 8; ++j) tail[j] = c + j < len && GFB_IN_BOUNDS(within(k0 + c + j, p.k)) ? at[j] : T(0.0f);
           v[r] = *reinterpret_cast<const uint4*>(tail);
         }
       }
@@ -1008,9 +1040,9 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
         const uint32_t word = (n & 3) == 0 ? w.x : (n & 3) == 1 ? w.y : (n & 3) == 2 ? w.z : w.w;
         h = word >= p.drop.threshold ? h * p.drop.scale : 0.0f;
       }
-      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(h);
+      if (GFB_IN_BOUNDS(within(n, p.ld_out))) static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(h);
     } else if (!live && n < p.hp && lane < p.tokens) {
-      static_cast<T*>(p.out)[lane * p.ld_out + n] = T(0.0f);
+      if (GFB_IN_BOUNDS(within(n, p.ld_out))) static_cast<T*>(p.out)[lane * p.ld_out + n] = T(0.0f);
     }
   } else {
     float y = 0.0f;
@@ -1023,7 +1055,7 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
       y = bias ? to_float(bias[n]) : 0.0f;
 #pragma unroll
       for (int i = 0; i < kShare; ++i) y += part[warp + i][lane];
-      static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(y);
+      if (GFB_IN_BOUNDS(within(n, p.n))) static_cast<T*>(p.out)[lane * p.ld_out + n] = from_float<T>(y);
     }
   }
 }
@@ -1067,7 +1099,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
     for (int u = 0; u < U; ++u) {
       live[u] = o < outer;
       const int64_t row = rows[u] = ROWS ? i : o, col = cols[u] = (int64_t)(ROWS ? o : i) * V;
-      if (live[u]) {
+      if (live[u] && GFB_IN_BOUNDS(within(row, p.rows) && within(col, p.cols, VEC ? V : 1))) {
         const T* x = static_cast<const T*>(p.x) + row * p.x_rs + col * p.x_cs;
         const T* res = static_cast<const T*>(p.res) + row * p.r_rs + col * p.r_cs;
         if constexpr (VEC) {
@@ -1101,6 +1133,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
           out[4 * b + j] = from_float<T>(v);
         }
       }
+      if (!GFB_IN_BOUNDS(within(rows[u], p.rows) && within(cols[u], p.cols, VEC ? V : 1))) continue;
       T* y = static_cast<T*>(p.y) + rows[u] * p.cols + cols[u];
       if constexpr (VEC) {
         *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(out);
@@ -1152,15 +1185,17 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
           const int c = 8 * (t + i * TPR);
 #pragma unroll
           for (int k = 0; k < (int)sizeof(T) / 2; ++k)
-            reinterpret_cast<uint4*>(held[i])[k] =
-                c < cols ? reinterpret_cast<const uint4*>(row + c)[k] : make_uint4(0, 0, 0, 0);
+            reinterpret_cast<uint4*>(held[i])[k] = c < cols && GFB_IN_BOUNDS(within(r, rows) && within(c, cols, 8))
+                                                       ? reinterpret_cast<const uint4*>(row + c)[k]
+                                                       : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
 #pragma unroll
           for (int j = 0; j < 8; ++j) see(to_float(held[i][j]));
       } else {
-        for (int c = t; c < cols; c += TPR) see(to_float(row[c]));
+        for (int c = t; c < cols; c += TPR)
+          if (GFB_IN_BOUNDS(within(r, rows) && within(c, cols))) see(to_float(row[c]));
       }
     }
     top = __reduce_max_sync(0xFFFFFFFFu, top);
@@ -1172,7 +1207,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
       for (int i = 0; i < 8; ++i) top = max(top, warp_max[i]);
       __syncthreads();
     }
-    if (!live) continue;
+    if (!live || !GFB_IN_BOUNDS(within(r, rows))) continue;
     const float most = __uint_as_float(top);
     float s = __fdiv_rn(most, 127.0f), inv = __fdiv_rn(127.0f, most);
     uint32_t mask = 0xFFFFFFFFu;
@@ -1190,7 +1225,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(int64_t rows, int co
         auto join = [](uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3) {
           return __byte_perm(__byte_perm(b0, b1, 0x0040), __byte_perm(b2, b3, 0x0040), 0x5410);
         };
-        if (c < cols)
+        if (c < cols && GFB_IN_BOUNDS(within(c, ld_q, 8)))
           *reinterpret_cast<uint2*>(out + c) = make_uint2(join(b[0], b[1], b[2], b[3]) & mask, join(b[4], b[5], b[6], b[7]) & mask);
       }
       for (int64_t c = cols + t; c < ld_q; c += TPR) out[c] = 0;

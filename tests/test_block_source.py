@@ -10,8 +10,8 @@ SOURCE = (CSRC / "gfblock.cu").read_text()
 
 
 def body(name: str) -> str:
-    """The text of the function ``name``, from its name to its closing brace."""
-    at = re.search(r"\b" + name + r"\s*\(", SOURCE).start()
+    """The text of the void function ``name``, from its name to its closing brace."""
+    at = re.search(r"(?:void|\)) " + name + r"\(", SOURCE).start()
     depth = 0
     for i in range(SOURCE.index("{", at), len(SOURCE)):
         depth += {"{": 1, "}": -1}.get(SOURCE[i], 0)
@@ -44,3 +44,17 @@ def test_both_ctas_of_a_pair_stay_for_their_copies():
     after = text[first:text.index("warp == 1", first)]
     assert "mbar_wait(full" in after.split("else if (!ok)")[0]
     assert "__nanosleep" in after.split("else if (!ok)")[1]
+
+
+def test_the_checked_build_checks_every_source():
+    from guass_b200 import _build
+
+    for src in _build.SOURCES:
+        assert _build._object(src, True) != _build._object(src, False)
+        assert "GF_CHECK" in src.read_text()
+
+
+def test_kernels_that_address_memory_themselves_check_their_bounds():
+    for kernel in ("join_kernel", "column_sums_kernel", "column_join_kernel", "align_kernel", "skinny_kernel",
+                   "dropout_kernel", "quantize_rows_kernel", "result", "fetch", "gemm_kernel"):
+        assert "GFB_IN_BOUNDS" in body(kernel), kernel
