@@ -993,7 +993,8 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
         }
       }
     };
-    constexpr int kStep = 256 * kShare, kAhead = 4;  // loads in flight
+    constexpr int kStep = 256 * kShare, kAhead = GATED ? 4 : 2;  // loads in flight
+    static_assert(kAhead * kStep <= kChunk, "the pipelined loop has to fit the chunk, or no lane enters it");
     const int whole = len & ~7;
     int c = 8 * (lane + 32 * (warp % kShare));
     for (; c + (kAhead - 1) * kStep < whole; c += kAhead * kStep) {
