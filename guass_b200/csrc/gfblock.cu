@@ -931,8 +931,16 @@ __global__ void __launch_bounds__(256) align_kernel(const __grid_constant__ Alig
 // takes a column of h (both its rows of w_in) or of y, four warps sharing a
 // long row; each lane holds 16 bytes of the row at a time against the tokens'
 // same columns in shared memory.  Rows are 16-byte aligned.
+//
+// Up to four tokens: every further one adds its arithmetic on all weights,
+// while the product kernel takes the same time for one token as for 128.
+// Whole forward from cold caches, us, walk / product kernel:
+//   tokens            1             4             5             8
+//   320 x 1280    6.1 / 12.3    9.0 / 12.7   11.6 / 12.7   13.3 / 12.6
+//   640 x 2560    8.2 / 15.2   12.6 / 15.7   16.7 / 15.5   19.3 / 15.5
+//   1280 x 5120  13.1 / 24.3   23.6 / 23.4   36.9 / 23.6   42.1 / 23.1
 
-constexpr int kSkinnyTokens = 8;
+constexpr int kSkinnyTokens = 4;
 constexpr int kSkinnyWarps = 8;
 
 struct SkinnyParams {
@@ -1691,9 +1699,7 @@ gf_status skinny(const SkinnyParams& p, cudaStream_t st) {
   // (gated: a warp per column of h, padding included; else four per column of y)
   const int cols = GATED ? p.hp : p.n, per = GATED ? kSkinnyWarps : kSkinnyWarps / 4;
   const int grid = (int)ceil_div(cols, per);
-  const auto kernel = p.tokens == 1   ? skinny_kernel<T, 1, GATED>
-                      : p.tokens <= 4 ? skinny_kernel<T, 4, GATED>
-                                      : skinny_kernel<T, kSkinnyTokens, GATED>;
+  const auto kernel = p.tokens == 1 ? skinny_kernel<T, 1, GATED> : skinny_kernel<T, kSkinnyTokens, GATED>;
   GFB_CUDA(launch(kernel, dim3(grid), 32 * kSkinnyWarps, st, p));
   return GF_OK;
 }

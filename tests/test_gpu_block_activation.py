@@ -27,7 +27,7 @@ def gates(dtype, low, high, rows):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("act", ["gelu", "silu"])
-@pytest.mark.parametrize("rows", [8, 300])  # the walk over the weights, and the product kernel
+@pytest.mark.parametrize("rows", [4, 8, 300])  # the walk over the weights, and the product kernel
 @pytest.mark.parametrize("low,high", [(-13, -3), (-8, -3), (-3, 3), (3, 13)])
 def test_activation_and_slope(low, high, rows, act, dtype):
     x = gates(dtype, low, high, rows).cuda().requires_grad_()
