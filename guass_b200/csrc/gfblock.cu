@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ GemmP
     const float f[4] = {s.x, s.y, s.z, s.w};
     T* out = static_cast<T*>(p.out) + row * p.ld_out + n;
     const T* bias = static_cast<const T*>(p.bias);
-    T r[4];
+    __align__(8) T r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = from_float<T>(f[j] + (bias && n + j < p.N ? to_float(bias[n + j]) : 0.0f));
     if (p.N % 8 == 0 && p.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0) {
@@ -1025,7 +1025,7 @@ __global__ void __launch_bounds__(32 * kSkinnyWarps) skinny_kernel(const __grid_
         if (c < whole) {
           v[r] = GFB_IN_BOUNDS(within(k0 + c, p.k, 8)) ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
         } else {  // the row's last few: what follows is not its own
-          T tail[8];
+          __align__(16) T tail[8];
           for (int j = 0; j < 8; ++j) tail[j] = c + j < len && GFB_IN_BOUNDS(within(k0 + c + j, p.k)) ? at[j] : T(0.0f);
           v[r] = *reinterpret_cast<const uint4*>(tail);
         }
@@ -1109,7 +1109,8 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
   I o = i / inner;
   i -= o * inner;
   while (o < outer) {
-    T in[U][V], add[U][V];
+    __align__(16) T in[U][V];
+    __align__(16) T add[U][V];
     int64_t rows[U], cols[U];
     bool live[U];
 #pragma unroll
@@ -1138,7 +1139,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ Dr
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!live[u]) continue;
-      T out[V];
+      __align__(16) T out[V];
 #pragma unroll
       for (int b = 0; b < V / 4; ++b) {
         const uint4 w = rng((uint32_t)(cols[u] / 4 + b), (uint64_t)rows[u]);

@@ -58,3 +58,13 @@ def test_kernels_that_address_memory_themselves_check_their_bounds():
     for kernel in ("join_kernel", "column_sums_kernel", "column_join_kernel", "align_kernel", "skinny_kernel",
                    "dropout_kernel", "quantize_rows_kernel", "result", "fetch", "gemm_kernel"):
         assert "GFB_IN_BOUNDS" in body(kernel), kernel
+
+
+def test_local_arrays_that_move_as_wide_words_are_aligned():
+    """An array of 16-bit elements is 2-byte aligned by itself; a wide access to one in local memory would fault."""
+    names = set(re.findall(r"reinterpret_cast<(?:const )?(?:uint|float)[24]\*>\(&?(\w+)[\[)]", SOURCE))
+    local = {n for n in names if re.search(r"^\s+(?:\S+ )*T " + n + r"\[", SOURCE, flags=re.M)}
+    assert {"r", "tail", "in", "add", "out", "held", "xs"} <= local
+    for n in local:
+        for line in re.findall(r"^.*\bT " + n + r"\[.*$", SOURCE, flags=re.M):
+            assert "__align__" in line, line
