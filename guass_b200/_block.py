@@ -204,20 +204,26 @@ def ld(v: torch.Tensor) -> int:
     return v.stride(0) if v.shape[0] > 1 else v.shape[1]
 
 
-class KeptSeed:
-    """A forward's seed for its backward.  A seed tensor is kept itself, not
-    through save_for_backward: under saved-tensor hooks (checkpointing,
-    offloading) that would neither keep its memory nor see that it changed."""
+class KeptRule:
+    """A forward's dropout rule for its backward.  A seed tensor is kept
+    itself, not through save_for_backward: under saved-tensor hooks
+    (checkpointing, offloading) that would neither keep its memory nor see
+    that it changed."""
 
-    def __init__(self, seed):
-        self.seed = seed
-        self.version = seed._version if isinstance(seed, torch.Tensor) else None
+    __slots__ = ("rule", "seed", "version")
 
-    def get(self):
-        if self.version is not None and self.seed._version != self.version:
-            raise RuntimeError("the dropout seed has been modified by an inplace operation between the forward and its "
-                               "backward")
-        return self.seed
+    def __init__(self, rule: GfDropoutRule, seed):
+        self.rule, self.seed = rule, seed if isinstance(seed, torch.Tensor) else None
+        self.version = None if self.seed is None else seed._version
+
+    def get(self, device) -> GfDropoutRule:
+        if self.seed is not None:
+            check_tensor("seed", self.seed, (torch.int64,), device)  # its .data may be another tensor's by now
+            if self.seed._version != self.version:
+                raise RuntimeError("the dropout seed has been modified by an inplace operation between the forward and "
+                                   "its backward")
+            self.rule.seed_ptr = self.seed.data_ptr()
+        return self.rule
 
 
 def make_rule(p: float, seed, site: int, device) -> GfDropoutRule:

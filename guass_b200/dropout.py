@@ -34,13 +34,13 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, site):
         rule = _block.make_rule(p, seed, site, x.device)
-        ctx.kept, ctx.p, ctx.site = _block.KeptSeed(seed), p, site
+        ctx.kept = _block.KeptRule(rule, seed)
         return _run(x, rule, residual)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        rule = _block.make_rule(ctx.p, ctx.kept.get(), ctx.site, dy.device)
+        rule = ctx.kept.get(dy.device)
         dx = _run(dy, rule, None) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 

@@ -70,7 +70,7 @@ class _GatedFeedForward(torch.autograd.Function):
         rule = _block.make_rule(p, seed, site, x.device)
         y, h = _forward(x, w_in, w_out, b_in, b_out, activation, rule, need[2])
         ctx.save_for_backward(x, w_in, w_out, b_in, h)
-        ctx.activation, ctx.kept, ctx.p, ctx.site = activation, _block.KeptSeed(seed), p, site
+        ctx.activation, ctx.kept = activation, _block.KeptRule(rule, seed)
         return y
 
     @staticmethod
@@ -82,8 +82,7 @@ class _GatedFeedForward(torch.autograd.Function):
         w_in, w_out = _block.rows_of(w_in, d), _block.rows_of(w_out, hidden)
         b_in = None if b_in is None else b_in.contiguous()
         L = _block.lib()
-        rule = _block.make_rule(ctx.p, ctx.kept.get(), ctx.site, dy.device)
-        f = _describe(x, w_in, w_out, b_in, None, ctx.activation, rule)
+        f = _describe(x, w_in, w_out, b_in, None, ctx.activation, ctx.kept.get(dy.device))
         f.dy, f.ld_dy = dy.data_ptr(), _block.ld(dy)
         if h is not None:
             f.h = h.data_ptr()

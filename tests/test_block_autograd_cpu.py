@@ -131,3 +131,22 @@ def test_casting_a_model_keeps_8_bit_scales(launches, cast):
     assert model[0] is layer and layer.weight_scale.dtype == torch.float32
     assert torch.equal(layer.weight_scale, scale) and layer.q_weight.dtype == torch.int8
     assert torch.equal(layer.state_dict()["weight_scale"], scale) and layer.bias.dtype != torch.float32
+
+
+@pytest.mark.parametrize("op", ["dropout", "feed_forward"])
+def test_a_seed_whose_memory_moved_is_read_where_it_is(launches, op):
+    """An assignment to .data gives the seed other memory: the backward reads that, never the old address."""
+    seen, _ = launches
+    seed = torch.tensor([5])
+    x = torch.ones(3, 4, requires_grad=True)
+    y = operators()[op](x, seed)
+    seed.data = torch.tensor([5])
+    gc.collect()
+    y.sum().backward()
+    assert seen[-1][1] == 5
+
+
+def test_a_seed_that_left_its_device_is_refused():
+    kept = _block.KeptRule(_block.GfDropoutRule(), torch.tensor([5]))
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        kept.get(torch.device("cuda", 0))
