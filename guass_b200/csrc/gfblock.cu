@@ -331,7 +331,8 @@ struct EpilogueWarp {
   float* vec1;
   const int lane;
   Philox rng;
-  float row_scale = 0.0f;
+  float row_scale = 0.0f;  // INT8: of this lane's row
+  bool far_scale = false;  // and whether any of the warp's could take a sum past fp32's range
 
   __device__ __forceinline__ EpilogueWarp(const GemmParams& p_, char* stage_, char* vectors)
       : p(p_), stage(stage_), vec0(reinterpret_cast<float*>(vectors)), vec1(vec0 + 32), lane(threadIdx.x & 31),
@@ -394,9 +395,18 @@ struct EpilogueWarp {
       fetch_next();
       tc::tmem_wait();
       release();
-      // |sum| < 2^31: one rounding to fp32, then the two scales and the bias
+      // |sum| <= 2^31: one rounding to fp32, then the two scales and the bias;
+      // the smaller scale first where the row's alone could overflow
+      if (!far_scale) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) d[i] = __float_as_uint((float)(int)d[i] * s * vec1[i] + vec0[i]);
+        for (int i = 0; i < 32; ++i) d[i] = __float_as_uint((float)(int)d[i] * s * vec1[i] + vec0[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const bool less = s < vec1[i];
+          d[i] = __float_as_uint((float)(int)d[i] * (less ? s : vec1[i]) * (less ? vec1[i] : s) + vec0[i]);
+        }
+      }
       uint32_t v[16];
       begin();
       if constexpr (std::is_same_v<T, float>) {
@@ -752,6 +762,7 @@ __global__ void __launch_bounds__(Config<EPI>::threads, 1) gemm_kernel(const __g
       if (EPI == EPI_INT8) {
         const int row = m + (int)(threadIdx.x & 31);
         epi.row_scale = row < p.M && GFB_IN_BOUNDS(within(row, p.M)) ? p.a_scale[row] : 0.0f;
+        epi.far_scale = __any_sync(0xFFFFFFFFu, fabsf(epi.row_scale) >= 79228162514264337593543950336.0f);  // 2^96
       }
       typename decltype(epi)::Ahead ahead;
       if (c < c_end) epi.fetch(ahead, t.n0 + c);
