@@ -276,11 +276,11 @@ static_assert(sizeof(Pipe) <= 512, "the room behind the staging blocks");
 // The tiles of one CTA or pair, columns first: with few column tiles a run of
 // consecutive ones, so that its rows of A come from memory once and from L2
 // after that; with many, every units-th, so that all units share the rows of
-// a few row tiles and neighbouring columns at a time.  Measured on the loads
-// alone: 10 column tiles (16384 x 320 x 1280 gated) 21 us in runs and 28
-// interleaved; the whole product with 40 (8 bits, 16384 x 1280 x 10240) 177 us
-// in runs and 162 interleaved.  Going on is an addition: a division would
-// stand in every role's way.
+// a few row tiles and neighbouring columns at a time.  us in runs / interleaved,
+// 8-bit products of 16384 x 1280 with 10 column tiles 45.8 / 48.5, 14 58.1 /
+// 59.3, 16 64.1 / 65.3, 20 83.0 / 83.1, 24 96.5 / 95.5, 40 162.8 / 157.7;
+// feed-forwards of 16384 rows with 10 46.9 / 47.5, 16 68.0 / 69.6, 20 125.3 /
+// 122.7.  Going on is an addition: a division would stand in every role's way.
 constexpr int kRunColumns = 16;
 struct Tile {
   int n, m, split;       // tile coordinates
@@ -1847,13 +1847,22 @@ cudaError_t launch_quantize(int64_t rows, int64_t cols, const void* x, int64_t l
                      cudaStream_t st) {
   const bool vec = aligned_rows(x, rows, ld_x, sizeof(T)) && cols % 8 == 0 && ld_q % 8 == 0 &&
                    (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-  // a warp for a row of up to 2048 values, a CTA for a longer one; aligned rows
-  // of up to 16384 stay in registers
+  // Aligned rows of up to 16384 values stay in registers.  A warp for a short
+  // row, a CTA for a long one (a CTA holds at least 4096, so rows of 1280 leave
+  // most of it idle), and a CTA too where every row can have its own at once.
+  // us for bf16 rows from cold caches, warp / CTA:
+  //   aligned  16384 x 1280  12.0 / 31.7   16384 x 2048  18.1 / 34.1   4736 x 2048  7.1 / 11.1
+  //              592 x 2048   2.8 /  2.7     148 x 2048   2.1 /  1.4     64 x 1280  1.6 /  1.5
+  //   others   16384 x 1001  27.2 / 35.1   16384 x 2047  47.0 / 43.7   4736 x 1537  15.1 / 15.2
+  //             2368 x 333    3.7 /  4.5    1184 x 333    3.6 /  2.8     64 x 1001  5.4 /  2.5
   if (vec && cols <= 512) return launch_quantize<T, 32, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
   if (vec && cols <= 1280) return launch_quantize<T, 32, 5>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (vec && cols <= 2048 && rows > 4 * (int64_t)sms)
+    return launch_quantize<T, 32, 8>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
   if (vec && cols <= 4096) return launch_quantize<T, 256, 2>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
   if (vec && cols <= 16384) return launch_quantize<T, 256, 8>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
-  if (cols <= 2048) return launch_quantize<T, 32, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
+  if (cols <= 1536 && rows > 8 * (int64_t)sms)
+    return launch_quantize<T, 32, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
   return launch_quantize<T, 256, 0>(rows, cols, x, ld_x, q, ld_q, scale, sms, st);
 }
 

@@ -51,3 +51,15 @@ def test_nan_scales_stay_nan_beside_large_ones():
     sb = torch.tensor([1e-7, float("nan")], device="cuda")
     y = int8_matmul(a, sa, a[:2], sb, out_dtype=torch.float32).cpu()
     assert torch.equal(torch.isnan(y), torch.tensor([[True, True], [False, True], [False, True]]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [300, 700, 1300])
+@pytest.mark.parametrize("cols", [333, 512, 1280, 1288, 1536, 1537, 2048, 2056])
+def test_quantised_rows_in_every_variant(rows, cols, dtype):
+    """A warp or a CTA for a row, held or read twice: the same numbers, those of the definition."""
+    x = (torch.randn(rows, cols, generator=torch.Generator().manual_seed(cols)) * 3).to(dtype)
+    x[0], x[rows - 1, cols - 1], x[rows // 2, 0] = 0, float("nan"), float("inf")
+    q, scale = quantize_rows(x.cuda())
+    want, ws = ref.quantise(x)
+    assert torch.equal(q.cpu(), want) and torch.equal(scale.cpu().nan_to_num(nan=-1.0), ws.nan_to_num(nan=-1.0))
