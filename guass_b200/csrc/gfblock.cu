@@ -1585,6 +1585,14 @@ FfPlan plan_ff(const gf_gated_ff& f, gf_pass pass, char* ws) {
   return p;
 }
 
+// every pointer a multiple of its element's size (the kernels access whole elements)
+template <typename... P>
+gf_status check_elements(const char* who, int es, const P*... ptrs) {
+  const uintptr_t all = (reinterpret_cast<uintptr_t>(ptrs) | ...);
+  if (all % es) return fail(GF_ERR_INVALID_ARG, "%s: a pointer is not aligned to its %d-byte elements", who, es);
+  return GF_OK;
+}
+
 gf_status check_ff(const char* who, const gf_gated_ff* f) {
   if (!f) return fail(GF_ERR_INVALID_ARG, "%s: the description must be non-null", who);
   if (f->tokens < 0 || f->in_features <= 0 || f->hidden <= 0 || f->out_features <= 0)
@@ -1595,6 +1603,10 @@ gf_status check_ff(const char* who, const gf_gated_ff* f) {
     return fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_BF16 or GF_F16", who);
   if (f->activation != GF_ACT_GELU && f->activation != GF_ACT_SILU)
     return fail(GF_ERR_INVALID_ARG, "%s: unknown activation", who);
+  if (const gf_status s = check_elements(who, 2, f->x, f->w_in, f->b_in, f->w_out, f->b_out, f->y, f->dy, f->dx, f->dw_in,
+                                         f->db_in, f->dw_out, f->db_out);
+      s != GF_OK)
+    return s;
   if (f->ld_x < f->in_features || f->ld_w_in < f->in_features || f->ld_w_out < f->hidden)
     return fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
   return check_rule(who, f->dropout);
@@ -1882,6 +1894,8 @@ gf_status check_int8(const char* who, const gf_int8_product* p, bool quantised) 
   if (p->k > 131071) return fail(GF_ERR_UNSUPPORTED, "%s: k must be at most 131071 (the sums are 32-bit integers)", who);
   if (!known_dtype(p->dtype)) return fail(GF_ERR_UNSUPPORTED, "%s: dtype must be GF_F32, GF_BF16 or GF_F16", who);
   if (p->reserved != 0) return fail(GF_ERR_INVALID_ARG, "%s: reserved fields must be 0", who);
+  if (const gf_status s = check_elements(who, dtype_size(p->dtype), p->bias, p->out); s != GF_OK) return s;
+  if (const gf_status s = check_elements(who, 4, quantised ? p->a_scale : nullptr, p->b_scale); s != GF_OK) return s;
   if ((quantised && p->ld_a < p->k) || p->ld_b < p->k || p->ld_out < p->n)
     return fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
   return GF_OK;
@@ -2024,6 +2038,7 @@ gf_status gf_dropout(int64_t rows, int64_t cols, int32_t dtype, const gf_dropout
   if (cols > (int64_t(1) << 33) || rows > (int64_t(1) << 62) / cols)
     return gf::fail(GF_ERR_UNSUPPORTED, "%s: more than 2^33 columns or 2^62 elements", who);
   if (!x || !y) return gf::fail(GF_ERR_INVALID_ARG, "%s: x and y must be non-null", who);
+  GFB_TRY(gfb::check_elements(who, gfb::dtype_size(dtype), x, residual, y));
   gfb::Range range("gfblock.dropout");
   const int es = gfb::dtype_size(dtype);
   gfb::DropoutParams p{};
@@ -2054,6 +2069,8 @@ gf_status gf_quantize_rows(int64_t rows, int64_t cols, int32_t dtype, const void
   if (ld_x < cols || ld_q < cols) return gf::fail(GF_ERR_INVALID_ARG, "%s: a leading dimension is smaller than its row", who);
   if (rows == 0) return GF_OK;
   if (!x || !q || !scale) return gf::fail(GF_ERR_INVALID_ARG, "%s: x, q and scale must be non-null", who);
+  GFB_TRY(gfb::check_elements(who, gfb::dtype_size(dtype), x));
+  GFB_TRY(gfb::check_elements(who, 4, scale));
   gfb::Range range("gfblock.quantize_rows");
   return gfb::quantise(rows, cols, dtype, x, ld_x, q, ld_q, scale, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -2094,6 +2111,7 @@ gf_status gf_int8_linear(const gf_int8_product* p, const void* x, int64_t ld_x, 
   if (p->m == 0) return GF_OK;
   if (!x || !p->b || !p->b_scale || !p->out)
     return gf::fail(GF_ERR_INVALID_ARG, "%s: x, b, b_scale and out must be non-null", who);
+  GFB_TRY(gfb::check_elements(who, gfb::dtype_size(x_dtype), x));
   gf_int8_product d = *p;
   const gfb::Quantised q = gfb::place_quantised(d, workspace);
   d.a = q.q;

@@ -11,9 +11,10 @@
  * library's last-error function.  Calls that overlap use different workspaces.
  *
  * Matrices are row-major; a leading dimension counts elements.  They may have
- * any size, alignment and leading dimension: operands whose rows do not start
- * on 16-byte boundaries are first copied into the workspace, which costs one
- * pass over them.
+ * any size and leading dimension and start at any element (a pointer that is
+ * no multiple of its element's size is refused): operands whose rows do not
+ * start on 16-byte boundaries, and a w_in whose hidden size is no multiple of
+ * 64, are first copied into the workspace, which costs one pass over them.
  */
 #ifndef GFBLOCK_H
 #define GFBLOCK_H
