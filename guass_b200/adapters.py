@@ -320,7 +320,8 @@ class BatchedAdapters:
         held in 8 bits (one scale per output channel; the activations are
         quantised per token at each call,
         :class:`guass_b200.int8.Int8Linear`).  The modules keep their base
-        weights; undo with :meth:`unquantize`."""
+        weights, and changes to parameters are not seen; undo with
+        :meth:`unquantize`."""
         from guass_b200.int8 import Int8Linear
 
         if self._int8:

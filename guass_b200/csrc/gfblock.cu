@@ -944,7 +944,7 @@ __global__ void __launch_bounds__(256) align_kernel(const __grid_constant__ Alig
 // same columns in shared memory.  Rows are 16-byte aligned.
 //
 // Up to four tokens: every further one adds its arithmetic on all weights,
-// while the product kernel takes the same time for one token as for 128.
+// while the product kernel takes the same time for one token as for eight.
 // Whole forward from cold caches, us, walk / product kernel:
 //   tokens            1             4             5             8
 //   320 x 1280    6.1 / 12.3    9.0 / 12.7   11.6 / 12.7   13.3 / 12.6
