@@ -399,7 +399,7 @@ class DataParallelTrainer:
         # optional list of (start, end) CUDA events around each step's all-reduce
         self.allreduce_events = None
         # the fused feed-forward's condition bits, looked at without waiting for the device
-        fused = any(getattr(m, "fused_ff", False) for m in model.modules())
+        fused = isinstance(model, nn.Module) and any(getattr(m, "fused_ff", False) for m in model.modules())
         self._flags = _block.FlagWatch(self.params[0].device) if fused and self.params[0].is_cuda else None
         drop = getattr(model, "dropout_seed", None)  # (not every model has dropout)
         if drop is not None:

@@ -91,3 +91,15 @@ def test_a_wait_that_ran_out_stops_the_training(monkeypatch):
     with pytest.raises(RuntimeError, match="0x10"):
         tr.step(inputs)
     assert Library.calls == 2
+
+
+def test_a_model_need_not_be_a_module():
+    class Plain:
+        def __init__(self, model):
+            self.model, self.adapters = model, model.adapters
+
+        def __call__(self, *args):
+            return self.model(*args)
+
+    tr = trainer(Plain(OtherModel()))
+    assert torch.isfinite(tr.step(sd15.synthetic_inputs(sd15.tiny_config(), 1, 3, dtype=torch.float32)))
