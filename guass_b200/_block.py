@@ -125,11 +125,13 @@ class FlagWatch:
     they are reset, so whichever copy arrived last shows them.)"""
 
     def __init__(self, device: torch.device):
-        self.device = device
+        self.there = torch.zeros(1, dtype=torch.int32, device=device)
         self.flags = torch.zeros(1, dtype=torch.int32, pin_memory=True)
 
     def look(self) -> None:
-        call(self.device, lib().gf_block_status_async, self.flags.data_ptr())
+        call(self.there.device, lib().gf_block_status_async, self.there.data_ptr())
+        # (torch's copy: its allocators keep both ends until it has run, this object gone or not)
+        self.flags.copy_(self.there, non_blocking=True)
 
     def check(self) -> None:
         if self.flags[0] != 0:

@@ -2140,9 +2140,11 @@ gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out) {
   return GF_OK;
 }
 
-gf_status gf_block_status_async(uint32_t* pinned_flags_out, gf_stream stream) {
-  if (!pinned_flags_out) return gf::fail(GF_ERR_INVALID_ARG, "gf_block_status_async: pinned_flags_out must be non-null");
-  GFB_CUDA(cudaMemcpyFromSymbolAsync(pinned_flags_out, gfb::g_status, sizeof(uint32_t), 0, cudaMemcpyDeviceToHost,
+gf_status gf_block_status_async(uint32_t* flags_out, gf_stream stream) {
+  const char* who = "gf_block_status_async";
+  if (!flags_out) return gf::fail(GF_ERR_INVALID_ARG, "%s: flags_out must be non-null", who);
+  GFB_TRY(gfb::check_elements(who, 4, flags_out));
+  GFB_CUDA(cudaMemcpyFromSymbolAsync(flags_out, gfb::g_status, sizeof(uint32_t), 0, cudaMemcpyDeviceToDevice,
                                      reinterpret_cast<cudaStream_t>(stream)));
   return GF_OK;
 }

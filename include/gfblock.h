@@ -133,8 +133,8 @@ gf_status gf_int8_linear(const gf_int8_product* p, const void* x, int64_t ld_x, 
 gf_status gf_block_status(gf_stream stream, int reset, uint32_t* flags_out);
 
 /* Enqueues a copy of those bits, as they are once the work before it on
- * `stream` is done, into pinned host memory; does not synchronise. */
-gf_status gf_block_status_async(uint32_t* pinned_flags_out, gf_stream stream);
+ * `stream` is done, into device memory; does not synchronise. */
+gf_status gf_block_status_async(uint32_t* flags_out, gf_stream stream);
 
 #ifdef __cplusplus
 }

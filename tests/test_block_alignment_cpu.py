@@ -50,3 +50,8 @@ def test_8_bit_product(name, off):
         assert refused(L.gf_int8_linear(ctypes.byref(p), FAKE, 16, _lib.GF_BF16, FAKE, 1 << 20, None))
     good = _block.GfInt8Product(**{**d, name: FAKE})
     assert refused(L.gf_int8_linear(ctypes.byref(good), FAKE + 2, 16, _lib.GF_F32, FAKE, 1 << 20, None))
+
+
+def test_status_copy():
+    L = _block.lib()
+    assert refused(L.gf_block_status_async(FAKE + 2, None)) and L.gf_block_status_async(None, None) == BAD
